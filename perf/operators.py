@@ -123,7 +123,8 @@ def _codes(x):
     """Codes 0 to 15, lowest value and step (bfloat16) of every vector of ``x`` [..., D], as the cache has them."""
     x = x.float()
     low = x.amin(-1, keepdim=True).to(torch.bfloat16)
-    step = ((x.amax(-1, keepdim=True) - low.float()) / 15).to(torch.bfloat16)
+    span = x.amax(-1, keepdim=True) - low.float()
+    step = (span / torch.full_like(span, 15)).to(torch.bfloat16)  # by a tensor: by a number is a product with its reciprocal
     at = torch.where(step > 0, (x - low.float()) / step.float(), 0.0)
     return at.round().clamp(0, 15).to(torch.uint8), low[..., 0], step[..., 0]
 
@@ -253,9 +254,10 @@ def run(state):
 def _plain_linear(x, values, scale):
     x = x.float()
     most = x.abs().amax(-1, keepdim=True)
-    by = torch.where(most < 2.0 ** -100, 0.0, 127 / most)  # the quotient stays in float32's range
+    top = torch.full_like(most, 127)  # a tensor: a quotient with a number is a product with a reciprocal
+    by = torch.where(most < 2.0 ** -100, 0.0, top / most)  # the quotient stays in float32's range
     sums = (x * by).round().double() @ values.double().t()  # whole numbers beyond 2^24
-    return sums.float() * (most / 127) * scale
+    return sums.float() * (most / top) * scale
 
 
 def _plain_store(state):
