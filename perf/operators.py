@@ -32,17 +32,17 @@ DEVICE = "cuda:0"
 def listed():
     return [
         # one user's next word: q, k and v of the 4B size, one row
-        _linear("8-bit product, 1 row", 1, 6144, 2560, "bfloat16"),
+        _linear("8-bit product 1 row", 1, 6144, 2560, "bfloat16"),
         # a decoding batch on the 8B size's q, k and v
-        _linear("8-bit product, 24 rows", 24, 6144, 4096, "bfloat16"),
+        _linear("8-bit product 24 rows", 24, 6144, 4096, "bfloat16"),
         # an ordinary prompt, the 4B size's down projection
-        _linear("8-bit product, 2048 rows", 2048, 2560, 9728, "bfloat16"),
+        _linear("8-bit product 2048 rows", 2048, 2560, 9728, "bfloat16"),
         # the 32-bit mode with sizes that no tile divides
-        _linear("8-bit product, 37 rows, float32", 37, 1001, 1100, "float32"),
+        _linear("8-bit product 37 rows float32", 37, 1001, 1100, "float32"),
         # the headline's batch of eight: the feed-forward's first half
-        _gated("gated 8-bit product, 8 rows", 8, 9728, 2560, "bfloat16"),
+        _gated("gated 8-bit product 8 rows", 8, 9728, 2560, "bfloat16"),
         # a prompt of 1,999 tokens through it
-        _gated("gated 8-bit product, 1999 rows", 1999, 9728, 2560, "bfloat16"),
+        _gated("gated 8-bit product 1999 rows", 1999, 9728, 2560, "bfloat16"),
         # eight requests store their next token
         _store("store 8 tokens", 8, 8, 128, 16, "bfloat16"),
         # a prompt's portion goes into the cache
@@ -54,7 +54,7 @@ def listed():
         # an ordinary prompt read in at once
         _attend("read 2048", 1, 2048, 2048, 2048, 32, 8, 128, 16, 0, "bfloat16"),
         # the 32-bit mode: short portions, a window, small pages
-        _attend("portions of 7 in a window, float32", 5, 7, 40, 700, 6, 2, 32, 8, 64, "float32"),
+        _attend("portions of 7 in a window float32", 5, 7, 40, 700, 6, 2, 32, 8, 64, "float32"),
     ]
 
 
