@@ -68,9 +68,19 @@ __device__ __forceinline__ void gated_act4(const float (&g)[4], const float (&u)
   else gated_act4_of<false>(g, u, limit, o);
 }
 
-// WM x WN waves, each with BM / WM rows and BN / WN columns of the tile, S stages in flight.
-template <int BM, int BN, int WM, int WN, int S>
+// What a tile multiplies: 16 bytes of an operand a lane, and four sums of 16 x 16.
+struct BfloatProducts {
+  typedef bf16x8_t Operand;
+  typedef f32x4_t Sums;
+  static __device__ __forceinline__ Sums add(Operand w, Operand a, Sums c) { return __builtin_amdgcn_mfma_f32_16x16x32_bf16(w, a, c, 0, 0, 0); }
+};
+
+// WM x WN waves, each with BM / WM rows and BN / WN columns of the tile, S stages in flight. A stage is 128 bytes of every
+// row whatever their type: 64 columns of bfloat16, 128 of 8-bit integers (PRODUCTS).
+template <int BM, int BN, int WM, int WN, int S, class PRODUCTS = BfloatProducts>
 struct Tile {
+  typedef typename PRODUCTS::Operand Operand;
+  typedef typename PRODUCTS::Sums Sums;
   static constexpr int WAVES = WM * WN, TM = BM / WM / 16, TN = BN / WN / 16;
   static constexpr int AU = BM / 8, WU = BN / 8;  // units of a stage; where they are no multiple of the waves, the last is loaded twice
   static constexpr int AL = (AU + WAVES - 1) / WAVES, WL = (WU + WAVES - 1) / WAVES, LOADS = AL + WL;
@@ -127,7 +137,7 @@ struct Tile {
   template <int POLICY = 0>
   static __device__ __forceinline__ void products(const __amdgpu_buffer_rsrc_t a_buf, const __amdgpu_buffer_rsrc_t w_buf,
                                                   const unsigned (&aoff)[AL], const unsigned (&woff)[WL], int s0, int stages,
-                                                  unsigned char* lds, int fetched, f32x4_t (&acc)[TM][TN]) {
+                                                  unsigned char* lds, int fetched, Sums (&acc)[TM][TN]) {
     const int lane = threadIdx.x & 63, wave = uniform_wave_number();
     const int wm = wave / WN, wn = wave % WN, r16 = lane & 15, quad = lane >> 4;
     auto stage_at = [&](int it) { return (s0 + it) * 128; };
@@ -135,19 +145,19 @@ struct Tile {
 #pragma unroll
     for (int i = 0; i < TM; ++i)
 #pragma unroll
-      for (int j = 0; j < TN; ++j) acc[i][j] = (f32x4_t){0.f, 0.f, 0.f, 0.f};
+      for (int j = 0; j < TN; ++j) acc[i][j] = (Sums){0, 0, 0, 0};
     const int read_at[2] = {r16 * 128 + 16 * (quad ^ (r16 & 7)), r16 * 128 + 16 * ((4 + quad) ^ (r16 & 7))};
     const int a_at = wm * (BM / WM) * 128, w_at = (BM + wn * (BN / WN)) * 128;
-    bf16x8_t a[2][TM], w[2][TN];
+    Operand a[2][TM], w[2][TN];
     constexpr int READS = TM + TN;
     auto read_one = [&](int slot, int h, int r) {  // operand r of k-step h: first the weights', then the activations'
       const unsigned char* src = lds + slot * STAGE + read_at[h];
-      if (r < TN) w[h][r] = *(const bf16x8_t*)(src + w_at + r * 2048);
-      else a[h][r - TN] = *(const bf16x8_t*)(src + a_at + (r - TN) * 2048);
+      if (r < TN) w[h][r] = *(const Operand*)(src + w_at + r * 2048);
+      else a[h][r - TN] = *(const Operand*)(src + a_at + (r - TN) * 2048);
     };
     auto row_of_products = [&](int h, int i) {
 #pragma unroll
-      for (int j = 0; j < TN; ++j) acc[i][j] = __builtin_amdgcn_mfma_f32_16x16x32_bf16(w[h][j], a[h][i], acc[i][j], 0, 0, 0);
+      for (int j = 0; j < TN; ++j) acc[i][j] = PRODUCTS::add(w[h][j], a[h][i], acc[i][j]);
     };
     // operands of the next k-step asked for behind each row of products, none behind the last
     constexpr int READS_A_ROW = TM > 1 ? (READS + TM - 2) / (TM - 1) : READS;

@@ -27,6 +27,7 @@ import numpy as np
 import torch
 
 from . import build
+from .int8 import MOST_WIDTH as INT8_MOST_WIDTH, Int8Weight
 
 F32, BF16 = 0, 1
 _CODE = {torch.float32: F32, torch.bfloat16: BF16}
@@ -1351,6 +1352,9 @@ class HipOps:
 
     # ---- matrix products -------------------------------------------------------
     def linear(self, x, w, out_f32=False):
+        """``x @ w.T``. ``w`` may be an ``Int8Weight``: the rows of ``x`` are then quantised one by one."""
+        if isinstance(w, Int8Weight):
+            return self._int8_product(x, w, out_f32)
         if isinstance(x, ScaledRows):
             out = None if out_f32 else self._scaled_product(x, w)
             return self.linear(x.made(), w, out_f32) if out is None else out
@@ -1533,11 +1537,13 @@ class HipOps:
         return None
 
     def linear_for_residual(self, x, w):
-        """``linear(x, w)`` for a result that is only ever added to the residual stream.
+        """``linear(x, w)`` for a result that is only ever added to the residual stream (of an ``Int8Weight`` in float32).
 
         May return the result in planes ``[P, T, N]`` float32 whose sum it is (``add_rmsnorm``
         adds them): a product with few rows and few weight rows then cuts K over several blocks
         per row tile, which fills the chip (160 row tiles for 256 compute units at the 4B size)."""
+        if isinstance(w, Int8Weight):
+            return self._int8_product(x, w, out_f32=True)
         m, k = x.shape
         n = w.shape[0]
         if (self.residual_planes and x.dtype == torch.float32 and w.dtype == torch.float32 and w.shape == (n, k)
@@ -1575,6 +1581,8 @@ class HipOps:
         """``linear_for_residual(x, w)`` for a result that goes to ``add_rmsnorm`` and nowhere else: up to 16 rows of
         bfloat16 come as a ``PendingProduct``. What it takes to make those: whole pairs of k-steps, a residual whose columns
         256 blocks share at up to 16 each, and that the next product can read in pairs of k-steps."""
+        if isinstance(w, Int8Weight):
+            return self.linear_for_residual(x, w)
         (m, k), n = x.shape, w.shape[0]
         if (m <= 16 and x.dtype == torch.bfloat16 and w.dtype == torch.bfloat16 and w.shape[1] == k and k % 64 == 0 and k > 0 and n % 64 == 0
                 and 256 <= n <= 4096 and (x.data_ptr() | w.data_ptr()) % 16 == 0):
@@ -1627,10 +1635,68 @@ class HipOps:
         return max(1, min(8, 256 // blocks, (k // 32) // 12))
 
 
+    # ---- products of 8-bit integers ----------------------------------------------
+    def quantize_rows(self, x):
+        """``(codes, scale)`` of the rows of ``x`` [T, K], bfloat16 or float32: int8 [T, width], K padded with zeros to a multiple of 128,
+        and float32 [T] with ``x = codes * scale`` up to rounding."""
+        if x.dim() != 2 or x.dtype not in _CODE or not 0 < x.shape[1] <= INT8_MOST_WIDTH:
+            raise OpsError(f"quantize_rows: rows of bfloat16 or float32 of up to {INT8_MOST_WIDTH} columns, not {tuple(x.shape)} of {x.dtype}")
+        _need(x, "x")
+        m, k = x.shape
+        width = -(-k // 128) * 128
+        codes = torch.empty((m, width), dtype=torch.int8, device=x.device)
+        scale = torch.empty((m,), dtype=torch.float32, device=x.device)
+        self._check(self.lib, self.lib.qrt_quantize_rows(_ptr(x), c_int(_CODE[x.dtype]), _ptr(codes), _ptr(scale), c_int(m), c_int(k),
+                                                         c_int(width), _stream()))
+        return codes, scale
+
+    # rows up to which a product of 8-bit integers streams the weight past them; more go by tiles
+    int8_max_rows = 64
+
+    def _int8_product(self, x, w, out_f32=False, gate=None):
+        """The product of rows by an ``Int8Weight``; ``gate`` = (activation, limit): gate rows, then up rows, and the activation of the two."""
+        if isinstance(x, ScaledRows):
+            x = x.made()
+        if x.dim() != 2 or x.dtype not in _CODE or x.shape[1] != w.shape[1]:
+            raise OpsError(f"linear: x is {tuple(x.shape)} of {x.dtype}, the weight in 8 bits is {tuple(w.shape)}")
+        _need(x, "x")
+        _need(w.values, "weight", torch.int8, (w.shape[0], w.width))
+        _need(w.scale, "weight's scales", torch.float32, (w.shape[0],))
+        if x.device != w.device:
+            raise OpsError(f"linear: x is on {x.device}, the weight on {w.device}")
+        (m, k), n, act, limit = x.shape, w.shape[0], -1, 0.0
+        if gate is not None:
+            act, limit = ACTIVATIONS[gate[0]], gate[1]
+            if act > ACTIVATIONS["clamped"] or n % 2:
+                raise OpsError(f"gated_linear: {gate[0]} of a weight {tuple(w.shape)}")
+            n //= 2
+        out = torch.empty((m, n), dtype=torch.float32 if out_f32 else x.dtype, device=x.device)
+        if m == 0:
+            return out
+        if self.lib.qrt_int8_rows_fuses(c_int(m), c_int(k), c_int(w.width)) and x.data_ptr() % 16 == 0:
+            rows, codes, scale = x, None, None
+        else:
+            rows, (codes, scale) = None, self.quantize_rows(x)
+        if m <= self.int8_max_rows:
+            self._check(self.lib, self.lib.qrt_int8_rows(
+                _ptr(rows), c_int(_CODE[x.dtype]), _ptr(codes), _ptr(scale), _ptr(w.values), _ptr(w.scale), _ptr(out), c_int(_CODE[out.dtype]),
+                c_int(m), c_int(n), c_int(k), c_int(w.width), c_int(act), c_float(limit), _stream()))
+        else:
+            # 128 columns of bytes are a stage, as 64 of bfloat16 are: the same bytes and the same cycles of the matrix cores
+            tile = self.choose_tile(m, n, w.width // 2, "gated" if gate is not None else "whole")[0]
+            self._check(self.lib, self.lib.qrt_int8_tiles(
+                _ptr(codes), _ptr(scale), _ptr(w.values), _ptr(w.scale), _ptr(out), c_int(_CODE[out.dtype]), c_int(m), c_int(n), c_int(w.width),
+                c_int(tile), c_int(act), c_float(limit), _stream()))
+        return out
+
     def gated_linear(self, x, w_gate_up, activation="swiglu", limit=0.0, row_scale=None):
         """``gated_act(linear(x, w_gate_up), ...)`` with ``w_gate_up`` [2I, K], gate rows first. With few
         rows one kernel forms both halves and applies the activation in its epilogue,
-        so the [T, 2I] intermediate never reaches memory."""
+        so the [T, 2I] intermediate never reaches memory. ``w_gate_up`` may be an ``Int8Weight``."""
+        if isinstance(w_gate_up, Int8Weight):
+            if row_scale is not None:
+                raise OpsError("gated_linear: no factors per row beside a weight in 8 bits")
+            return self._int8_product(x, w_gate_up, gate=(activation, limit))
         m, k = x.shape
         two_i, kw = w_gate_up.shape
         if k != kw or two_i % 2:

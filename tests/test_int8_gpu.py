@@ -1,0 +1,236 @@
+"""Products of weights in 8-bit integers against the same sums in 64 bits, and what they refuse."""
+
+import pytest
+import torch
+
+from qwen3_runtime_amd.ops import Int8Weight
+
+DEV = "cuda:0"
+gpu = pytest.mark.gpu
+
+
+def rnd(*shape, seed=0, dtype=torch.float32, device=DEV):
+    return torch.randn(*shape, generator=torch.Generator().manual_seed(seed)).to(dtype).to(device)
+
+
+def codes_of(x):
+    """Codes and scales of rows by the definition: 127 / the largest magnitude, and the product with it, in float32."""
+    most = x.float().abs().amax(-1)
+    top = torch.full_like(most, 127)  # a tensor: a quotient with a number is a product with its reciprocal
+    by = torch.where(most < 2.0 ** -100, 0.0, top / most)
+    return (x.float() * by[:, None]).round(), most / top
+
+
+def product(x, w):
+    q, s = codes_of(x)
+    return (q.double() @ w.values[:, : w.shape[1]].double().t()) * s.double()[:, None] * w.scale.double()
+
+
+def ops():
+    from qwen3_runtime_amd.ops.hip import HipOps
+
+    return HipOps()
+
+
+# Sum and scales in float32: the sum of whole numbers is rounded to 24 bits once, two products round once each: 3 * 2^-24. A result in
+# bfloat16 is rounded once more, by 2^-8 of it at most.
+STEP = {torch.float32: 3.2 * 2.0 ** -24, torch.bfloat16: 2.0 ** -8 * 1.001}
+
+
+def near(got, want, dtype, what=""):
+    off = (got.double() - want).abs() - STEP[dtype] * want.abs()
+    assert got.dtype == dtype and float(off.max()) <= 1e-30, f"{what} {float(off.max())}"
+
+
+ROWS = [1, 2, 3, 4, 5, 8, 9, 16, 17, 32, 33, 48, 49, 64, 65, 130, 257]
+
+
+@gpu
+@pytest.mark.parametrize("k", [1, 7, 128, 136, 1100, 2560, 9728])
+@pytest.mark.parametrize("dtype", [torch.bfloat16, torch.float32])
+def test_codes_of_rows(k, dtype):
+    x = rnd(9, k, seed=k, dtype=dtype)
+    x[1] = 0
+    x[2] *= 1e-33
+    x[3, -1] = -1000
+    got, scale = ops().quantize_rows(x)
+    q, s = codes_of(x)
+    assert got.shape[1] % 128 == 0 and torch.equal(got[:, :k].float(), q) and not got[:, k:].any()
+    assert torch.equal(scale, s)
+
+
+@gpu
+@pytest.mark.parametrize("m", ROWS)
+@pytest.mark.parametrize("n,k", [(5, 1), (16, 128), (96, 272), (333, 1100), (1000, 640)])
+@pytest.mark.parametrize("dtype", [torch.bfloat16, torch.float32])
+def test_products(m, n, k, dtype):
+    x, w = rnd(m, k, seed=m, dtype=dtype), Int8Weight.quantize(rnd(n, k, seed=n))
+    near(ops().linear(x, w), product(x, w), dtype)
+    near(ops().linear(x, w, out_f32=True), product(x, w), torch.float32)
+    near(ops().linear_for_residual(x, w), product(x, w), torch.float32)
+
+
+@gpu
+@pytest.mark.parametrize("m,n,k", [(1, 6144, 2560), (8, 2560, 9728), (16, 2560, 4096), (24, 6144, 4096), (40, 2560, 4096), (64, 1024, 9728), (300, 2560, 9728), (2047, 6144, 2560)])
+def test_products_of_a_models_sizes(m, n, k):
+    x, w = rnd(m, k, seed=m, dtype=torch.bfloat16), Int8Weight.quantize(rnd(n, k, seed=n))
+    near(ops().linear(x, w), product(x, w), torch.bfloat16)
+
+
+@gpu
+@pytest.mark.parametrize("tile", range(14))
+@pytest.mark.parametrize("gated", [False, True])
+@pytest.mark.parametrize("n", [304, 301])
+def test_every_tile(tile, gated, n, monkeypatch):
+    o = ops()
+    monkeypatch.setattr(type(o), "choose_tile", staticmethod(lambda *a: (tile, 1)))
+    m, k = 270, 650
+    x, w = rnd(m, k, seed=1, dtype=torch.bfloat16), Int8Weight.quantize(rnd(2 * n if gated else n, k, seed=2) / 25)
+    for dtype in (torch.bfloat16, torch.float32):
+        x = x.to(dtype)
+        if gated:
+            near_gated(o.gated_linear(x, w), x, w, dtype)
+        else:
+            near(o.linear(x, w), product(x, w), dtype)
+
+
+def near_gated(got, x, w, dtype, activation="swiglu", limit=0.0):
+    """Gate and up values are off by 3 * 2^-24 of themselves; the activation's slope is at most 1.1 and its own
+    evaluation off by some 5 * 2^-24 of it, x * sigmoid(x) by |x| times that of the sigmoid's argument: (8 + 2 |gate|) * 2^-24."""
+    y = product(x, w)
+    g, u = y.chunk(2, -1)
+    if activation == "clamped":
+        g, u = g.clamp(max=limit), u.clamp(-limit, limit) + 1
+        want, per = g * torch.sigmoid(1.702 * g) * u, (12 + 4 * g.abs()) * 2.0 ** -24
+    else:
+        want, per = g * torch.sigmoid(g) * u, (12 + 4 * g.abs()) * 2.0 ** -24
+    off = (got.double() - want).abs() - want.abs() * (per + (2.0 ** -8 * 1.001 if dtype == torch.bfloat16 else 0.0))
+    if activation == "clamped":  # up + 1 may cancel: up's own error counts whole
+        off -= 4 * 2.0 ** -24 * (g.abs() * (u.abs() + 1))
+    assert got.dtype == dtype and float(off.max()) <= 1e-30, float(off.max())
+
+
+@gpu
+@pytest.mark.parametrize("m", ROWS)
+@pytest.mark.parametrize("n,k", [(5, 3), (64, 128), (333, 1100), (1000, 640)])
+@pytest.mark.parametrize("dtype", [torch.bfloat16, torch.float32])
+def test_gated_products(m, n, k, dtype):
+    x, w = rnd(m, k, seed=m, dtype=dtype), Int8Weight.quantize(rnd(2 * n, k, seed=n) * k ** -0.5)
+    near_gated(ops().gated_linear(x, w), x, w, dtype)
+    near_gated(ops().gated_linear(x, w, "clamped", 1.5), x, w, dtype, "clamped", 1.5)
+
+
+@gpu
+@pytest.mark.parametrize("m", [3, 20, 100])
+@pytest.mark.parametrize("bad", [float("nan"), float("inf"), float("-inf")])
+def test_rows_that_are_not_finite_are_nan_and_leave_the_others(m, bad):
+    x, w = rnd(m, 640, seed=3, dtype=torch.bfloat16), Int8Weight.quantize(rnd(96, 640, seed=4))
+    x[0] = 0
+    want = ops().linear(x, w)
+    assert not want[0].any()
+    x[1, 639] = bad
+    got = ops().linear(x, w)
+    assert got[1].isnan().all()
+    keep = torch.arange(m) != 1
+    assert torch.equal(got[keep], want[keep])
+
+
+@gpu
+@pytest.mark.parametrize("m,n,k", [(2, 300, 2560), (24, 300, 1100), (300, 512, 1280)])
+def test_a_captured_product_is_the_eager_one(m, n, k):
+    o = ops()
+    x, w = rnd(m, k, seed=1, dtype=torch.bfloat16), Int8Weight.quantize(rnd(n, k, seed=2))
+    o.linear(x, w), o.gated_linear(x, w)
+    graph = torch.cuda.CUDAGraph()
+    torch.cuda.synchronize()
+    with torch.cuda.graph(graph):
+        y, z = o.linear(x, w), o.gated_linear(x, w)
+    for seed in range(4):
+        x.copy_(rnd(m, k, seed=seed + 7, dtype=torch.bfloat16))
+        graph.replay()
+        torch.cuda.synchronize()
+        assert torch.equal(y, o.linear(x, w)) and torch.equal(z, o.gated_linear(x, w))
+
+
+@gpu
+def test_products_on_another_stream():
+    o, s = ops(), torch.cuda.Stream()
+    x, w = rnd(40, 640, seed=1, dtype=torch.bfloat16), Int8Weight.quantize(rnd(320, 640, seed=2))
+    want = o.linear(x, w)
+    s.wait_stream(torch.cuda.current_stream())
+    with torch.cuda.stream(s):
+        got = o.linear(x, w)
+    s.synchronize()
+    assert torch.equal(got, want)
+
+
+@gpu
+def test_no_rows_and_refusals_on_the_device():
+    from qwen3_runtime_amd.ops import OpsError
+
+    o, w = ops(), Int8Weight.quantize(rnd(30, 640))
+    assert o.linear(rnd(0, 640, dtype=torch.bfloat16), w).shape == (0, 30)
+    assert o.gated_linear(rnd(0, 640), w).shape == (0, 15)
+    for x in (rnd(2, 639), rnd(2, 640, dtype=torch.float16), rnd(2, 1280)[:, ::2], rnd(640)):
+        with pytest.raises(OpsError):
+            o.linear(x, w)
+    with pytest.raises(OpsError):
+        o.gated_linear(rnd(2, 640), Int8Weight.quantize(rnd(31, 640)))
+    with pytest.raises(OpsError):
+        o.gated_linear(rnd(2, 640), w, row_scale=torch.ones(2, device=DEV))
+    with pytest.raises(OpsError):
+        o.gated_linear(rnd(2, 640), w, "relu2")
+
+
+# ---- needs no GPU
+
+
+def test_a_weight_in_8_bits():
+    w = rnd(7, 130, seed=5, device="cpu", dtype=torch.bfloat16)
+    w[3] = 0
+    q = Int8Weight.quantize(w)
+    assert q.shape == (7, 130) and q.width == 256 and q.values.shape == (7, 256) and not q.values[:, 130:].any()
+    assert q.num_bytes == 7 * 256 + 28
+    off = (q.values[:, :130].float() * q.scale[:, None] - w.float()).abs()
+    assert bool((off <= q.scale[:, None] * (0.5 + 1e-4)).all()) and not q.values[3].any()
+    # held as it is where it can be
+    v = torch.ones(4, 256, dtype=torch.int8)
+    assert Int8Weight(v, torch.ones(4)).values is v
+
+
+@pytest.mark.parametrize("values,scale", [
+    (torch.zeros(4, 8), torch.ones(4)), (torch.zeros(4, dtype=torch.int8), torch.ones(4)), (torch.zeros(4, 8, dtype=torch.int8), torch.ones(3)),
+    (torch.zeros(4, 8, dtype=torch.int8), torch.ones(4, dtype=torch.float64)), (torch.zeros(0, 8, dtype=torch.int8), torch.ones(0)),
+    (torch.zeros(1, (1 << 17) + 1, dtype=torch.int8), torch.ones(1))])
+def test_a_weight_in_8_bits_refuses(values, scale):
+    with pytest.raises(ValueError):
+        Int8Weight(values, scale)
+
+
+def test_a_weight_that_is_not_finite_is_refused():
+    w = torch.ones(3, 4)
+    w[1, 2] = float("nan")
+    with pytest.raises(ValueError, match="infinity or a NaN"):
+        Int8Weight.quantize(w)
+    with pytest.raises(ValueError):
+        Int8Weight.quantize(torch.ones(3, 4, dtype=torch.int32))
+
+
+def test_entry_points_refuse_sizes_on_the_host():
+    from ctypes import c_float, c_int, c_void_p
+
+    from qwen3_runtime_amd.ops.hip import HipOps
+
+    lib, p = HipOps().lib, c_void_p(1 << 20)  # not read: the sizes are refused
+    rows = lambda m, n, k, width, act=-1, dtype=1, x=None: lib.qrt_int8_rows(  # noqa: E731
+        x, c_int(1), p, p, p, p, p, c_int(dtype), c_int(m), c_int(n), c_int(k), c_int(width), c_int(act), c_float(0), None)
+    for bad in ((65, 16, 128, 128), (1, 0, 128, 128), (1, 16, 128, 100), (1, 16, 200, 128), (1, 16, 0, 128), (1, 16, 1 << 18, 1 << 18), (-1, 16, 128, 128)):
+        assert rows(*bad) != 0
+    assert rows(1, 16, 128, 128, act=2) != 0 and rows(1, 16, 128, 128, dtype=2) != 0 and rows(16, 16, 9728, 9728, x=p) != 0
+    tiles = lambda m, n, width, tile=0, act=-1, dtype=1: lib.qrt_int8_tiles(  # noqa: E731
+        p, p, p, p, p, c_int(dtype), c_int(m), c_int(n), c_int(width), c_int(tile), c_int(act), c_float(0), None)
+    for bad in ((1, 16, 100), (1, 0, 128), (-1, 16, 128), (1 << 20, 16, 1 << 13), (1, 16, 128, 14), (1, 16, 128, 0, 2), (1, 16, 128, 0, -1, 2)):
+        assert tiles(*bad) != 0
+    quantize = lambda m, k, width, dtype=1: lib.qrt_quantize_rows(p, c_int(dtype), p, p, c_int(m), c_int(k), c_int(width), None)  # noqa: E731
+    for bad in ((1, 129, 128), (1, 0, 128), (-1, 128, 128), (1, 128, 136), (1, 128, 128, 2)):
+        assert quantize(*bad) != 0
