@@ -18,7 +18,7 @@ Device layout of a paged cache: one tensor per ``PagedStream`` of its spec,
 ``[page, head, offset, width]`` or, transposed, ``[page, head, width, offset]``.
 Keys and values (``"paged_kv"``) are the streams ``k`` and ``v``, the values
 transposed inside a page, so that the attention kernels read keys-contiguous
-operands for both products; a mixer that keeps something else per token (values of
+operands for both products (in 4 bits the streams ``k``, ``v`` and ``steps`` of csrc/cache4.h); a mixer that keeps something else per token (values of
 another width than its keys, one latent vector) names its own streams.
 """
 
@@ -86,6 +86,8 @@ class CacheManager:
         by_key: dict[tuple, _Group] = {}
         for cid, spec in enumerate(self.specs):
             if spec.paged:
+                if spec.bits is not None and self.page_size % 4:
+                    raise ValueError(f"a cache of 4 bits has pages of a multiple of 4 tokens, not {self.page_size}")
                 key = spec.group_key()
                 if key not in by_key:
                     by_key[key] = _Group(key, spec, [], PagePool(num_pages), self.page_size, spec.window, spec.chunk,
@@ -102,7 +104,7 @@ class CacheManager:
             for g in self.groups:
                 g.storage = [
                     torch.zeros((len(g.cache_ids), g.pool.num_pages, stream.elements_per_token() * self.page_size),
-                                dtype=dtype, device=self.device)
+                                dtype=dtype if stream.dtype == "model" else getattr(torch, stream.dtype), device=self.device)
                     for stream in g.spec.page_streams()
                 ]
 
@@ -114,7 +116,7 @@ class CacheManager:
         4B shape, bfloat16, 16 tokens: 2*36*8*128*2*16 = 2,359,296
         (reference: qwen3_runtime/engine/memory.py:8-14).
         """
-        return sum(s.elements_per_token() * page_size * dtype_bytes for s in specs if s.paged)
+        return sum(s.bytes_per_token(dtype_bytes) * page_size for s in specs if s.paged)
 
     def bytes_read(self, kv_lens: Sequence[int], dtype_bytes: int | None = None) -> int:
         """Bytes of cache a step has to read for requests that hold ``kv_lens`` tokens: every
@@ -125,7 +127,7 @@ class CacheManager:
         for spec in self.specs:
             if spec.paged:
                 seen = sum(self._visible(spec, n) for n in kv_lens)
-                total += seen * spec.elements_per_token() * width
+                total += seen * spec.bytes_per_token(width)
         for state in self._state_of_cache.values():
             total += len(kv_lens) * state[0].numel() * state.element_size()
         return total

@@ -1,0 +1,507 @@
+// Attention over a paged cache of 4 bits (cache4.h), for one head size (QRT_HEAD_DIM).
+//
+// Scores are formed transposed, S^T = K Q^T, and outputs O^T = V^T P^T, on the bfloat16 MFMA of 16 x 16 x 32. A code n is put under an
+// exponent by a mask and an or, OFF + n exactly, two at a time, and what that adds is taken out again behind the sums:
+//   score = step * (sum q (OFF + n)) + (lo - OFF step) * sum q
+//   out   = sum w (OFF + n) + sum (p (lo + 8 step) - (OFF + 8) w),  w = p * step rounded as it is multiplied,
+// so that w's rounding multiplies n - 8 alone. Keys and values of 16 keys are D / 8 neighbouring bytes a lane: no operand crosses
+// lanes and nothing goes through LDS. A block of 32 keys is on its way while another is multiplied, its page numbers one block before that.
+//
+// bfloat16 queries: OFF = 128, weights w in bfloat16 (their errors average out, as in every attention that multiplies
+// probabilities in 16 bits). float32 queries: q and w as three bfloat16 each (24 bits in all, whole), OFF = 16, which leaves three more bits
+// of a sum to what is wanted.
+//
+// KEYS: up to 16 rows (token x head of the group); the four waves of a block take its blocks of keys in turn and meet in LDS. Otherwise a
+// wave has 16 RT rows of its own, and the four of a block read the same keys at about the same time. Either way a launch may cut the
+// keys into pieces of one length, which a second kernel joins. Sums, maxima and outputs are float32.
+#include "common.h"
+#include "cache4.h"
+
+constexpr int D = QRT_HEAD_DIM;
+static_assert(D % 32 == 0 && D >= 32 && D <= 256, "heads of 32 to 256 in steps of 32");
+constexpr int KS = D / 32;  // steps of 32 elements: words a lane holds of 16 keys, and of 16 values
+constexpr float LOG2E = 1.4426950408889634f;
+
+struct Attention4Args {
+  const void* q;
+  void* out;
+  const uint8_t* k;
+  const uint8_t* v;
+  const unsigned* steps;
+  const int* cu_q;
+  const int* kv_lens;
+  const int* table;
+  const int* tile_seq;   // null: tile i is sequence i from its first row
+  const int* tile_row0;  // null: from the first row
+  float* part_o;         // [rows, pieces, D], not divided by the sums
+  float* part_ml;        // [rows, pieces, 2]
+  const int* merge_tokens;  // null: all
+  int num_merge_tokens;
+  int table_width, num_tiles, num_pages, num_seqs, nq, nkv, page_size;
+  int window, chunk, keep_first, sink;
+  float scale, softcap;
+  int piece, pieces;  // blocks of 32 keys in a piece; how many pieces the launch has room for
+};
+
+// The blocks of 32 keys that rows [base, base + rows_of_tile) of a sequence see: first those of the kept first tokens, then a run.
+struct Blocks {
+  int kept, first, count;
+  __device__ __forceinline__ int at(int i) const { return i < kept ? i : first + i - kept; }
+};
+__device__ __forceinline__ int lowest_seen(const Attention4Args& a, int pos) {
+  if (a.window) return max(0, pos - a.window + 1);
+  return a.chunk ? pos - pos % a.chunk : 0;
+}
+__device__ __forceinline__ Blocks blocks_of(const Attention4Args& a, int base, int tile_rows, int rows, int g, int before) {
+  const int last = before + (min(base + tile_rows, rows) - 1) / g;
+  const int low = lowest_seen(a, before + base / g);
+  Blocks b;
+  b.first = low >> 5;
+  b.kept = min((a.keep_first + 31) >> 5, b.first);
+  b.count = b.kept + (last >> 5) + 1 - b.first;
+  return b;
+}
+
+template <int N>
+struct Words {
+  unsigned w[N];
+};
+template <int N>
+__device__ __forceinline__ Words<N> load_words(const void* p) {
+  Words<N> r;
+  __builtin_memcpy(&r, __builtin_assume_aligned(p, N % 4 == 0 ? 16 : N % 2 == 0 ? 8 : 4), sizeof(r));
+  return r;
+}
+
+struct Stage {
+  Words<KS> k[2], v[2];
+  Words<8> s[2];
+};
+struct Pages {
+  int k[2], g[2];
+};
+
+template <int OFF>
+__device__ __forceinline__ unsigned place(unsigned x, int nibble) {  // nibbles `nibble` and `nibble` + 4 of x as a pair of bfloat16
+  if constexpr (OFF == 128) return ((x >> (4 * nibble)) & 0x000f000fu) | 0x43004300u;
+  else return ((nibble == 0 ? x << 3 : x >> (4 * nibble - 3)) & 0x00780078u) | 0x41804180u;
+}
+
+template <int RT, int NS, bool KEYS>
+struct Walk {
+  static constexpr int OFF = NS == 1 ? 128 : 16;
+  bf16x8_t q[NS][RT][KS];
+  float qsum[RT], m[RT], l[RT], c[RT];
+  int pos[RT], low[RT];
+  f32x4_t acc[RT][2 * KS];
+
+  template <typename T>
+  __device__ __forceinline__ void load_queries(const Attention4Args& a, int head, int g, int q0, int base, int rows, int before, int lane) {
+    const int quad = lane >> 4;
+#pragma unroll
+    for (int t = 0; t < RT; ++t) {
+      const int r = min(base + 16 * t + (lane & 15), rows - 1);
+      pos[t] = before + r / g;
+      low[t] = lowest_seen(a, pos[t]);
+      const T* src = (const T*)a.q + ((size_t)(q0 + r / g) * a.nq + head * g + r % g) * D + quad * (D / 4);
+      float sum = 0.f;
+#pragma unroll
+      for (int s = 0; s < KS; ++s) {
+        float x[8];
+        if constexpr (sizeof(T) == 2) {
+          const bf16x8_t y = *(const bf16x8_t*)(src + 8 * s);
+#pragma unroll
+          for (int e = 0; e < 8; ++e) x[e] = (float)y[e];
+        } else {
+          const f32x4_t y = *(const f32x4_t*)(src + 8 * s), z = *(const f32x4_t*)(src + 8 * s + 4);
+#pragma unroll
+          for (int e = 0; e < 4; ++e) x[e] = y[e], x[4 + e] = z[e];
+        }
+#pragma unroll
+        for (int e = 0; e < 8; ++e) {
+          sum += x[e];
+          float rest = x[e];
+#pragma unroll
+          for (int n = 0; n < NS; ++n) {  // in the order in which codes leave their word: 0 and 4, 1 and 5, ...
+            const bf16_t part = (bf16_t)rest;
+            q[n][t][s][e < 4 ? 2 * e : 2 * (e - 4) + 1] = part;
+            rest -= (float)part;
+          }
+        }
+      }
+      sum += __shfl_xor(sum, 16);
+      sum += __shfl_xor(sum, 32);
+      qsum[t] = sum;
+      m[t] = -INFINITY, l[t] = 0.f, c[t] = 0.f;
+#pragma unroll
+      for (int d = 0; d < 2 * KS; ++d) acc[t][d] = (f32x4_t){0.f, 0.f, 0.f, 0.f};
+    }
+  }
+
+  // One block of 32 keys. `inside`: every row of the wave sees all of it.
+  __device__ __forceinline__ void block(const Attention4Args& a, const Stage& st, int b, bool inside, int lane) {
+    const int quad = lane >> 4;
+    f32x4_t sc[RT][2];
+#pragma unroll
+    for (int t = 0; t < RT; ++t)
+#pragma unroll
+      for (int h = 0; h < 2; ++h) sc[t][h] = (f32x4_t){0.f, 0.f, 0.f, 0.f};
+#pragma unroll
+    for (int h = 0; h < 2; ++h)
+#pragma unroll
+      for (int s = 0; s < KS; ++s) {
+        const unsigned x = st.k[h].w[s];
+        const u32x4_t w = {place<OFF>(x, 0), place<OFF>(x, 1), place<OFF>(x, 2), place<OFF>(x, 3)};
+#pragma unroll
+        for (int t = 0; t < RT; ++t)
+#pragma unroll
+          for (int n = 0; n < NS; ++n)
+            sc[t][h] = __builtin_amdgcn_mfma_f32_16x16x32_bf16(__builtin_bit_cast(bf16x8_t, w), q[n][t][s], sc[t][h], 0, 0, 0);
+      }
+    // scores in units of log2, of rows lane & 15 and keys 16 h + 4 quad + r
+    const float unit = a.softcap > 0.f ? a.scale : a.scale * LOG2E;
+    float kmul[2][4], kadd[2][4], vstep[2][4], vmid[2][4];
+#pragma unroll
+    for (int h = 0; h < 2; ++h)
+#pragma unroll
+      for (int r = 0; r < 4; ++r) {
+        const unsigned x = st.s[h].w[2 * r], y = st.s[h].w[2 * r + 1];
+        const float kstep = __uint_as_float(x & 0xffff0000u);
+        kmul[h][r] = kstep * unit;
+        kadd[h][r] = fmaf(-(float)OFF, kstep, __uint_as_float(x << 16)) * unit;
+        vstep[h][r] = __uint_as_float(y & 0xffff0000u);
+        vmid[h][r] = fmaf(8.f, vstep[h][r], __uint_as_float(y << 16));
+      }
+#pragma unroll
+    for (int t = 0; t < RT; ++t)
+#pragma unroll
+      for (int h = 0; h < 2; ++h)
+#pragma unroll
+        for (int r = 0; r < 4; ++r) sc[t][h][r] = fmaf(kmul[h][r], sc[t][h][r], kadd[h][r] * qsum[t]);
+    if (a.softcap > 0.f) {
+#pragma unroll
+      for (int t = 0; t < RT; ++t)
+#pragma unroll
+        for (int h = 0; h < 2; ++h)
+#pragma unroll
+          for (int r = 0; r < 4; ++r) sc[t][h][r] = a.softcap * tanhf(sc[t][h][r] / a.softcap) * LOG2E;
+    }
+    auto seen = [&](int t, int h, int r) {
+      const int key = 32 * b + 16 * h + 4 * quad + r;
+      return key <= pos[t] && (key >= low[t] || key < a.keep_first);
+    };
+    if (!inside) {
+#pragma unroll
+      for (int t = 0; t < RT; ++t)
+#pragma unroll
+        for (int h = 0; h < 2; ++h)
+#pragma unroll
+          for (int r = 0; r < 4; ++r) sc[t][h][r] = seen(t, h, r) ? sc[t][h][r] : -INFINITY;
+    }
+    // exponentials are taken against a reference that moves only where a score is above it by more than 2^8
+    float top[RT];
+    bool above = false;
+#pragma unroll
+    for (int t = 0; t < RT; ++t) {
+      top[t] = fmaxf(fmaxf(fmaxf(sc[t][0][0], sc[t][0][1]), fmaxf(sc[t][0][2], sc[t][0][3])),
+                     fmaxf(fmaxf(sc[t][1][0], sc[t][1][1]), fmaxf(sc[t][1][2], sc[t][1][3])));
+      above |= top[t] > m[t] + 8.f;
+    }
+    if (__builtin_amdgcn_ballot_w64(above) != 0) {
+#pragma unroll
+      for (int t = 0; t < RT; ++t) {
+        float x = fmaxf(top[t], __shfl_xor(top[t], 16));
+        x = fmaxf(x, __shfl_xor(x, 32));
+        const float to = x > m[t] + 8.f ? x : m[t];  // by the row's own scores alone, whatever its neighbours need
+        const float by = to > m[t] ? __builtin_amdgcn_exp2f(m[t] - to) : 1.f;  // 0 where there was nothing yet
+        m[t] = to;
+        l[t] *= by, c[t] *= by;
+#pragma unroll
+        for (int d = 0; d < 2 * KS; ++d) acc[t][d] *= by;
+      }
+    }
+    bf16x8_t p[NS][RT];
+#pragma unroll
+    for (int t = 0; t < RT; ++t) {
+      const float from = m[t] == -INFINITY ? 0.f : m[t];
+#pragma unroll
+      for (int h = 0; h < 2; ++h)
+#pragma unroll
+        for (int r = 0; r < 4; ++r) {
+          const float e = __builtin_amdgcn_exp2f(sc[t][h][r] - from);
+          l[t] += e;
+          float w = e * vstep[h][r], mid = vmid[h][r];
+          if (!inside) {  // a value that is not finite touches only rows that see it
+            const bool sees = seen(t, h, r);
+            w = sees ? w : 0.f, mid = sees ? mid : 0.f;
+          }
+          const int slot = 4 * h + (r == 1 ? 2 : r == 2 ? 1 : r);  // codes leave a word of four tokens as 0 and 2, 1 and 3
+          float sum = 0.f, rest = w;
+#pragma unroll
+          for (int n = 0; n < NS; ++n) {
+            const bf16_t part = (bf16_t)rest;
+            p[n][t][slot] = part;
+            rest -= (float)part;
+            sum += (float)part;
+          }
+          c[t] = fmaf(e, mid, fmaf(-(float)(OFF + 8), sum, c[t]));
+        }
+    }
+#pragma unroll
+    for (int w = 0; w < KS; ++w) {
+      const unsigned x = st.v[0].w[w], y = st.v[1].w[w];
+      const u32x4_t lo = {place<OFF>(x, 0), place<OFF>(x, 2), place<OFF>(y, 0), place<OFF>(y, 2)};
+      const u32x4_t hi = {place<OFF>(x, 1), place<OFF>(x, 3), place<OFF>(y, 1), place<OFF>(y, 3)};
+#pragma unroll
+      for (int t = 0; t < RT; ++t)
+#pragma unroll
+        for (int n = 0; n < NS; ++n) {
+          acc[t][2 * w] = __builtin_amdgcn_mfma_f32_16x16x32_bf16(__builtin_bit_cast(bf16x8_t, lo), p[n][t], acc[t][2 * w], 0, 0, 0);
+          acc[t][2 * w + 1] = __builtin_amdgcn_mfma_f32_16x16x32_bf16(__builtin_bit_cast(bf16x8_t, hi), p[n][t], acc[t][2 * w + 1], 0, 0, 0);
+        }
+    }
+  }
+};
+
+template <typename T>
+__device__ __forceinline__ void store_out4(T* to, f32x4_t x) {
+  if constexpr (sizeof(T) == 4) *(f32x4_t*)to = x;
+  else *(bf16x4_t*)to = (bf16x4_t){(bf16_t)x[0], (bf16_t)x[1], (bf16_t)x[2], (bf16_t)x[3]};
+}
+// What divides a row's sums: with a sink, one more term of score 0. `m` in log2, 0 for a row that sees nothing.
+__device__ __forceinline__ float inverse_sum(float m, float l, bool sink) {
+  if (sink) {
+    if (m == -INFINITY) return 0.f;
+    const float top = fmaxf(m, 0.f), by = __builtin_amdgcn_exp2f(m - top);
+    return by / (l * by + __builtin_amdgcn_exp2f(-top));
+  }
+  return l == 0.f ? 0.f : 1.f / l;
+}
+
+// Waves a SIMD holds: two, one where queries and sums alone take most of the registers of that.
+constexpr int residents(int NS) { return NS == 3 && D > 160 ? 1 : 2; }
+
+template <int RT, int NS, bool KEYS, typename T>
+__global__ __launch_bounds__(256, residents(NS)) void attention4_kernel(Attention4Args a, PageMagic magic) {
+  const int lane = threadIdx.x & 63, wave = uniform_wave_number(), quad = lane >> 4;
+  const int tile = blockIdx.x / a.nkv, head = blockIdx.x - tile * a.nkv, piece = blockIdx.y;
+  const int seq = a.tile_seq ? a.tile_seq[tile] : tile, row0 = a.tile_row0 ? a.tile_row0[tile] : 0;
+  const int g = a.nq / a.nkv;
+  const int q0 = a.cu_q[seq], q_len = a.cu_q[seq + 1] - q0, kv_len = a.kv_lens[seq];
+  const int rows = q_len * g, before = kv_len - q_len;
+  constexpr int TILE_ROWS = KEYS ? 16 : 64 * RT;
+  if (row0 >= rows || before < 0) return;
+  const Blocks all = blocks_of(a, row0, TILE_ROWS, rows, g, before);
+  int i0 = piece * a.piece, end = min(all.count, i0 + a.piece);
+  if (i0 >= all.count) return;
+  const int base = KEYS ? row0 : row0 + wave * 16 * RT;
+  const int last_pos = before + (min(base + 16 * RT, rows) - 1) / g, first_pos = before + base / g;
+  if (KEYS) {
+    i0 += wave;
+  } else {
+    if (base >= rows) return;
+    // this wave's own rows may see less than the tile's
+    end = min(end, all.kept + max(0, (last_pos >> 5) + 1 - all.first));
+    const int own_first = all.kept + (lowest_seen(a, first_pos) >> 5) - all.first;
+    if (a.keep_first == 0) i0 = max(i0, own_first);
+  }
+  const int last_low = lowest_seen(a, last_pos);
+  Walk<RT, NS, KEYS> walk;
+  walk.template load_queries<T>(a, head, g, q0, base, rows, before, lane);
+
+  constexpr int STEP = KEYS ? 4 : 1;
+  const int* table = a.table + (size_t)seq * a.table_width;
+  auto block_at = [&](int i) { return all.at(max(0, min(i, all.count - 1))); };  // past the end the last one, not used
+  // A page number from the table, wherever it points, is brought into the pool: given-back pages are masked, but asked for.
+  auto pages = [&](int i) {
+    Pages p;
+    const int b = block_at(i);
+#pragma unroll
+    for (int h = 0; h < 2; ++h) {
+      int page, off;
+      page_of(magic, 32 * b + 16 * h + (lane & 15), page, off);
+      p.k[h] = table[min(page, a.table_width - 1)];
+      page_of(magic, 32 * b + 16 * h + 4 * quad, page, off);
+      p.g[h] = table[min(page, a.table_width - 1)];
+    }
+    return p;
+  };
+  auto load = [&](int i, const Pages& p) {
+    Stage st;
+    const int b = block_at(i);
+#pragma unroll
+    for (int h = 0; h < 2; ++h) {
+      int page, off;
+      page_of(magic, 32 * b + 16 * h + (lane & 15), page, off);
+      const int64_t krow = ((int64_t)max(0, min(p.k[h], a.num_pages - 1)) * a.nkv + head) * a.page_size + off;
+      st.k[h] = load_words<KS>(a.k + krow * (D / 2) + quad * (D / 8));
+      page_of(magic, 32 * b + 16 * h + 4 * quad, page, off);
+      const int64_t grow = ((int64_t)max(0, min(p.g[h], a.num_pages - 1)) * a.nkv + head) * a.page_size + off;
+      st.v[h] = load_words<KS>(a.v + grow * (D / 2) + (lane & 15) * (D / 8));
+      st.s[h] = load_words<8>(a.steps + 2 * grow);
+    }
+    return st;
+  };
+  auto use = [&](const Stage& st, int i) {
+    const int b = block_at(i);
+    const bool inside = 32 * b + 31 <= first_pos && (32 * b >= last_low || 32 * b + 31 < a.keep_first);
+    walk.block(a, st, b, inside, lane);
+  };
+  if (i0 < end) {
+    Pages p0 = pages(i0), p1 = pages(i0 + STEP);
+    Stage s0 = load(i0, p0);
+    p0 = pages(i0 + 2 * STEP);
+    for (int i = i0; i < end; i += 2 * STEP) {
+      Stage s1 = load(i + STEP, p1);
+      p1 = pages(i + 3 * STEP);
+      use(s0, i);
+      if (i + STEP >= end) break;
+      s0 = load(i + 2 * STEP, p0);
+      p0 = pages(i + 4 * STEP);
+      use(s1, i + STEP);
+    }
+  }
+#pragma unroll
+  for (int t = 0; t < RT; ++t) {
+    walk.l[t] += __shfl_xor(walk.l[t], 16), walk.l[t] += __shfl_xor(walk.l[t], 32);
+    walk.c[t] += __shfl_xor(walk.c[t], 16), walk.c[t] += __shfl_xor(walk.c[t], 32);
+  }
+  if constexpr (KEYS) {
+    __shared__ float row_m[4][16], row_l[4][16], row_c[4][16];
+    __shared__ f32x4_t meet[3][2 * KS][64];
+    if (quad == 0) row_m[wave][lane] = walk.m[0], row_l[wave][lane] = walk.l[0], row_c[wave][lane] = walk.c[0];
+    __syncthreads();
+    const int r = lane & 15;
+    const float m = fmaxf(fmaxf(row_m[0][r], row_m[1][r]), fmaxf(row_m[2][r], row_m[3][r]));
+    float l = 0.f, c = 0.f;
+#pragma unroll
+    for (int w = 0; w < 4; ++w) {
+      const float by = row_m[w][r] == -INFINITY ? 0.f : __builtin_amdgcn_exp2f(row_m[w][r] - m);
+      // a wave without a block has no sums; one whose scores are all NaN has sums that are
+      l += row_m[w][r] == -INFINITY ? row_l[w][r] : row_l[w][r] * by;
+      c += row_m[w][r] == -INFINITY ? row_c[w][r] : row_c[w][r] * by;
+      if (w == wave && row_m[w][r] != -INFINITY)
+#pragma unroll
+        for (int d = 0; d < 2 * KS; ++d) walk.acc[0][d] *= by;
+    }
+    if (wave > 0)
+#pragma unroll
+      for (int d = 0; d < 2 * KS; ++d) meet[wave - 1][d][lane] = walk.acc[0][d];
+    __syncthreads();
+    if (wave > 0) return;
+#pragma unroll
+    for (int d = 0; d < 2 * KS; ++d) walk.acc[0][d] += meet[0][d][lane] + (meet[1][d][lane] + meet[2][d][lane]);
+    walk.m[0] = m, walk.l[0] = l, walk.c[0] = c;
+  }
+#pragma unroll
+  for (int t = 0; t < RT; ++t) {
+    const int r = base + 16 * t + (lane & 15);
+    if (r >= rows) continue;
+    const size_t row = (size_t)(q0 + r / g) * a.nq + head * g + r % g;
+    if (a.pieces > 1) {
+      float* to = a.part_o + (row * a.pieces + piece) * D;
+#pragma unroll
+      for (int d = 0; d < 2 * KS; ++d) *(f32x4_t*)(to + 16 * d + 4 * quad) = walk.acc[t][d] + walk.c[t];
+      if (quad == 0) a.part_ml[2 * (row * a.pieces + piece)] = walk.m[t], a.part_ml[2 * (row * a.pieces + piece) + 1] = walk.l[t];
+    } else {
+      const float by = inverse_sum(walk.m[t], walk.l[t], a.sink);
+      T* to = (T*)a.out + row * D;
+#pragma unroll
+      for (int d = 0; d < 2 * KS; ++d) store_out4<T>(to + 16 * d + 4 * quad, (walk.acc[t][d] + walk.c[t]) * by);
+    }
+  }
+}
+
+// The pieces of a row: a wave a row, its elements over the lanes.
+template <typename T>
+__global__ __launch_bounds__(256) void attention4_merge_kernel(Attention4Args a, int tile_rows) {
+  const int lane = threadIdx.x & 63;
+  const int item = blockIdx.x * 4 + uniform_wave_number();
+  const int index = item / a.nq, head = item - index * a.nq;
+  if (index >= a.num_merge_tokens) return;
+  const int token = a.merge_tokens ? a.merge_tokens[index] : index;
+  // the token's sequence: the last one that begins at it or before
+  int lo = 0, hi = a.num_seqs - 1;
+  while (lo < hi) {
+    const int mid = (lo + hi + 1) / 2;
+    if (a.cu_q[mid] <= token) lo = mid;
+    else hi = mid - 1;
+  }
+  const int g = a.nq / a.nkv, q0 = a.cu_q[lo], q_len = a.cu_q[lo + 1] - q0, before = a.kv_lens[lo] - q_len;
+  if (token >= q0 + q_len || before < 0) return;  // behind the last sequence
+  const int r = (token - q0) * g + head % g;
+  const Blocks all = blocks_of(a, r / tile_rows * tile_rows, tile_rows, q_len * g, g, before);
+  const int n = min(a.pieces, (all.count + a.piece - 1) / a.piece);
+  const size_t row = (size_t)token * a.nq + head;
+  const float* ml = a.part_ml + 2 * row * a.pieces;
+  float m = -INFINITY;
+  for (int i = lane; i < n; i += 64) m = fmaxf(m, ml[2 * i]);
+  m = wave_max(m);
+  float l = 0.f;
+  constexpr int E = (D + 63) / 64;
+  float o[E];
+#pragma unroll
+  for (int e = 0; e < E; ++e) o[e] = 0.f;
+  for (int first = 0; first < n; first += 64) {
+    const int i = first + lane;
+    float by = 0.f, part = 0.f;
+    if (i < n) {
+      by = ml[2 * i] == -INFINITY ? (ml[2 * i + 1] == 0.f ? 0.f : 1.f) : __builtin_amdgcn_exp2f(ml[2 * i] - m);  // 1: sums that are NaN
+      part = ml[2 * i + 1] * by;
+    }
+    l += wave_sum(part);
+    const int here = min(64, n - first);
+#pragma unroll 4
+    for (int j = 0; j < here; ++j) {
+      const float w = __shfl(by, j);
+      const float* src = a.part_o + (row * a.pieces + first + j) * D;
+#pragma unroll
+      for (int e = 0; e < E; ++e)
+        if (64 * e + lane < D) o[e] = w == 0.f ? o[e] : fmaf(w, src[64 * e + lane], o[e]);
+    }
+  }
+  const float by = inverse_sum(m, l, a.sink);
+  T* to = (T*)a.out + row * D;
+#pragma unroll
+  for (int e = 0; e < E; ++e)
+    if (64 * e + lane < D) to[64 * e + lane] = from_f32<T>(o[e] * by);
+}
+
+template <int RT, int NS, bool KEYS, typename T>
+static int launch(const Attention4Args& a, hipStream_t stream) {
+  attention4_kernel<RT, NS, KEYS, T><<<dim3(a.num_tiles * a.nkv, a.pieces), 256, 0, stream>>>(a, page_magic(a.page_size));
+  QRT_LAUNCH_CHECK("attention4");
+  if (a.pieces > 1) {
+    const int64_t items = (int64_t)a.num_merge_tokens * a.nq;
+    attention4_merge_kernel<T><<<(unsigned)((items + 3) / 4), 256, 0, stream>>>(a, KEYS ? 16 : 64 * RT);
+    QRT_LAUNCH_CHECK("attention4 (merge)");
+  }
+  return 0;
+}
+
+// keys: tiles of up to 16 rows, the waves of a block share its keys; otherwise tiles of 64 row_tiles rows.
+extern "C" int qrt_attention4(const Attention4Args* args, int dtype, int keys, int row_tiles, hipStream_t stream) {
+  const Attention4Args& a = *args;
+  QRT_CHECK(dtype == QRT_BF16 || dtype == QRT_F32, "attention4: unknown dtype %d", dtype);
+  QRT_CHECK(a.nq > 0 && a.nkv > 0 && a.nq % a.nkv == 0, "attention4: %d query heads on %d key heads", a.nq, a.nkv);
+  QRT_CHECK(a.page_size >= 4 && a.page_size % 4 == 0 && a.num_pages > 0 && a.table_width > 0, "attention4: pages of a multiple of 4 tokens, not %d", a.page_size);
+  QRT_CHECK(a.window >= 0 && a.chunk >= 0 && a.keep_first >= 0 && !(a.window && a.chunk) && !(a.keep_first && !a.window), "attention4: bad mask");
+  QRT_CHECK(a.piece > 0 && a.pieces > 0 && a.pieces <= 65535, "attention4: bad pieces %d of %d", a.pieces, a.piece);
+  QRT_CHECK(a.pieces == 1 || (a.part_o && a.part_ml && a.num_merge_tokens > 0), "attention4: pieces need room for their parts");
+  QRT_CHECK((a.tile_seq != nullptr) == (a.tile_row0 != nullptr) || keys, "attention4: a list of tiles has sequences and rows");
+  QRT_CHECK(!keys || a.nq / a.nkv <= 16, "attention4: %d rows a token in a tile of 16", a.nq / a.nkv);
+  QRT_CHECK((int64_t)a.num_tiles * a.nkv < (1ll << 31), "attention4: too many tiles");
+  QRT_CHECK(((uintptr_t)a.q | (uintptr_t)a.out | (uintptr_t)a.k | (uintptr_t)a.v | (uintptr_t)a.steps) % 16 == 0, "attention4: tensors must begin at multiples of 16 bytes");
+  if (a.num_tiles <= 0) return 0;
+  if (dtype == QRT_F32) {
+    if (keys) return launch<1, 3, true, float>(a, stream);
+    QRT_CHECK(row_tiles == 1, "attention4: float32 rows go by one tile a wave");
+    return launch<1, 3, false, float>(a, stream);
+  }
+  if (keys) return launch<1, 1, true, bf16_t>(a, stream);
+  if (row_tiles == 1) return launch<1, 1, false, bf16_t>(a, stream);
+  if constexpr (D <= 128) {
+    if (row_tiles == 2) return launch<2, 1, false, bf16_t>(a, stream);
+  }
+  return qrt_fail("attention4: no kernel with %d row tiles a wave", row_tiles);
+}

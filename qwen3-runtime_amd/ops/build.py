@@ -1,8 +1,9 @@
 """Compile the HIP sources into shared libraries, in-tree, and find them again.
 
-Two kinds of library of the engine's own: ``core`` (everything whose sizes are
-run-time arguments) and ``attn_bf16_d<D>`` (the MFMA attention kernel, one build
-per head size, ``attn_bf16_d<D>v<DV>`` where values have another size than keys). A part defined elsewhere brings its kernels with
+Three kinds of library of the engine's own: ``core`` (everything whose sizes are
+run-time arguments), ``attn_bf16_d<D>`` (the MFMA attention kernel, one build
+per head size, ``attn_bf16_d<D>v<DV>`` where values have another size than keys) and ``attn4_d<D>``
+(attention over a cache of 4 bits). A part defined elsewhere brings its kernels with
 ``register_library(name, sources)`` and loads them with ``ops.hip.load_library``:
 same flags, same cache, same error reporting, no edit here. A library is rebuilt when the hash of its sources and flags changes. The build
 is plain ``hipcc`` for gfx950: seconds per file, no Python headers involved, so
@@ -38,7 +39,7 @@ FLAGS = [
 FLAGS += os.environ.get("QWEN3_RUNTIME_AMD_HIPCC_FLAGS", "").split()
 CORE_SOURCES = ["runtime.hip", "elementwise.hip", "gemm_f32.hip", "gemm_bf16.hip", "gemm_tiles.hip", "gemm_residual.hip", "gemm_even.hip", "attention_f32.hip", "sampling.hip",
                 "streams.hip", "moe.hip", "experts.hip", "delta.hip", "combine.hip", "rotary.hip", "latent.hip", "retention.hip", "jointnorm.hip", "groupnorm.hip",
-                "statespace.hip", "memory.hip", "int8.hip", "int8_tiles.hip"]
+                "statespace.hip", "memory.hip", "int8.hip", "int8_tiles.hip", "cache4.hip"]
 
 
 class BuildError(RuntimeError):
@@ -54,7 +55,7 @@ def register_library(name: str, sources, defines=()) -> None:
     include ``common.h`` of this package, which is on the include path, and then link
     ``runtime.hip`` for ``qrt_fail`` / ``qrt_last_error`` by listing it as ``"runtime.hip"``).
     Registering the same name with the same sources again is allowed."""
-    if name in ("core", "peaks") or name.startswith("attn_bf16_d"):
+    if name in ("core", "peaks") or name.startswith(("attn_bf16_d", "attn4_d")):
         raise BuildError(f"{name!r} is a library of the engine's own")
     paths = [CSRC / s if not Path(s).is_absolute() else Path(s) for s in sources]
     for path in paths:
@@ -109,6 +110,11 @@ def library_spec(name: str) -> tuple[list, list[str]]:
         return ["runtime.hip", "peaks.hip"], []
     if name in _REGISTERED:
         return list(_REGISTERED[name][0]), list(_REGISTERED[name][1])
+    if name.startswith("attn4_d"):
+        d = int(name[len("attn4_d"):])
+        if d % 32 or not 32 <= d <= 256:
+            raise BuildError(f"attention over a cache of 4 bits takes head sizes 32..256 in steps of 32, not {d}")
+        return ["runtime.hip", "attention4.hip"], [f"-DQRT_HEAD_DIM={d}"]
     if name.startswith("attn_bf16_d"):
         # attn_bf16_d<D>, or attn_bf16_d<D>v<DV> where values have another size than keys
         sizes = [int(x) for x in name[len("attn_bf16_d"):].split("v")]
@@ -184,12 +190,12 @@ def build_library(name: str, force: bool = False) -> Path:
 
 def build_all(head_dims=(16, 32, 48, 64, 80, 96, 112, 128, 160, 176, 192, 208, 256, 320, 448, 512),
               value_dims=((16, 48), (32, 16), (32, 80), (64, 16), (64, 32), (64, 128), (80, 48), (128, 64), (256, 16), (320, 64), (64, 320)),
-              force: bool = True) -> list[Path]:
+              cache4_dims=(32, 64, 96, 128, 160, 192, 224, 256), force: bool = True) -> list[Path]:
     """Every library the tests, the smoke run and the measurements load (head sizes above 256 are
     those of latent rows: latent plus turned key part; ``value_dims``: sizes of keys and values where they
     differ). Three libraries at a time."""
     names = ["core", "peaks"] + [f"attn_bf16_d{d}" for d in head_dims] + \
-        [f"attn_bf16_d{d}v{dv}" for d, dv in value_dims] + registered_libraries()
+        [f"attn_bf16_d{d}v{dv}" for d, dv in value_dims] + [f"attn4_d{d}" for d in cache4_dims] + registered_libraries()
     first = build_library(names[0], force=force)  # the one with many sources compiles them side by side itself
     with ThreadPoolExecutor(3) as pool:
         return [first] + list(pool.map(lambda n: build_library(n, force=force), names[1:]))

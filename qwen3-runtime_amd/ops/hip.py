@@ -64,6 +64,17 @@ class _AttnArgs(Structure):
     ]
 
 
+class _Attn4Args(Structure):
+    _fields_ = [
+        ("q", c_void_p), ("out", c_void_p), ("k", c_void_p), ("v", c_void_p), ("steps", c_void_p),
+        ("cu_q", c_void_p), ("kv_lens", c_void_p), ("table", c_void_p), ("tile_seq", c_void_p), ("tile_row0", c_void_p),
+        ("part_o", c_void_p), ("part_ml", c_void_p), ("merge_tokens", c_void_p), ("num_merge_tokens", c_int),
+        ("table_width", c_int), ("num_tiles", c_int), ("num_pages", c_int), ("num_seqs", c_int), ("nq", c_int), ("nkv", c_int),
+        ("page_size", c_int), ("window", c_int), ("chunk", c_int), ("keep_first", c_int), ("sink", c_int),
+        ("scale", c_float), ("softcap", c_float), ("piece", c_int), ("pieces", c_int),
+    ]
+
+
 class _MixNormArgs(Structure):
     _fields_ = [
         ("x_in", c_void_p), ("x_out", c_void_p), ("y", c_void_p), ("mix", c_void_p), ("out_w", c_void_p),
@@ -203,6 +214,16 @@ def attention_library(head_dim: int, value_dim: int | None = None) -> ctypes.CDL
     return _attn[key]
 
 
+_attn4: dict[int, ctypes.CDLL] = {}
+
+
+def attention4_library(head_dim: int) -> ctypes.CDLL:
+    """The attention over a cache of 4 bits, for one head size."""
+    if head_dim not in _attn4:
+        _attn4[head_dim] = _load(f"attn4_d{head_dim}")
+    return _attn4[head_dim]
+
+
 _extra: dict[str, ctypes.CDLL] = {}
 
 
@@ -212,6 +233,11 @@ def load_library(name: str) -> ctypes.CDLL:
     if name not in _extra:
         _extra[name] = _load(name)
     return _extra[name]
+
+
+def _bits(cache) -> int | None:
+    """How many bits the elements of a paged cache of keys and values are held in (None: the model's dtype)."""
+    return getattr(cache.spec, "bits", None)
 
 
 def _ptr(t: torch.Tensor | None):
@@ -1752,9 +1778,13 @@ class HipOps:
         the cache, in one pass over ``qkv``; returns the queries. ``value_turn`` (frequencies, a name for them
         as ``angles_key``): the values turn too, over all their elements, before they are stored. With the step's context given,
         the angles of a long step come from ``rope_table`` (``angles_key`` as there). Values may
-        have ``value_dim`` elements a head; ``extra`` columns behind them are left alone."""
+        have ``value_dim`` elements a head; ``extra`` columns behind them are left alone. Into a cache of 4 bits keys are
+        quantised as they are rounded to ``qkv``'s type."""
         t, width = qkv.shape
         dv = d if value_dim is None else int(value_dim)
+        four = cache is not None and _bits(cache) == 4
+        if four and (dv != d or value_turn is not None):
+            raise OpsError("a cache of 4 bits holds values as wide as keys, not turned")
         _need(qkv, "qkv", shape=(t, (nq + nkv) * d + nkv * dv + extra))
         for name, w in (("q_norm", q_w), ("k_norm", k_w)):
             if w is not None:
@@ -1785,8 +1815,11 @@ class HipOps:
             if ctx is None or value_turn[0].numel() * 2 != dv:
                 raise OpsError(f"turned values of {dv} take the step's context and {dv // 2} frequencies")
             a.v_rope = self.rope_table(ctx, *value_turn).data_ptr()
-        pages = 0
-        if cache is not None:
+        pages, k = 0, None
+        if four:
+            k = torch.empty((t, nkv * d), dtype=qkv.dtype, device=qkv.device)
+            a.k_out, a.nv = k.data_ptr(), 0
+        elif cache is not None:
             pages = self._check_cache(cache, nkv, d, qkv.dtype, dv)
             _need(cache.group.slots, "slots", torch.int32, (t,))
             a.slots, a.k_cache, a.v_cache = _addr(cache.group.slots), _addr(cache.k), _addr(cache.v)
@@ -1794,6 +1827,8 @@ class HipOps:
         else:
             a.nkv = a.nv = 0  # keys and values go nowhere: only queries are needed
         self._qk(a, qkv.dtype, pages)
+        if four:
+            self._store4(k, qkv[:, (nq + nkv) * d: (nq + 2 * nkv) * d], nkv, d, cache)
         return q
 
     def qk_joint_norm_store(self, qk, nq, nkv, d, bias, q_w, k_w, eps, positions, q_temp, values_are_keys, cache):
@@ -1863,10 +1898,33 @@ class HipOps:
         self._qk(a, q.dtype)
         return q_out, k_out
 
+    def _store4(self, k, v, nkv, d, cache):
+        """Keys and values of tokens, rows of ``nkv * d`` with any stride, into a cache of 4 bits."""
+        pages = self._check_cache4(cache, nkv, d)
+        slots = _need(cache.group.slots, "slots", torch.int32, (k.shape[0],))
+        if not (k.device == v.device == cache.k.device == slots.device) or k.dtype not in _CODE:
+            raise OpsError(f"keys {k.dtype} on {k.device}, values on {v.device}, a cache on {cache.k.device}")
+        self._check(self.lib, self.lib.qrt_store4(
+            _ptr(k), _ptr(v), c_int(_CODE[k.dtype]), c_long(k.stride(0)), c_long(v.stride(0)), _ptr(cache.k), _ptr(cache.v),
+            _ptr(cache.pages["steps"]), _ptr(slots), c_long(pages), c_int(k.shape[0]), c_int(nkv), c_int(d), c_int(cache.group.page_size), _stream()))
+
+    @staticmethod
+    def _check_cache4(cache, nkv, d) -> int:
+        ps, pages = cache.group.page_size, cache.k.shape[0]
+        if d % 32 or not 32 <= d <= 256 or ps % 4:
+            raise OpsError(f"a cache of 4 bits has heads of 32 to 256 in steps of 32 and pages of a multiple of 4 tokens, not {d} and {ps}")
+        _need(cache.k, "key cache", torch.uint8, (pages, nkv, ps, d // 2))
+        _need(cache.v, "value cache", torch.uint8, (pages, nkv, ps, d // 2))
+        _need(cache.pages.get("steps", cache.k), "steps of the cache", torch.bfloat16, (pages, nkv, ps, 4))
+        return pages
+
     def kv_store(self, k, v, cache):
+        """``k``, ``v`` [T, heads, D] into their places in the cache."""
         t, nkv, d = k.shape
         _need(k, "k")
         _need(v, "v", k.dtype, (t, nkv, d))
+        if _bits(cache) == 4:
+            return self._store4(k.view(t, nkv * d), v.view(t, nkv * d), nkv, d, cache)
         pages = self._check_cache(cache, nkv, d, k.dtype)
         _need(cache.group.slots, "slots", torch.int32, (t,))
         a = _QkArgs()
@@ -1967,10 +2025,14 @@ class HipOps:
         the query's. Beyond the plain form: a mask of
         chunks instead of a window (``chunk``), a tanh cap on the scaled scores (``softcap``),
         values of ``value_dim`` elements, and a ``gate`` [T, nq * value_dim] (columns of a wider
-        matrix will do) whose sigmoid multiplies the output."""
+        matrix will do) whose sigmoid multiplies the output. Over a cache of 4 bits: without the last three."""
         t = ctx.num_tokens
         dv = d if value_dim is None else int(value_dim)
         _need(q, "q", shape=(t, nq * d))
+        if _bits(cache) == 4:
+            if gate is not None or dv != d or value_turn is not None:
+                raise OpsError("attention over a cache of 4 bits has values as wide as keys, not turned, and no gate")
+            return self._attention4(q, cache, ctx, nq, nkv, d, scale, window or 0, chunk or 0, softcap or 0.0, int(keep_first), bool(sink))
         self._check_cache(cache, nkv, d, q.dtype, dv)
         if gate is not None and (gate.dtype != q.dtype or tuple(gate.shape) != (t, nq * dv) or gate.stride(1) != 1):
             raise OpsError(f"gate {tuple(gate.shape)} {gate.dtype} does not fit {t} tokens of {nq} heads of {dv}")
@@ -2004,6 +2066,108 @@ class HipOps:
             a.num_seqs, a.max_q_len, a.min_q_len = ctx.num_seqs, ctx.max_q_len, min(ctx.q_lens_host, default=0)
             self._check(self.lib, self.lib.qrt_attention_f32(byref(a), _CODE[q.dtype], _stream()))
         return out
+
+    # ---- attention over a cache of 4 bits --------------------------------------------
+    def _attention4(self, q, cache, ctx, nq, nkv, d, scale, window, chunk, softcap, keep_first, sink):
+        """Sequences of at most 16 rows (tokens by heads of a group) go by blocks whose waves share their keys, the others by tiles of rows;
+        a step that has both takes a launch for either."""
+        pages = self._check_cache4(cache, nkv, d)
+        if q.dtype not in _CODE:
+            raise OpsError(f"queries of {q.dtype}; the attention takes bfloat16 and float32")
+        if nq % nkv or not math.isfinite(scale) or softcap < 0:
+            raise OpsError(f"{nq} query heads on {nkv} key heads, scale {scale}, cap {softcap}")
+        if (keep_first and not window) or (window and chunk) or min(window, chunk, keep_first) < 0:
+            raise OpsError("a window, beside which first keys may stay in sight, or a mask of chunks")
+        ps, g, s = cache.group.page_size, nq // nkv, ctx.num_seqs
+        table = _need(cache.group.block_table, "block table", torch.int32)
+        if table.dim() != 2 or table.shape[0] != s:
+            raise OpsError(f"block table {tuple(table.shape)} for {s} sequences")
+        if table.shape[1] * ps < ctx.max_kv_len:
+            raise OpsError(f"block table is {table.shape[1]} pages wide, the longest sequence has {ctx.max_kv_len} tokens")
+        if len(ctx.q_lens_host) != s or sum(ctx.q_lens_host) != ctx.num_tokens:
+            raise OpsError(f"{ctx.num_tokens} tokens in {s} sequences, of lengths {ctx.q_lens_host}")
+        if not (q.device == cache.k.device == table.device):
+            raise OpsError(f"queries on {q.device}, a cache on {cache.k.device}, its table on {table.device}")
+        out = torch.empty((ctx.num_tokens, nq * d), dtype=q.dtype, device=q.device)
+        a = _Attn4Args()
+        a.q, a.out, a.k, a.v, a.steps = q.data_ptr(), out.data_ptr(), cache.k.data_ptr(), cache.v.data_ptr(), cache.pages["steps"].data_ptr()
+        a.cu_q = _need(ctx.cu_q, "cu_q", torch.int32, (s + 1,)).data_ptr()
+        a.kv_lens = _need(ctx.kv_lens, "kv_lens", torch.int32, (s,)).data_ptr()
+        a.table, a.table_width, a.num_pages, a.num_seqs = table.data_ptr(), table.shape[1], pages, s
+        a.nq, a.nkv, a.page_size = nq, nkv, ps
+        a.window, a.chunk, a.keep_first, a.sink, a.scale, a.softcap = window, chunk, keep_first, int(sink), scale, softcap
+        if ctx.num_tokens == 0:
+            return out
+        few = [i for i in range(s) if ctx.q_lens_host[i] * g <= 16]
+        if len(few) == s:
+            self._launch_attention4(a, q, ctx, None, True, d)
+        else:
+            if any(ctx.q_lens_host[i] for i in few):
+                self._launch_attention4(a, q, ctx, few, True, d)
+            self._launch_attention4(a, q, ctx, [i for i in range(s) if ctx.q_lens_host[i] * g > 16], False, d)
+        return out
+
+    @staticmethod
+    def attention4_blocks(kv: int, q_len: int, window: int, chunk: int, keep_first: int) -> int:
+        """Blocks of 32 keys that the last ``q_len`` of ``kv`` tokens see, at most."""
+        if window:
+            return min(-(-kv // 32), -(-(window + q_len) // 32) + 1 + -(-keep_first // 32))
+        if chunk:
+            return min(-(-kv // 32), -(-(chunk + q_len) // 32) + 1)
+        return -(-kv // 32)
+
+    def _launch_attention4(self, a, q, ctx, subset, keys, d):
+        g = a.nq // a.nkv
+        bf = q.dtype == torch.bfloat16
+        seqs = range(ctx.num_seqs) if subset is None else subset
+        q_lens = [ctx.q_lens_host[i] for i in seqs]
+        kv_lens = [ctx.kv_lens_host[i] for i in seqs]
+        row_tiles = 2 if bf and d <= 128 and not keys and max(q_lens) * g > 64 else 1
+        key = ("attn4_plan", g, a.nkv, keys, row_tiles, None if subset is None else tuple(subset))
+        plan = ctx.scratch.get(key)
+        if plan is None:  # the same for every layer of the step
+            tiles = tokens = None
+            n_tiles = ctx.num_seqs
+            if not keys:
+                host, n_tiles = self.plan_tiles(q_lens, kv_lens, g, 64 * row_tiles, a.nkv, seq_ids=list(seqs))
+                tiles = torch.from_numpy(host).to(q.device)
+            elif subset is not None:
+                n_tiles = len(q_lens)
+                tiles = torch.tensor(list(seqs) + [0] * n_tiles, dtype=torch.int32, device=q.device)
+            if subset is not None:  # the tokens of these sequences: where a merge of pieces writes
+                cu = np.concatenate([[0], np.cumsum(ctx.q_lens_host)])
+                tokens = torch.from_numpy(np.concatenate([np.arange(cu[i], cu[i + 1]) for i in seqs]).astype(np.int32)).to(q.device)
+            plan = ctx.scratch[key] = (tiles, n_tiles, tokens)
+        tiles, n_tiles, tokens = plan
+        a.tile_seq = a.tile_row0 = a.merge_tokens = a.part_o = a.part_ml = None
+        if tiles is not None:
+            a.tile_seq, a.tile_row0 = tiles.data_ptr(), tiles.data_ptr() + 4 * n_tiles
+        a.num_tiles = n_tiles
+        a.num_merge_tokens = ctx.num_tokens
+        if tokens is not None:
+            a.merge_tokens, a.num_merge_tokens = tokens.data_ptr(), tokens.numel()
+        # a captured step is launched for its bucket's lengths, and told the lengths of its moment beside
+        lens = (ctx.scratch.get("attn_lens") if subset is None else None) or kv_lens
+        most_q = max(q_lens)
+        most = self.attention4_blocks(max(kv_lens), most_q, a.window, a.chunk, a.keep_first)
+        total = sum(self.attention4_blocks(n, most_q, a.window, a.chunk, a.keep_first) for n in lens)
+        splits = ctx.scratch.get("attn_splits")
+        a.piece = -(-most // splits) if splits else self.choose_attention4_piece(most, total, n_tiles, a.nkv, keys)
+        a.pieces = -(-most // a.piece)
+        if a.pieces > 1:
+            parts = ctx.num_tokens * a.nq * a.pieces
+            room = torch.empty((parts * (d + 2),), dtype=torch.float32, device=q.device)
+            a.part_o, a.part_ml = room.data_ptr(), room.data_ptr() + 4 * parts * d
+        lib = attention4_library(d)
+        self._check(lib, lib.qrt_attention4(byref(a), c_int(_CODE[q.dtype]), c_int(int(keys)), c_int(row_tiles), _stream()))
+
+    @staticmethod
+    def choose_attention4_piece(most: int, total: int, tiles: int, nkv: int, keys: bool) -> int:
+        """Blocks of 32 keys that one block of the launch walks."""
+        if keys:  # about 1,024 blocks of the launch, four waves of each with two blocks of keys or more, 64 pieces at most
+            return max(8, -(-total * nkv // 1024), -(-most // 64))
+        launch = tiles * nkv
+        return most if launch >= 512 else max(16, -(-most // -(-512 // launch)))
 
     resident_blocks = 512  # blocks of the prompt kernels the chip holds at once: 2 on each of 256 CUs
 

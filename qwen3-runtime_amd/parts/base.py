@@ -248,6 +248,7 @@ class CacheView:
     writes: bool = True
     group: GroupView | None = None
     # paged_kv: keys [pages, heads, page_size, D]; values [pages, heads, Dv, page_size]
+    # (in 4 bits bytes, [pages, heads, page_size, D / 2] each, with pages["steps"] beside them)
     k: torch.Tensor | None = None
     v: torch.Tensor | None = None
     # state: [slots, *shape]

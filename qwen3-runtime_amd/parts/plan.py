@@ -48,24 +48,33 @@ class TensorDecl:
     storage: str = "float"
 
 
+_DTYPE_BYTES = {"uint8": 1, "bfloat16": 2, "float32": 4, "int32": 4}
+
+
 @dataclass(frozen=True)
 class PagedStream:
     """One tensor a paged cache keeps for every token: ``heads`` x ``width`` elements.
 
     Within a page the tensor is ``[head, offset, width]``, or, ``transposed``,
     ``[head, width, offset]`` (the tokens of a page contiguous for one element: what a kernel
-    wants that multiplies probabilities over keys with values)."""
+    wants that multiplies probabilities over keys with values). ``dtype`` is a torch dtype name, or ``"model"``
+    for the model's dtype."""
 
     name: str
     heads: int
     width: int
     transposed: bool = False
+    dtype: str = "model"
 
     def page_shape(self, page_size: int) -> tuple[int, int, int]:
         return (self.heads, self.width, page_size) if self.transposed else (self.heads, page_size, self.width)
 
     def elements_per_token(self) -> int:
         return self.heads * self.width
+
+    def bytes_per_token(self, model_bytes: int) -> int:
+        """``model_bytes``: the size of an element of the model's dtype."""
+        return self.elements_per_token() * (model_bytes if self.dtype == "model" else _DTYPE_BYTES[self.dtype])
 
 
 @dataclass(frozen=True)
@@ -78,7 +87,9 @@ class CacheSpec:
     positions, counted from position 0, that the newest token lies in),
     ``heads`` x ``head_dim`` keys and ``heads`` x ``value_dim``
     values (``head_dim`` when None), held in pages; the values transposed within a
-    page. ``kind == "paged"``: any other set of per-token tensors, named by
+    page. With ``bits`` = 4 keys and values are held in 4 bits, as codes (streams ``k`` and ``v``, bytes) between a
+    lowest value and a step for every token and head (stream ``steps``: the key's two, the value's two, bfloat16);
+    csrc/cache4.h says in which order. Heads of 32 to 256 in steps of 32, values as wide as keys. ``kind == "paged"``: any other set of per-token tensors, named by
     ``streams`` (one latent vector per token, say), with the same pages, tables and
     window. ``kind == "state"``: a fixed-size tensor of ``shape`` per request, held
     in a slot; ``dtype`` is a torch dtype name or ``"model"`` for the model's dtype.
@@ -94,8 +105,15 @@ class CacheSpec:
     streams: tuple[PagedStream, ...] = ()
     chunk: int | None = None
     keep_first: int = 0
+    bits: int | None = None
 
     def __post_init__(self) -> None:
+        if self.bits is not None:
+            if self.bits != 4 or self.kind != "paged_kv":
+                raise ValueError(f"a paged cache of keys and values may be held in 4 bits, not {self.kind!r} in {self.bits}")
+            if self.head_dim % 32 or not 32 <= self.head_dim <= 256 or self.value_dim not in (None, self.head_dim):
+                raise ValueError(f"a cache of 4 bits has heads of 32 to 256 in steps of 32 and values of the same size, "
+                                 f"not {self.head_dim} and {self.value_dim}")
         if self.window is not None and self.chunk is not None:
             raise ValueError("a cache keeps a window of keys or a chunk of them, not both")
         if self.keep_first < 0 or (self.keep_first and self.window is None):
@@ -111,6 +129,10 @@ class CacheSpec:
     def page_streams(self) -> tuple[PagedStream, ...]:
         """The per-token tensors of a paged cache; a ``CacheView`` holds one device tensor for each,
         under the stream's name."""
+        if self.bits == 4:
+            return (PagedStream("k", self.heads, self.head_dim // 2, dtype="uint8"),
+                    PagedStream("v", self.heads, self.head_dim // 2, dtype="uint8"),
+                    PagedStream("steps", self.heads, 4, dtype="bfloat16"))
         if self.kind == "paged_kv":
             return (PagedStream("k", self.heads, self.head_dim),
                     PagedStream("v", self.heads, self.head_dim if self.value_dim is None else self.value_dim, True))
@@ -122,6 +144,9 @@ class CacheSpec:
 
     def elements_per_token(self) -> int:
         return sum(s.elements_per_token() for s in self.page_streams())
+
+    def bytes_per_token(self, model_bytes: int) -> int:
+        return sum(s.bytes_per_token(model_bytes) for s in self.page_streams())
 
     def group_key(self) -> tuple:
         """Caches with equal keys share pages' geometry and lifetime, hence a pool."""
