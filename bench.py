@@ -123,6 +123,8 @@ def main() -> int:
     ap.add_argument("--context", type=int, default=None, help="default 8192 (capacity: 32768)")
     ap.add_argument("--layers", type=int, default=None, help="run fewer layers than the configuration has")
     ap.add_argument("--dtype", default="bfloat16", choices=["bfloat16", "float32"])
+    ap.add_argument("--weights", default="model", choices=["model", "int8"], help="int8: projections and dense feed-forwards in 8 bits")
+    ap.add_argument("--cache-bits", type=int, default=None, choices=[4], help="4: keys and values are cached in 4 bits")
     ap.add_argument("--no-graph", action="store_true")
     ap.add_argument("--no-points", action="store_true", help="skip batch 1 / 64 and the prefill measurement")
     ap.add_argument("--no-peaks", action="store_true", help="skip the microbenchmark of the device's own peaks")
@@ -192,7 +194,7 @@ def main() -> int:
     engine = build_engine(
         None, config=raw, seed=20260825, dtype=args.dtype, block_size=page, num_kv_blocks=pages,
         max_num_seqs=max_batch, max_num_batched_tokens=budget, max_model_len=args.context,
-        cuda_graph=not args.no_graph,
+        cuda_graph=not args.no_graph, weights=args.weights, cache_bits=args.cache_bits,
     )
     say(f"model on device in {time.time() - t0:.1f} s, {engine.loaded.weight_bytes / 1e9:.2f} GB of weights, "
         f"{pages} pages")
@@ -376,6 +378,8 @@ def main() -> int:
             "page_size": page,
             "hip_graph": not args.no_graph,
             "parallelism": "single GPU",
+            **({"weights": args.weights} if args.weights != "model" else {}),
+            **({"cache_bits": args.cache_bits} if args.cache_bits else {}),
         },
         "trials": {"windows": trials, "steps_each": steps, "reported": "median window",
                    "ms_per_step": [round(w[0] / steps * 1e3, 4) for w in windows],

@@ -30,6 +30,8 @@ def main(argv=None) -> int:
     ap.add_argument("--cuda-graph", action=argparse.BooleanOptionalAction, default=None,
                     help="replay decode steps from captured (HIP) graphs; default on")
     ap.add_argument("--dtype", default="bfloat16", choices=["bfloat16", "float32"])
+    ap.add_argument("--weights", default="model", choices=["model", "int8"], help="int8: projections and dense feed-forwards in 8 bits")
+    ap.add_argument("--cache-bits", type=int, default=None, choices=[4], help="4: keys and values are cached in 4 bits")
     ap.add_argument("--temperature", type=float, default=0.0)
     ap.add_argument("--top-k", type=int, default=0)
     ap.add_argument("--top-p", type=float, default=1.0)
@@ -62,7 +64,7 @@ def main(argv=None) -> int:
         config=preset_config(args.preset) if args.preset else None, seed=args.seed,
         max_num_seqs=args.max_num_seqs, max_num_batched_tokens=args.max_num_batched_tokens,
         block_size=args.block_size, num_kv_blocks=args.num_kv_blocks, dtype=args.dtype,
-        cuda_graph=args.cuda_graph,
+        cuda_graph=args.cuda_graph, weights=args.weights, cache_bits=args.cache_bits,
     )
     prompt = args.prompt_tokens
     vocab = engine.runner.vocab_size

@@ -10,6 +10,7 @@ from __future__ import annotations
 from dataclasses import dataclass
 
 DTYPES = ("bfloat16", "float32")
+WEIGHTS = ("model", "int8")
 
 
 @dataclass(frozen=True)
@@ -29,6 +30,11 @@ class EngineConfig:
     memory_fraction: float = 0.85
     # replay pure-decode steps from captured HIP graphs
     hip_graph: bool = True
+    # "int8": the projections and dense feed-forwards hold their matrices in 8 bits, a scale for every output channel, and
+    # multiply them by activations quantised token by token
+    weights: str = "model"
+    # 4: keys and values are cached in 4 bits, between a lowest value and a step for every token and head
+    cache_bits: int | None = None
 
     def __post_init__(self) -> None:
         if self.page_size < 1:
@@ -41,5 +47,9 @@ class EngineConfig:
             raise ValueError("max_num_batched_tokens must be positive")
         if self.dtype not in DTYPES:
             raise ValueError(f"dtype must be one of {DTYPES}, got {self.dtype!r}")
+        if self.weights not in WEIGHTS:
+            raise ValueError(f"weights must be one of {WEIGHTS}, got {self.weights!r}")
+        if self.cache_bits not in (None, 4):
+            raise ValueError(f"cache_bits must be 4, or None for the dtype's own, got {self.cache_bits!r}")
         if not 0.0 < self.memory_fraction <= 1.0:
             raise ValueError("memory_fraction must be in (0, 1]")

@@ -18,6 +18,7 @@ from ..cache import CacheManager
 from ..config.engine import EngineConfig
 from ..config.model import read_config_json
 from ..parts.model import DecoderModel
+from ..parts.plan import with_cache_bits
 from ..registry import architecture_for
 from ..weights import SafetensorsSource, load_model
 from .runner import ModelRunner
@@ -34,10 +35,11 @@ class LoadedModel:
     weight_bytes: int
 
 
-def build_model(raw_config: dict) -> tuple[object, DecoderModel]:
+def build_model(raw_config: dict, cache_bits: int | None = None) -> tuple[object, DecoderModel]:
     arch = architecture_for(raw_config)
     cfg = arch.read_config(raw_config)
-    return cfg, DecoderModel(arch.make_plan(cfg))
+    plan = arch.make_plan(cfg)
+    return cfg, DecoderModel(plan if cache_bits is None else with_cache_bits(plan, cache_bits))
 
 
 def pages_for_memory(model: DecoderModel, engine: EngineConfig, dtype: torch.dtype, device) -> int:
@@ -65,7 +67,7 @@ def load(model_dir: str | Path | None, engine: EngineConfig, *, source=None, raw
     device = torch.device(engine.device)
     if raw_config is None:
         raw_config = read_config_json(model_dir)
-    cfg, model = build_model(raw_config)
+    cfg, model = build_model(raw_config, engine.cache_bits)
     if source is None:
         source = SafetensorsSource(model_dir)
     if ops is None:
@@ -74,7 +76,7 @@ def load(model_dir: str | Path | None, engine: EngineConfig, *, source=None, raw
         if device.type != "cuda":
             raise RuntimeError("the engine runs on a GPU only; there is no CPU path")
         ops = HipOps(residual_planes=True)  # parts give its results to norms
-    loader = load_model(model, source, device, dtype, where=f" in {model_dir}" if model_dir else "")
+    loader = load_model(model, source, device, dtype, where=f" in {model_dir}" if model_dir else "", weights=engine.weights)
     num_pages = engine.num_pages or pages_for_memory(model, engine, dtype, device)
     cache = CacheManager(
         model.plan.caches, page_size=engine.page_size, num_pages=num_pages,

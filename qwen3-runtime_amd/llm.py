@@ -53,12 +53,15 @@ def build_engine(
     seed: int = 0,
     norm_jitter: float = 0.0,
     ops=None,
+    weights: str = "model",
+    cache_bits: int | None = None,
 ) -> Engine:
     """Engine over a model folder, or over random weights of ``config`` when the folder is None.
 
     Option names follow the reference's factory (qwen3_runtime/engine/factory.py:110-186):
     ``block_size`` is the page size, ``num_kv_blocks`` the number of pages, ``cuda_graph``
-    switches the replay of decode steps from captured graphs (HIP graphs here).
+    switches the replay of decode steps from captured graphs (HIP graphs here). ``weights="int8"`` holds the
+    projections and dense feed-forwards in 8 bits, ``cache_bits=4`` keys and values in 4 (``EngineConfig``).
     """
     raw = source = None
     if model_dir is None:
@@ -72,6 +75,7 @@ def build_engine(
         page_size=block_size, num_pages=num_kv_blocks, max_num_seqs=max_num_seqs,
         max_num_batched_tokens=max_num_batched_tokens, eos_token_id=eos, dtype=dtype, device=device,
         max_model_len=max_model_len, hip_graph=True if cuda_graph is None else bool(cuda_graph),
+        weights=weights, cache_bits=cache_bits,
     )
     loaded = load(model_dir, engine_cfg, source=source, raw_config=raw, ops=ops)
     return Engine(engine_cfg, loaded)

@@ -39,7 +39,8 @@ are the request's state, kept in its slot); rotation in pairs of neighbours (``n
 ``2i`` of a head's first ``dims`` turns against ``2i + 1``, where the encoding turns ``i`` against
 ``i + dims / 2``: the rows of the query and key projections, with their taps, biases and norm weights, are
 brought into the encoding's order when the weights are placed; queries and keys share the order, and
-neither a score nor a head's norm depends on it). A norm without weights after a rotation is the norm
+neither a score nor a head's norm depends on it); a cache of 4 bits (``cache_bits=4``: keys and values are quantised as
+they are stored, csrc/cache4.h says how, and every query, the token's own among them, reads them so). A norm without weights after a rotation is the norm
 before it: a rotation leaves a head's root mean square as it is.
 """
 
@@ -81,6 +82,7 @@ class GroupedQueryAttention(Mixer):
         value_turn: float | None = None,
         conv: int | None = None,
         neighbour_pairs: bool = False,
+        cache_bits: int | None = None,
         tensors=None,
     ):
         super().__init__(tensors)
@@ -143,12 +145,18 @@ class GroupedQueryAttention(Mixer):
             if self.joint_norm or output_gate or bias:
                 raise NotImplementedError("convolutions behind the projections, with biases, an output gate or a q/k norm "
                                           "over the whole projection")
+        self.cache_bits = None if cache_bits is None else int(cache_bits)
+        if self.cache_bits is not None and (self.joint_norm or output_gate or value_turn is not None or self.value_dim != self.head_dim):
+            raise ValueError("a cache of 4 bits goes without a q/k norm over the whole projection, an output gate, turned values, and "
+                             "values of another size than keys")
         self.row_order = None
         if neighbour_pairs and position is not None:
             if self.position.fused_form != "half" or self.value_turn is not None:
                 raise ValueError("pairs of neighbours are brought into the order of a half rotation of plain queries and keys")
             n = self.position.dims
             self.row_order = torch.tensor([*range(0, n, 2), *range(1, n, 2), *range(n, self.head_dim)], dtype=torch.long)
+
+    int8_products = ("qkv", "o")
 
     @property
     def takes_scaled_rows(self):
@@ -166,7 +174,7 @@ class GroupedQueryAttention(Mixer):
     def cache_spec(self):
         return CacheSpec("paged_kv", heads=self.num_kv_heads, head_dim=self.head_dim, window=self.window,
                          chunk=self.chunk, value_dim=None if self.value_dim == self.head_dim else self.value_dim,
-                         keep_first=self.keep_first)
+                         keep_first=self.keep_first, bits=self.cache_bits)
 
     def cache_specs(self):
         specs = super().cache_specs()

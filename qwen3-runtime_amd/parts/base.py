@@ -81,11 +81,15 @@ class Part:
     # wants every portion of a prompt but the last to be a multiple of it.
     # ``takes_scaled_rows``: a mixer or feed-forward that hands its input to ``ops.linear`` and
     # ``ops.gated_linear`` only may be given rows that lack the factor of their norm. ``before_norm``:
-    # set by a block on the sub-layers whose output it hands to its norms as it is.
+    # set by a block on the sub-layers whose output it hands to its norms as it is. ``int8_products``: the part's attributes that
+    # hold its matrices and go to products of ``ops`` alone, so that they may be weights in 8 bits; all of them or none
+    # (``weights_in_int8``, set as they are loaded).
     graph_capturable = True
     portion_multiple = 1
     takes_scaled_rows = False
     before_norm = False
+    int8_products: tuple[str, ...] = ()
+    weights_in_int8 = False
 
     def __init__(self, tensors: Mapping[str, str] | None = None):
         self.tensor_names: dict[str, str] = dict(tensors or {})
@@ -115,7 +119,8 @@ class Part:
             n = 1
             for dim in decl.shape:
                 n *= dim
-            cost.weight_bytes[decl.file_name] = n * elem_bytes
+            whole = self.weights_in_int8 and decl.init == "matrix" and len(decl.shape) == 2
+            cost.weight_bytes[decl.file_name] = n + 4 * decl.shape[0] if whole else n * elem_bytes  # 8 bits: a scale a row beside
             if decl.init == "matrix" and len(decl.shape) == 2:
                 cost.flop += 2.0 * tokens * n
         return cost

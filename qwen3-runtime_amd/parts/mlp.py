@@ -29,6 +29,8 @@ class SwiGLU(FeedForward):
         self.gate_up = None
         self.down = None
 
+    int8_products = ("gate_up", "down")
+
     @property
     def takes_scaled_rows(self):
         return type(self).forward is SwiGLU.forward
@@ -53,6 +55,8 @@ class SwiGLU(FeedForward):
 @register_part("feed_forward", "act_mlp")
 class ActMLP(FeedForward):
     """``tensors``: ``up``, ``down``."""
+
+    int8_products = ("up", "down")
 
     def __init__(self, hidden_size: int, intermediate_size: int, activation: str = "relu2", tensors=None):
         super().__init__(tensors)

@@ -14,7 +14,7 @@ Parts never see the plan or the configuration; they see only their own
 
 from __future__ import annotations
 
-from dataclasses import dataclass, field
+from dataclasses import dataclass, field, replace
 from typing import Any, Mapping, Sequence
 
 
@@ -228,3 +228,20 @@ class ModelPlan:
                     writers.add(cache)
                 elif cache not in writers:
                     raise ValueError(f"order[{i}] reads cache {cache} before any step writes it")
+
+
+def with_cache_bits(plan: ModelPlan, bits: int) -> ModelPlan:
+    """``plan`` with its caches of keys and values held in ``bits`` bits. State in slots stays as it is; a paged cache of another
+    kind, and a mixer whose attention has no such form, are an error."""
+    paged = {c for c, spec in enumerate(plan.caches) if spec.paged}
+    for c in sorted(paged):
+        if plan.caches[c].kind != "paged_kv":
+            raise ValueError(f"cache {c} holds {[s.name for s in plan.caches[c].page_streams()]} in pages; only keys and values may be held in {bits} bits")
+    caches = [replace(spec, bits=bits) if c in paged else spec for c, spec in enumerate(plan.caches)]
+    readers = {step.layer for step in plan.order if paged.intersection(step.cache_ids())}
+    layers = [replace(layer, mixer=replace(layer.mixer, args={**layer.mixer.args, "cache_bits": bits})) if i in readers else layer
+              for i, layer in enumerate(plan.layers)]
+    for i in sorted(readers):
+        if plan.layers[i].mixer.kind != "gqa_attention":
+            raise ValueError(f"layer {i}'s mixer {plan.layers[i].mixer.kind!r} does not read a cache of {bits} bits")
+    return replace(plan, caches=caches, layers=layers)

@@ -23,6 +23,7 @@ from typing import Sequence
 
 import torch
 
+from ..ops.int8 import Int8Weight
 from ..parts.plan import TensorDecl
 
 
@@ -87,6 +88,7 @@ class WeightLoader:
         self.device = torch.device(device)
         self.dtype = dtype
         self._cache: dict[tuple, torch.Tensor] = {}
+        self._int8: dict[tuple, Int8Weight] = {}
         self.num_bytes = 0
 
     def _placed_dtype(self, stored: torch.dtype) -> torch.dtype:
@@ -136,9 +138,37 @@ class WeightLoader:
         return tensor.to(self.device).contiguous()
 
 
-def load_model(model, source, device, dtype, where: str = "") -> WeightLoader:
-    """Check ``source`` against ``model``'s declarations, then load every part."""
+    def quantize(self, part) -> None:
+        """The matrices that ``part`` has just loaded in 8 bits in their place, one after the other (``Part.int8_products``)."""
+        for name in part.int8_products:
+            w = getattr(part, name)
+            key = next((k for k, t in self._cache.items() if t is w), None)
+            made = self._int8.get(key)
+            if made is None:
+                try:
+                    made = Int8Weight.quantize(w)
+                except ValueError as exc:
+                    raise ValueError(f"{name} of {sorted(part.tensor_names.values())}: {exc}") from None
+                self.num_bytes += made.num_bytes
+            if key is not None:  # a part that asks for the same matrix shares its 8-bit form; the floats are not held beside it
+                self._int8[key] = made
+                del self._cache[key]
+                self.num_bytes -= w.numel() * w.element_size()
+            setattr(part, name, made)
+        part.weights_in_int8 = bool(part.int8_products)
+
+
+def load_model(model, source, device, dtype, where: str = "", weights: str = "model") -> WeightLoader:
+    """Check ``source`` against ``model``'s declarations, then load every part. ``weights="int8"``: the matrices of parts that have a
+    form for it (attention's projections, dense feed-forwards) are held in 8 bits; embeddings, heads and everything else as they are."""
+    if weights not in ("model", "int8"):
+        raise ValueError(f"weights are held as the model has them or in 'int8', not {weights!r}")
     check_source(source, model.tensor_decls(), model.plan.ignorable, where)
     loader = WeightLoader(source, device, dtype)
-    model.load(loader)
+    if weights == "model":
+        model.load(loader)
+        return loader
+    for part in model.parts():
+        part.load(loader)
+        loader.quantize(part)
     return loader

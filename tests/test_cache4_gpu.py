@@ -280,6 +280,7 @@ def test_pages_named_in_the_table_that_are_not_in_the_pool_are_not_read_beyond_i
 
 
 @gpu
+@torch.inference_mode()
 def test_a_captured_step_is_the_eager_one():
     """Store and attention in one graph, replayed as the sequences grow; two graphs, one after the other."""
     o, nq, nkv, d, ps = ops(), 8, 2, 128, 16

@@ -136,6 +136,7 @@ def test_rows_that_are_not_finite_are_nan_and_leave_the_others(m, bad):
 
 
 @gpu
+@torch.inference_mode()
 @pytest.mark.parametrize("m,n,k", [(2, 300, 2560), (24, 300, 1100), (300, 512, 1280)])
 def test_a_captured_product_is_the_eager_one(m, n, k):
     o = ops()
