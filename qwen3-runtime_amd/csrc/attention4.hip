@@ -20,6 +20,7 @@
 constexpr int D = QRT_HEAD_DIM;
 static_assert(D % 32 == 0 && D >= 32 && D <= 256, "heads of 32 to 256 in steps of 32");
 constexpr int KS = D / 32;  // steps of 32 elements: words a lane holds of 16 keys, and of 16 values
+typedef float f32x2_t __attribute__((ext_vector_type(2)));
 constexpr float LOG2E = 1.4426950408889634f;
 
 struct Attention4Args {
@@ -81,22 +82,46 @@ struct Pages {
   int k[2], g[2];
 };
 
+// Nibbles `nibble` and `nibble` + 4 of x as a pair of bfloat16, OFF + n each. Mask and exponent are kept in registers where the compiler
+// does not see their values: it then takes one instruction, v_and_or_b32, for what two with literals would do.
 template <int OFF>
-__device__ __forceinline__ unsigned place(unsigned x, int nibble) {  // nibbles `nibble` and `nibble` + 4 of x as a pair of bfloat16
-  if constexpr (OFF == 128) return ((x >> (4 * nibble)) & 0x000f000fu) | 0x43004300u;
-  else return ((nibble == 0 ? x << 3 : x >> (4 * nibble - 3)) & 0x00780078u) | 0x41804180u;
-}
+struct Place {
+  unsigned mask, exponent;
+  __device__ __forceinline__ Place() {
+    if constexpr (OFF == 128) {
+      asm("s_mov_b32 %0, 0x000f000f" : "=s"(mask));
+      asm("v_mov_b32 %0, 0x43004300" : "=v"(exponent));
+    } else {
+      asm("s_mov_b32 %0, 0x00780078" : "=s"(mask));
+      asm("v_mov_b32 %0, 0x41804180" : "=v"(exponent));
+    }
+  }
+  __device__ __forceinline__ unsigned operator()(unsigned x, int nibble) const {
+    const unsigned y = OFF == 128 ? x >> (4 * nibble) : nibble == 0 ? x << 3 : x >> (4 * nibble - 3);
+    return (y & mask) | exponent;
+  }
+};
 
-template <int RT, int NS, bool KEYS>
+// lo + by * step of a pair of bfloat16, in float32
+template <int BY>
+__device__ __forceinline__ float lo_plus(unsigned pair) {
+  return fmaf((float)BY, __uint_as_float(pair & 0xffff0000u), __uint_as_float(pair << 16));
+}
+constexpr float NOTHING = -3.4028235e38f;  // the reference of a row that has seen no key
+
+template <int RT, int NS, bool CAP>
 struct Walk {
   static constexpr int OFF = NS == 1 ? 128 : 16;
+  Place<OFF> place;
   bf16x8_t q[NS][RT][KS];
-  float qsum[RT], m[RT], l[RT], c[RT];
+  float qsum[RT];              // sum of the row's query, times the unit of the scores
+  float ref[RT];               // what exponents are taken against, in log2
+  float l[RT], c[RT];          // this lane's part of sum e, and of sum e (lo + 8 step)
   int pos[RT], low[RT];
-  f32x4_t acc[RT][2 * KS];
+  f32x4_t acc[RT][2 * KS], weights[RT];  // sum w (OFF + n); sum w, four times the same
 
   template <typename T>
-  __device__ __forceinline__ void load_queries(const Attention4Args& a, int head, int g, int q0, int base, int rows, int before, int lane) {
+  __device__ __forceinline__ void load_queries(const Attention4Args& a, float unit, int head, int g, int q0, int base, int rows, int before, int lane) {
     const int quad = lane >> 4;
 #pragma unroll
     for (int t = 0; t < RT; ++t) {
@@ -131,15 +156,16 @@ struct Walk {
       }
       sum += __shfl_xor(sum, 16);
       sum += __shfl_xor(sum, 32);
-      qsum[t] = sum;
-      m[t] = -INFINITY, l[t] = 0.f, c[t] = 0.f;
+      qsum[t] = sum * unit;
+      ref[t] = NOTHING, l[t] = 0.f, c[t] = 0.f;
+      weights[t] = (f32x4_t){0.f, 0.f, 0.f, 0.f};
 #pragma unroll
       for (int d = 0; d < 2 * KS; ++d) acc[t][d] = (f32x4_t){0.f, 0.f, 0.f, 0.f};
     }
   }
 
-  // One block of 32 keys. `inside`: every row of the wave sees all of it.
-  __device__ __forceinline__ void block(const Attention4Args& a, const Stage& st, int b, bool inside, int lane) {
+  // One block of 32 keys. `inside`: every row of the wave sees all of it. `unit`: of the scores, log2 but with a cap.
+  __device__ __forceinline__ void block(const Attention4Args& a, float unit, const Stage& st, int b, bool inside, int lane) {
     const int quad = lane >> 4;
     f32x4_t sc[RT][2];
 #pragma unroll
@@ -147,111 +173,133 @@ struct Walk {
 #pragma unroll
       for (int h = 0; h < 2; ++h) sc[t][h] = (f32x4_t){0.f, 0.f, 0.f, 0.f};
 #pragma unroll
-    for (int h = 0; h < 2; ++h)
+    for (int s = 0; s < KS; ++s)
 #pragma unroll
-      for (int s = 0; s < KS; ++s) {
+      for (int h = 0; h < 2; ++h) {
         const unsigned x = st.k[h].w[s];
-        const u32x4_t w = {place<OFF>(x, 0), place<OFF>(x, 1), place<OFF>(x, 2), place<OFF>(x, 3)};
+        const u32x4_t w = {place(x, 0), place(x, 1), place(x, 2), place(x, 3)};
 #pragma unroll
         for (int t = 0; t < RT; ++t)
 #pragma unroll
           for (int n = 0; n < NS; ++n)
             sc[t][h] = __builtin_amdgcn_mfma_f32_16x16x32_bf16(__builtin_bit_cast(bf16x8_t, w), q[n][t][s], sc[t][h], 0, 0, 0);
       }
-    // scores in units of log2, of rows lane & 15 and keys 16 h + 4 quad + r
-    const float unit = a.softcap > 0.f ? a.scale : a.scale * LOG2E;
-    float kmul[2][4], kadd[2][4], vstep[2][4], vmid[2][4];
+    // of rows lane & 15 and keys 16 h + 4 quad + r: score = kmul * sc + kadd * qsum
+    float kmul[2][4], kadd[2][4];
 #pragma unroll
     for (int h = 0; h < 2; ++h)
 #pragma unroll
       for (int r = 0; r < 4; ++r) {
-        const unsigned x = st.s[h].w[2 * r], y = st.s[h].w[2 * r + 1];
-        const float kstep = __uint_as_float(x & 0xffff0000u);
-        kmul[h][r] = kstep * unit;
-        kadd[h][r] = fmaf(-(float)OFF, kstep, __uint_as_float(x << 16)) * unit;
-        vstep[h][r] = __uint_as_float(y & 0xffff0000u);
-        vmid[h][r] = fmaf(8.f, vstep[h][r], __uint_as_float(y << 16));
+        const unsigned x = st.s[h].w[2 * r];
+        kmul[h][r] = __uint_as_float(x & 0xffff0000u) * unit;
+        kadd[h][r] = lo_plus<-OFF>(x);
       }
+    auto score = [&](int t, int h, int r) {
+      const float x = fmaf(kmul[h][r], sc[t][h][r], kadd[h][r] * qsum[t]);
+      return CAP ? a.softcap * tanhf(x / a.softcap) * LOG2E : x;
+    };
+    auto against = [&](int t, int h, int r) {  // the score less the reference
+      return CAP ? score(t, h, r) - ref[t] : fmaf(kmul[h][r], sc[t][h][r], fmaf(kadd[h][r], qsum[t], -ref[t]));
+    };
+    // exponents against the reference, which moves only where a score is above it by more than 8
+    float ex[RT][2][4];
 #pragma unroll
     for (int t = 0; t < RT; ++t)
 #pragma unroll
       for (int h = 0; h < 2; ++h)
 #pragma unroll
-        for (int r = 0; r < 4; ++r) sc[t][h][r] = fmaf(kmul[h][r], sc[t][h][r], kadd[h][r] * qsum[t]);
-    if (a.softcap > 0.f) {
-#pragma unroll
-      for (int t = 0; t < RT; ++t)
-#pragma unroll
-        for (int h = 0; h < 2; ++h)
-#pragma unroll
-          for (int r = 0; r < 4; ++r) sc[t][h][r] = a.softcap * tanhf(sc[t][h][r] / a.softcap) * LOG2E;
-    }
-    auto seen = [&](int t, int h, int r) {
-      const int key = 32 * b + 16 * h + 4 * quad + r;
-      return key <= pos[t] && (key >= low[t] || key < a.keep_first);
-    };
+        for (int r = 0; r < 4; ++r) ex[t][h][r] = against(t, h, r);
     if (!inside) {
 #pragma unroll
       for (int t = 0; t < RT; ++t)
 #pragma unroll
         for (int h = 0; h < 2; ++h)
 #pragma unroll
-          for (int r = 0; r < 4; ++r) sc[t][h][r] = seen(t, h, r) ? sc[t][h][r] : -INFINITY;
+          for (int r = 0; r < 4; ++r) {
+            const int key = 32 * b + 16 * h + 4 * quad + r;
+            const bool sees = key <= pos[t] && (key >= low[t] || key < a.keep_first);
+            ex[t][h][r] = sees ? ex[t][h][r] : -INFINITY;
+          }
     }
-    // exponentials are taken against a reference that moves only where a score is above it by more than 2^8
-    float top[RT];
     bool above = false;
 #pragma unroll
     for (int t = 0; t < RT; ++t) {
-      top[t] = fmaxf(fmaxf(fmaxf(sc[t][0][0], sc[t][0][1]), fmaxf(sc[t][0][2], sc[t][0][3])),
-                     fmaxf(fmaxf(sc[t][1][0], sc[t][1][1]), fmaxf(sc[t][1][2], sc[t][1][3])));
-      above |= top[t] > m[t] + 8.f;
+      const float top = fmaxf(fmaxf(fmaxf(ex[t][0][0], ex[t][0][1]), fmaxf(ex[t][0][2], ex[t][0][3])),
+                              fmaxf(fmaxf(ex[t][1][0], ex[t][1][1]), fmaxf(ex[t][1][2], ex[t][1][3])));
+      above |= top > 8.f;
     }
     if (__builtin_amdgcn_ballot_w64(above) != 0) {
 #pragma unroll
       for (int t = 0; t < RT; ++t) {
-        float x = fmaxf(top[t], __shfl_xor(top[t], 16));
+        float x = -INFINITY;  // the row's highest score, from all four quarters of its keys
+#pragma unroll
+        for (int h = 0; h < 2; ++h)
+#pragma unroll
+          for (int r = 0; r < 4; ++r) x = fmaxf(x, ex[t][h][r] == -INFINITY ? -INFINITY : score(t, h, r));
+        x = fmaxf(x, __shfl_xor(x, 16));
         x = fmaxf(x, __shfl_xor(x, 32));
-        const float to = x > m[t] + 8.f ? x : m[t];  // by the row's own scores alone, whatever its neighbours need
-        const float by = to > m[t] ? __builtin_amdgcn_exp2f(m[t] - to) : 1.f;  // 0 where there was nothing yet
-        m[t] = to;
+        // by the row's own scores alone, whatever its neighbours need
+        const float to = x - ref[t] > 8.f ? x : ref[t];
+        const float by = to > ref[t] ? __builtin_amdgcn_exp2f(ref[t] - to) : 1.f;
+        ref[t] = to;
         l[t] *= by, c[t] *= by;
+        weights[t] *= by;
 #pragma unroll
         for (int d = 0; d < 2 * KS; ++d) acc[t][d] *= by;
+#pragma unroll
+        for (int h = 0; h < 2; ++h)
+#pragma unroll
+          for (int r = 0; r < 4; ++r) ex[t][h][r] = ex[t][h][r] == -INFINITY ? -INFINITY : against(t, h, r);
       }
     }
     bf16x8_t p[NS][RT];
 #pragma unroll
-    for (int t = 0; t < RT; ++t) {
-      const float from = m[t] == -INFINITY ? 0.f : m[t];
+    for (int h = 0; h < 2; ++h)
+#pragma unroll
+      for (int r = 0; r < 4; ++r) {
+        const unsigned y = st.s[h].w[2 * r + 1];
+        const float vstep = __uint_as_float(y & 0xffff0000u), vmid = lo_plus<8>(y);
+#pragma unroll
+        for (int t = 0; t < RT; ++t) {
+          const float e = __builtin_amdgcn_exp2f(ex[t][h][r]);
+          l[t] += e;
+          if (inside) {
+            c[t] = fmaf(e, vmid, c[t]);
+            ex[t][h][r] = e * vstep;
+          } else {  // a value that is not finite touches only rows that see it
+            const bool sees = ex[t][h][r] != -INFINITY;
+            c[t] = fmaf(e, sees ? vmid : 0.f, c[t]);
+            ex[t][h][r] = sees ? e * vstep : 0.f;
+          }
+        }
+      }
+#pragma unroll
+    for (int t = 0; t < RT; ++t)
 #pragma unroll
       for (int h = 0; h < 2; ++h)
 #pragma unroll
         for (int r = 0; r < 4; ++r) {
-          const float e = __builtin_amdgcn_exp2f(sc[t][h][r] - from);
-          l[t] += e;
-          float w = e * vstep[h][r], mid = vmid[h][r];
-          if (!inside) {  // a value that is not finite touches only rows that see it
-            const bool sees = seen(t, h, r);
-            w = sees ? w : 0.f, mid = sees ? mid : 0.f;
-          }
           const int slot = 4 * h + (r == 1 ? 2 : r == 2 ? 1 : r);  // codes leave a word of four tokens as 0 and 2, 1 and 3
-          float sum = 0.f, rest = w;
+          float rest = ex[t][h][r];
 #pragma unroll
           for (int n = 0; n < NS; ++n) {
             const bf16_t part = (bf16_t)rest;
             p[n][t][slot] = part;
             rest -= (float)part;
-            sum += (float)part;
           }
-          c[t] = fmaf(e, mid, fmaf(-(float)(OFF + 8), sum, c[t]));
         }
-    }
+    constexpr unsigned ONES = 0x3f803f80u;
+    const u32x4_t ones = {ONES, ONES, ONES, ONES};
+#pragma unroll
+    for (int t = 0; t < RT; ++t)
+#pragma unroll
+      for (int n = 0; n < NS; ++n)
+        weights[t] = __builtin_amdgcn_mfma_f32_16x16x32_bf16(__builtin_bit_cast(bf16x8_t, ones), p[n][t], weights[t], 0, 0, 0);
 #pragma unroll
     for (int w = 0; w < KS; ++w) {
       const unsigned x = st.v[0].w[w], y = st.v[1].w[w];
-      const u32x4_t lo = {place<OFF>(x, 0), place<OFF>(x, 2), place<OFF>(y, 0), place<OFF>(y, 2)};
-      const u32x4_t hi = {place<OFF>(x, 1), place<OFF>(x, 3), place<OFF>(y, 1), place<OFF>(y, 3)};
+      const u32x4_t lo = {place(x, 0), place(x, 2), place(y, 0), place(y, 2)};
+      const u32x4_t hi = {place(x, 1), place(x, 3), place(y, 1), place(y, 3)};
 #pragma unroll
       for (int t = 0; t < RT; ++t)
 #pragma unroll
@@ -259,6 +307,17 @@ struct Walk {
           acc[t][2 * w] = __builtin_amdgcn_mfma_f32_16x16x32_bf16(__builtin_bit_cast(bf16x8_t, lo), p[n][t], acc[t][2 * w], 0, 0, 0);
           acc[t][2 * w + 1] = __builtin_amdgcn_mfma_f32_16x16x32_bf16(__builtin_bit_cast(bf16x8_t, hi), p[n][t], acc[t][2 * w + 1], 0, 0, 0);
         }
+    }
+  }
+
+  // The lanes' parts together: of every row its sums, and what its outputs still lack.
+  __device__ __forceinline__ void end() {
+#pragma unroll
+    for (int t = 0; t < RT; ++t) {
+      l[t] += __shfl_xor(l[t], 16), l[t] += __shfl_xor(l[t], 32);
+      c[t] += __shfl_xor(c[t], 16), c[t] += __shfl_xor(c[t], 32);
+      c[t] = fmaf(-(float)(OFF + 8), weights[t][0], c[t]);
+      if (ref[t] == NOTHING) ref[t] = -INFINITY;
     }
   }
 };
@@ -281,7 +340,8 @@ __device__ __forceinline__ float inverse_sum(float m, float l, bool sink) {
 // Waves a SIMD holds: two, one where queries and sums alone take most of the registers of that.
 constexpr int residents(int NS) { return NS == 3 && D > 160 ? 1 : 2; }
 
-template <int RT, int NS, bool KEYS, typename T>
+// BY16: pages of a multiple of 16 tokens, so that 16 keys lie in one page, whose number is the same for the whole wave.
+template <int RT, int NS, bool KEYS, bool CAP, bool BY16, typename T>
 __global__ __launch_bounds__(256, residents(NS)) void attention4_kernel(Attention4Args a, PageMagic magic) {
   const int lane = threadIdx.x & 63, wave = uniform_wave_number(), quad = lane >> 4;
   const int tile = blockIdx.x / a.nkv, head = blockIdx.x - tile * a.nkv, piece = blockIdx.y;
@@ -293,7 +353,11 @@ __global__ __launch_bounds__(256, residents(NS)) void attention4_kernel(Attentio
   if (row0 >= rows || before < 0) return;
   const Blocks all = blocks_of(a, row0, TILE_ROWS, rows, g, before);
   int i0 = piece * a.piece, end = min(all.count, i0 + a.piece);
-  if (i0 >= all.count) return;
+  if (i0 >= all.count) {  // the sequence has no such piece: its parts say so
+    for (int r = row0 + threadIdx.x; r < min(row0 + TILE_ROWS, rows); r += 256)
+      *(f32x2_t*)(a.part_ml + 2 * (((size_t)(q0 + r / g) * a.nq + head * g + r % g) * a.pieces + piece)) = (f32x2_t){-INFINITY, 0.f};
+    return;
+  }
   const int base = KEYS ? row0 : row0 + wave * 16 * RT;
   const int last_pos = before + (min(base + 16 * RT, rows) - 1) / g, first_pos = before + base / g;
   if (KEYS) {
@@ -306,70 +370,77 @@ __global__ __launch_bounds__(256, residents(NS)) void attention4_kernel(Attentio
     if (a.keep_first == 0) i0 = max(i0, own_first);
   }
   const int last_low = lowest_seen(a, last_pos);
-  Walk<RT, NS, KEYS> walk;
-  walk.template load_queries<T>(a, head, g, q0, base, rows, before, lane);
+  Walk<RT, NS, CAP> walk;
+  const float unit = CAP ? a.scale : a.scale * LOG2E;
+  walk.template load_queries<T>(a, unit, head, g, q0, base, rows, before, lane);
 
   constexpr int STEP = KEYS ? 4 : 1;
+  typedef const int __attribute__((address_space(4)))* constant_ints;
   const int* table = a.table + (size_t)seq * a.table_width;
   auto block_at = [&](int i) { return all.at(max(0, min(i, all.count - 1))); };  // past the end the last one, not used
-  // A page number from the table, wherever it points, is brought into the pool: given-back pages are masked, but asked for.
+  // Rows of the pages (a row: one token of a head) of keys 32 b + 16 h + (lane & 15) and 32 b + 16 h + 4 quad. A page number from the
+  // table, wherever it points, is brought into the pool: given-back pages are masked, but asked for.
+  auto row_of = [&](int entry, int off) { return (unsigned)((max(0, min(entry, a.num_pages - 1)) * a.nkv + head) * a.page_size + off); };
   auto pages = [&](int i) {
     Pages p;
     const int b = block_at(i);
 #pragma unroll
     for (int h = 0; h < 2; ++h) {
       int page, off;
-      page_of(magic, 32 * b + 16 * h + (lane & 15), page, off);
-      p.k[h] = table[min(page, a.table_width - 1)];
-      page_of(magic, 32 * b + 16 * h + 4 * quad, page, off);
-      p.g[h] = table[min(page, a.table_width - 1)];
+      if constexpr (BY16) {
+        page_of(magic, __builtin_amdgcn_readfirstlane(32 * b + 16 * h), page, off);
+        p.k[h] = ((constant_ints)table)[__builtin_amdgcn_readfirstlane(min(page, a.table_width - 1))];
+        p.g[h] = off;
+      } else {
+        page_of(magic, 32 * b + 16 * h + (lane & 15), page, off);
+        p.k[h] = row_of(table[min(page, a.table_width - 1)], off);
+        page_of(magic, 32 * b + 16 * h + 4 * quad, page, off);
+        p.g[h] = row_of(table[min(page, a.table_width - 1)], off);
+      }
     }
     return p;
   };
-  auto load = [&](int i, const Pages& p) {
+  auto load = [&](const Pages& p) {
     Stage st;
-    const int b = block_at(i);
 #pragma unroll
     for (int h = 0; h < 2; ++h) {
-      int page, off;
-      page_of(magic, 32 * b + 16 * h + (lane & 15), page, off);
-      const int64_t krow = ((int64_t)max(0, min(p.k[h], a.num_pages - 1)) * a.nkv + head) * a.page_size + off;
-      st.k[h] = load_words<KS>(a.k + krow * (D / 2) + quad * (D / 8));
-      page_of(magic, 32 * b + 16 * h + 4 * quad, page, off);
-      const int64_t grow = ((int64_t)max(0, min(p.g[h], a.num_pages - 1)) * a.nkv + head) * a.page_size + off;
-      st.v[h] = load_words<KS>(a.v + grow * (D / 2) + (lane & 15) * (D / 8));
-      st.s[h] = load_words<8>(a.steps + 2 * grow);
+      if constexpr (BY16) {
+        const size_t row = (unsigned)__builtin_amdgcn_readfirstlane(row_of(p.k[h], p.g[h]));
+        st.k[h] = load_words<KS>(a.k + row * (D / 2) + (unsigned)((lane & 15) * (D / 2) + quad * (D / 8)));
+        st.v[h] = load_words<KS>(a.v + row * (D / 2) + (unsigned)(quad * (2 * D) + (lane & 15) * (D / 8)));
+        st.s[h] = load_words<8>((const char*)a.steps + row * 8 + (unsigned)(32 * quad));
+      } else {
+        st.k[h] = load_words<KS>(a.k + (size_t)(unsigned)p.k[h] * (D / 2) + quad * (D / 8));
+        st.v[h] = load_words<KS>(a.v + (size_t)(unsigned)p.g[h] * (D / 2) + (lane & 15) * (D / 8));
+        st.s[h] = load_words<8>((const char*)a.steps + (size_t)(unsigned)p.g[h] * 8);
+      }
     }
     return st;
   };
   auto use = [&](const Stage& st, int i) {
     const int b = block_at(i);
     const bool inside = 32 * b + 31 <= first_pos && (32 * b >= last_low || 32 * b + 31 < a.keep_first);
-    walk.block(a, st, b, inside, lane);
+    walk.block(a, unit, st, b, inside, lane);
   };
   if (i0 < end) {
     Pages p0 = pages(i0), p1 = pages(i0 + STEP);
-    Stage s0 = load(i0, p0);
+    Stage s0 = load(p0);
     p0 = pages(i0 + 2 * STEP);
     for (int i = i0; i < end; i += 2 * STEP) {
-      Stage s1 = load(i + STEP, p1);
+      Stage s1 = load(p1);
       p1 = pages(i + 3 * STEP);
       use(s0, i);
       if (i + STEP >= end) break;
-      s0 = load(i + 2 * STEP, p0);
+      s0 = load(p0);
       p0 = pages(i + 4 * STEP);
       use(s1, i + STEP);
     }
   }
-#pragma unroll
-  for (int t = 0; t < RT; ++t) {
-    walk.l[t] += __shfl_xor(walk.l[t], 16), walk.l[t] += __shfl_xor(walk.l[t], 32);
-    walk.c[t] += __shfl_xor(walk.c[t], 16), walk.c[t] += __shfl_xor(walk.c[t], 32);
-  }
+  walk.end();
   if constexpr (KEYS) {
     __shared__ float row_m[4][16], row_l[4][16], row_c[4][16];
     __shared__ f32x4_t meet[3][2 * KS][64];
-    if (quad == 0) row_m[wave][lane] = walk.m[0], row_l[wave][lane] = walk.l[0], row_c[wave][lane] = walk.c[0];
+    if (quad == 0) row_m[wave][lane] = walk.ref[0], row_l[wave][lane] = walk.l[0], row_c[wave][lane] = walk.c[0];
     __syncthreads();
     const int r = lane & 15;
     const float m = fmaxf(fmaxf(row_m[0][r], row_m[1][r]), fmaxf(row_m[2][r], row_m[3][r]));
@@ -391,7 +462,7 @@ __global__ __launch_bounds__(256, residents(NS)) void attention4_kernel(Attentio
     if (wave > 0) return;
 #pragma unroll
     for (int d = 0; d < 2 * KS; ++d) walk.acc[0][d] += meet[0][d][lane] + (meet[1][d][lane] + meet[2][d][lane]);
-    walk.m[0] = m, walk.l[0] = l, walk.c[0] = c;
+    walk.ref[0] = m, walk.l[0] = l, walk.c[0] = c;
   }
 #pragma unroll
   for (int t = 0; t < RT; ++t) {
@@ -402,9 +473,9 @@ __global__ __launch_bounds__(256, residents(NS)) void attention4_kernel(Attentio
       float* to = a.part_o + (row * a.pieces + piece) * D;
 #pragma unroll
       for (int d = 0; d < 2 * KS; ++d) *(f32x4_t*)(to + 16 * d + 4 * quad) = walk.acc[t][d] + walk.c[t];
-      if (quad == 0) a.part_ml[2 * (row * a.pieces + piece)] = walk.m[t], a.part_ml[2 * (row * a.pieces + piece) + 1] = walk.l[t];
+      if (quad == 0) *(f32x2_t*)(a.part_ml + 2 * (row * a.pieces + piece)) = (f32x2_t){walk.ref[t], walk.l[t]};
     } else {
-      const float by = inverse_sum(walk.m[t], walk.l[t], a.sink);
+      const float by = inverse_sum(walk.ref[t], walk.l[t], a.sink);
       T* to = (T*)a.out + row * D;
 #pragma unroll
       for (int d = 0; d < 2 * KS; ++d) store_out4<T>(to + 16 * d + 4 * quad, (walk.acc[t][d] + walk.c[t]) * by);
@@ -412,68 +483,71 @@ __global__ __launch_bounds__(256, residents(NS)) void attention4_kernel(Attentio
   }
 }
 
-// The pieces of a row: a wave a row, its elements over the lanes.
+// The pieces of a row, a block a row: weights of all pieces first, then their sums, every group of D / 4 threads a share of the pieces
+// with its loads on their way together. A piece that says it has seen nothing was not written and is not read (its load goes to the first one).
+constexpr int MOST_PIECES = 1024;
 template <typename T>
-__global__ __launch_bounds__(256) void attention4_merge_kernel(Attention4Args a, int tile_rows) {
+__global__ __launch_bounds__(256) void attention4_merge_kernel(T* out, const float* part_o, const float* part_ml, const int* merge_tokens, int nq, int pieces, int sink) {
+  constexpr int E = D / 4, GROUPS = 256 / E;
+  __shared__ float weight[MOST_PIECES];
+  __shared__ f32x4_t sums[GROUPS][E];
   const int lane = threadIdx.x & 63;
-  const int item = blockIdx.x * 4 + uniform_wave_number();
-  const int index = item / a.nq, head = item - index * a.nq;
-  if (index >= a.num_merge_tokens) return;
-  const int token = a.merge_tokens ? a.merge_tokens[index] : index;
-  // the token's sequence: the last one that begins at it or before
-  int lo = 0, hi = a.num_seqs - 1;
-  while (lo < hi) {
-    const int mid = (lo + hi + 1) / 2;
-    if (a.cu_q[mid] <= token) lo = mid;
-    else hi = mid - 1;
-  }
-  const int g = a.nq / a.nkv, q0 = a.cu_q[lo], q_len = a.cu_q[lo + 1] - q0, before = a.kv_lens[lo] - q_len;
-  if (token >= q0 + q_len || before < 0) return;  // behind the last sequence
-  const int r = (token - q0) * g + head % g;
-  const Blocks all = blocks_of(a, r / tile_rows * tile_rows, tile_rows, q_len * g, g, before);
-  const int n = min(a.pieces, (all.count + a.piece - 1) / a.piece);
-  const size_t row = (size_t)token * a.nq + head;
-  const float* ml = a.part_ml + 2 * row * a.pieces;
-  float m = -INFINITY;
-  for (int i = lane; i < n; i += 64) m = fmaxf(m, ml[2 * i]);
+  const int index = blockIdx.x / nq, head = blockIdx.x - index * nq;
+  const size_t row = (size_t)(merge_tokens ? merge_tokens[index] : index) * nq + head;
+  const f32x2_t* ml = (const f32x2_t*)part_ml + row * pieces;
+  float m = -INFINITY;  // every wave for itself
+  for (int i = lane; i < pieces; i += 64) m = fmaxf(m, ml[i][0]);
   m = wave_max(m);
   float l = 0.f;
-  constexpr int E = (D + 63) / 64;
-  float o[E];
-#pragma unroll
-  for (int e = 0; e < E; ++e) o[e] = 0.f;
-  for (int first = 0; first < n; first += 64) {
+  for (int first = 0; first < pieces; first += 64) {
     const int i = first + lane;
-    float by = 0.f, part = 0.f;
-    if (i < n) {
-      by = ml[2 * i] == -INFINITY ? (ml[2 * i + 1] == 0.f ? 0.f : 1.f) : __builtin_amdgcn_exp2f(ml[2 * i] - m);  // 1: sums that are NaN
-      part = ml[2 * i + 1] * by;
+    float part = 0.f;
+    if (i < pieces) {
+      const f32x2_t x = ml[i];
+      const float by = x[0] == -INFINITY ? (x[1] == 0.f ? 0.f : 1.f) : __builtin_amdgcn_exp2f(x[0] - m);  // 1: sums that are NaN
+      part = x[1] * by;
+      if (threadIdx.x < 64) weight[i] = by;
     }
     l += wave_sum(part);
-    const int here = min(64, n - first);
-#pragma unroll 4
-    for (int j = 0; j < here; ++j) {
-      const float w = __shfl(by, j);
-      const float* src = a.part_o + (row * a.pieces + first + j) * D;
-#pragma unroll
-      for (int e = 0; e < E; ++e)
-        if (64 * e + lane < D) o[e] = w == 0.f ? o[e] : fmaf(w, src[64 * e + lane], o[e]);
-    }
   }
-  const float by = inverse_sum(m, l, a.sink);
-  T* to = (T*)a.out + row * D;
+  __syncthreads();
+  const int group = threadIdx.x / E, e = threadIdx.x - group * E;
+  f32x4_t o = {0.f, 0.f, 0.f, 0.f};
+  if (group < GROUPS) {
+    const float* src = part_o + row * pieces * D + 4 * e;
+#pragma unroll 8
+    for (int i = group; i < pieces; i += GROUPS) {
+      const float w = weight[i];
+      const f32x4_t x = *(const f32x4_t*)(src + (w == 0.f ? 0 : (size_t)i * D));
 #pragma unroll
-  for (int e = 0; e < E; ++e)
-    if (64 * e + lane < D) to[64 * e + lane] = from_f32<T>(o[e] * by);
+      for (int k = 0; k < 4; ++k) o[k] = w == 0.f ? o[k] : fmaf(w, x[k], o[k]);
+    }
+    sums[group][e] = o;
+  }
+  __syncthreads();
+  if (threadIdx.x >= E) return;
+  o = sums[0][threadIdx.x];
+#pragma unroll
+  for (int i = 1; i < GROUPS; ++i) o += sums[i][threadIdx.x];
+  store_out4<T>(out + row * D + 4 * threadIdx.x, o * inverse_sum(m, l, sink));
 }
 
 template <int RT, int NS, bool KEYS, typename T>
 static int launch(const Attention4Args& a, hipStream_t stream) {
-  attention4_kernel<RT, NS, KEYS, T><<<dim3(a.num_tiles * a.nkv, a.pieces), 256, 0, stream>>>(a, page_magic(a.page_size));
+  const dim3 grid(a.num_tiles * a.nkv, a.pieces);
+  const bool by16 = a.page_size % 16 == 0;
+#define GO(CAP, BY16) attention4_kernel<RT, NS, KEYS, CAP, BY16, T><<<grid, 256, 0, stream>>>(a, page_magic(a.page_size))
+  if (a.softcap > 0.f) {
+    if (by16) GO(true, true);
+    else GO(true, false);
+  } else {
+    if (by16) GO(false, true);
+    else GO(false, false);
+  }
+#undef GO
   QRT_LAUNCH_CHECK("attention4");
   if (a.pieces > 1) {
-    const int64_t items = (int64_t)a.num_merge_tokens * a.nq;
-    attention4_merge_kernel<T><<<(unsigned)((items + 3) / 4), 256, 0, stream>>>(a, KEYS ? 16 : 64 * RT);
+    attention4_merge_kernel<T><<<(unsigned)(a.num_merge_tokens * a.nq), 256, 0, stream>>>((T*)a.out, a.part_o, a.part_ml, a.merge_tokens, a.nq, a.pieces, a.sink);
     QRT_LAUNCH_CHECK("attention4 (merge)");
   }
   return 0;
@@ -485,9 +559,10 @@ extern "C" int qrt_attention4(const Attention4Args* args, int dtype, int keys, i
   QRT_CHECK(dtype == QRT_BF16 || dtype == QRT_F32, "attention4: unknown dtype %d", dtype);
   QRT_CHECK(a.nq > 0 && a.nkv > 0 && a.nq % a.nkv == 0, "attention4: %d query heads on %d key heads", a.nq, a.nkv);
   QRT_CHECK(a.page_size >= 4 && a.page_size % 4 == 0 && a.num_pages > 0 && a.table_width > 0, "attention4: pages of a multiple of 4 tokens, not %d", a.page_size);
+  QRT_CHECK((int64_t)a.num_pages * a.nkv * a.page_size < (1ll << 31), "attention4: a pool of %d pages of %d tokens and %d heads has too many rows", a.num_pages, a.page_size, a.nkv);
   QRT_CHECK(a.window >= 0 && a.chunk >= 0 && a.keep_first >= 0 && !(a.window && a.chunk) && !(a.keep_first && !a.window), "attention4: bad mask");
-  QRT_CHECK(a.piece > 0 && a.pieces > 0 && a.pieces <= 65535, "attention4: bad pieces %d of %d", a.pieces, a.piece);
-  QRT_CHECK(a.pieces == 1 || (a.part_o && a.part_ml && a.num_merge_tokens > 0), "attention4: pieces need room for their parts");
+  QRT_CHECK(a.piece > 0 && a.pieces > 0 && a.pieces <= MOST_PIECES, "attention4: bad pieces %d of %d", a.pieces, a.piece);
+  QRT_CHECK(a.pieces == 1 || (a.part_o && a.part_ml && a.num_merge_tokens > 0 && (int64_t)a.num_merge_tokens * a.nq < (1ll << 31)), "attention4: pieces need room for their parts");
   QRT_CHECK((a.tile_seq != nullptr) == (a.tile_row0 != nullptr) || keys, "attention4: a list of tiles has sequences and rows");
   QRT_CHECK(!keys || a.nq / a.nkv <= 16, "attention4: %d rows a token in a tile of 16", a.nq / a.nkv);
   QRT_CHECK((int64_t)a.num_tiles * a.nkv < (1ll << 31), "attention4: too many tiles");

@@ -2131,7 +2131,7 @@ class HipOps:
             tiles = tokens = None
             n_tiles = ctx.num_seqs
             if not keys:
-                host, n_tiles = self.plan_tiles(q_lens, kv_lens, g, 64 * row_tiles, a.nkv, seq_ids=list(seqs))
+                host, n_tiles = self.plan_tiles(q_lens, kv_lens, g, 64 * row_tiles, a.nkv, self.resident_blocks, list(seqs))
                 tiles = torch.from_numpy(host).to(q.device)
             elif subset is not None:
                 n_tiles = len(q_lens)
@@ -2154,7 +2154,7 @@ class HipOps:
         most = self.attention4_blocks(max(kv_lens), most_q, a.window, a.chunk, a.keep_first)
         total = sum(self.attention4_blocks(n, most_q, a.window, a.chunk, a.keep_first) for n in lens)
         splits = ctx.scratch.get("attn_splits")
-        a.piece = -(-most // splits) if splits else self.choose_attention4_piece(most, total, n_tiles, a.nkv, keys)
+        a.piece = max(-(-most // splits), -(-most // 1024)) if splits else self.choose_attention4_piece(most, total, n_tiles, a.nkv, keys)
         a.pieces = -(-most // a.piece)
         if a.pieces > 1:
             parts = ctx.num_tokens * a.nq * a.pieces
