@@ -74,12 +74,33 @@ __device__ __forceinline__ Words<N> load_words(const void* p) {
   return r;
 }
 
+#ifdef __HIP_DEVICE_COMPILE__  // the host's compiler knows no buffer resources
+template <int N>
+__device__ __forceinline__ Words<N> load_words(const __amdgpu_buffer_rsrc_t from, unsigned lane_at, unsigned at) {
+  Words<N> r;
+  constexpr int FOURS = N / 4, REST = N % 4;
+#pragma unroll
+  for (int i = 0; i < FOURS; ++i) {
+    const auto x = __builtin_amdgcn_raw_buffer_load_b128(from, lane_at + 16 * i, at, 0);
+#pragma unroll
+    for (int e = 0; e < 4; ++e) r.w[4 * i + e] = x[e];
+  }
+  if constexpr (REST == 1) {
+    r.w[N - 1] = __builtin_amdgcn_raw_buffer_load_b32(from, lane_at + 16 * FOURS, at, 0);
+  } else if constexpr (REST == 2) {
+    const auto x = __builtin_amdgcn_raw_buffer_load_b64(from, lane_at + 16 * FOURS, at, 0);
+    r.w[N - 2] = x[0], r.w[N - 1] = x[1];
+  } else if constexpr (REST == 3) {
+    const auto x = __builtin_amdgcn_raw_buffer_load_b96(from, lane_at + 16 * FOURS, at, 0);
+    r.w[N - 3] = x[0], r.w[N - 2] = x[1], r.w[N - 1] = x[2];
+  }
+  return r;
+}
+#endif
+
 struct Stage {
   Words<KS> k[2], v[2];
   Words<8> s[2];
-};
-struct Pages {
-  int k[2], g[2];
 };
 
 // Nibbles `nibble` and `nibble` + 4 of x as a pair of bfloat16, OFF + n each. Mask and exponent are kept in registers where the compiler
@@ -121,14 +142,16 @@ struct Walk {
   f32x4_t acc[RT][2 * KS], weights[RT];  // sum w (OFF + n); sum w, four times the same
 
   template <typename T>
-  __device__ __forceinline__ void load_queries(const Attention4Args& a, float unit, int head, int g, int q0, int base, int rows, int before, int lane) {
+  __device__ __forceinline__ void load_queries(const Attention4Args& a, float unit, int head, PageMagic g, int q0, int base, int rows, int before, int lane) {
     const int quad = lane >> 4;
 #pragma unroll
     for (int t = 0; t < RT; ++t) {
       const int r = min(base + 16 * t + (lane & 15), rows - 1);
-      pos[t] = before + r / g;
+      int token, in_group;
+      page_of(g, r, token, in_group);
+      pos[t] = before + token;
       low[t] = lowest_seen(a, pos[t]);
-      const T* src = (const T*)a.q + ((size_t)(q0 + r / g) * a.nq + head * g + r % g) * D + quad * (D / 4);
+      const T* src = (const T*)a.q + ((size_t)(q0 + token) * a.nq + head * (int)g.size + in_group) * D + quad * (D / 4);
       float sum = 0.f;
 #pragma unroll
       for (int s = 0; s < KS; ++s) {
@@ -337,22 +360,71 @@ __device__ __forceinline__ float inverse_sum(float m, float l, bool sink) {
   return l == 0.f ? 0.f : 1.f / l;
 }
 
-// Waves a SIMD holds: two, one where queries and sums alone take most of the registers of that.
-constexpr int residents(int NS) { return NS == 3 && D > 160 ? 1 : 2; }
+// Waves a SIMD holds: three where a wave has few rows of up to 128 elements, one where queries and sums alone take most of half the registers.
+constexpr int residents(int RT, int NS) { return NS == 3 && D > 160 ? 1 : 2; }
 
-// BY16: pages of a multiple of 16 tokens, so that 16 keys lie in one page, whose number is the same for the whole wave.
+// BY16: pages of a multiple of 16 tokens, so that 16 keys lie in one page and where they begin is the same for the whole wave, and pools of
+// less than 4 GiB. A lane finds the page of 16 keys, 32 blocks of 32 at a time, and the loads take it from there into a scalar: finding
+// pages with scalar instructions, block after block, took a hundred of them a block.
 template <int RT, int NS, bool KEYS, bool CAP, bool BY16, typename T>
-__global__ __launch_bounds__(256, residents(NS)) void attention4_kernel(Attention4Args a, PageMagic magic) {
+__global__ __launch_bounds__(256, residents(RT, NS)) void attention4_kernel(Attention4Args a, PageMagic magic, PageMagic g_magic) {
   const int lane = threadIdx.x & 63, wave = uniform_wave_number(), quad = lane >> 4;
-  const int tile = blockIdx.x / a.nkv, head = blockIdx.x - tile * a.nkv, piece = blockIdx.y;
-  const int seq = a.tile_seq ? a.tile_seq[tile] : tile, row0 = a.tile_row0 ? a.tile_row0[tile] : 0;
-  const int g = a.nq / a.nkv;
-  const int q0 = a.cu_q[seq], q_len = a.cu_q[seq + 1] - q0, kv_len = a.kv_lens[seq];
+  const int head = blockIdx.x, tile = blockIdx.y, piece = blockIdx.z;
+  constexpr int TILE_ROWS = KEYS ? 16 : 64 * RT, STEP = KEYS ? 4 : 1;
+  // What the launch's shapes hang on is read through the scalar cache: the page numbers of the first keys, which without a window do not
+  // wait for the lengths, and these come together.
+  typedef const int __attribute__((address_space(4)))* constant_ints;
+  auto constant = [](const int* p, int i) { return ((constant_ints)p)[__builtin_amdgcn_readfirstlane(i)]; };
+  const int seq = a.tile_seq ? constant(a.tile_seq, tile) : tile, row0 = a.tile_row0 ? constant(a.tile_row0, tile) : 0;
+  const int g = g_magic.size;
+  const bool from_start = !a.window && !a.chunk;
+  const int* table = a.table + (size_t)seq * a.table_width;
+  // A row: one token of a head. A page number from the table, wherever it points, is brought into the pool: given-back pages are
+  // masked, but asked for.
+  auto row_of = [&](int entry, int off) { return (unsigned)((max(0, min(entry, a.num_pages - 1)) * a.nkv + head) * a.page_size + off); };
+  auto row_of_key = [&](int key) {
+    int page, off;
+    page_of(magic, key, page, off);
+    return row_of(table[min(page, a.table_width - 1)], off);
+  };
+#ifdef __HIP_DEVICE_COMPILE__
+  constexpr int RAW = 0x00020000;  // a buffer of bytes
+  const unsigned pool_rows = (unsigned)a.num_pages * a.nkv * a.page_size;
+  const __amdgpu_buffer_rsrc_t k_buf = __builtin_amdgcn_make_buffer_rsrc((void*)a.k, 0, (int)(pool_rows * (D / 2)), RAW);
+  const __amdgpu_buffer_rsrc_t v_buf = __builtin_amdgcn_make_buffer_rsrc((void*)a.v, 0, (int)(pool_rows * (D / 2)), RAW);
+  const __amdgpu_buffer_rsrc_t s_buf = __builtin_amdgcn_make_buffer_rsrc((void*)a.steps, 0, (int)(pool_rows * 8), RAW);
+#endif
+  // keys 16 h + (lane & 15) and 16 h + 4 quad of block b; `found`: BY16, the rows that the lanes have found, those of this block in 2 j and 2 j + 1
+  auto load = [&](int b, unsigned found, int j) {
+    Stage st;
+#ifdef __HIP_DEVICE_COMPILE__
+#pragma unroll
+    for (int h = 0; h < 2; ++h) {
+      if constexpr (BY16) {
+        const unsigned row = (unsigned)__builtin_amdgcn_readlane((int)found, 2 * j + h);
+        st.k[h] = load_words<KS>(k_buf, (lane & 15) * (D / 2) + quad * (D / 8), row * (D / 2));
+        st.v[h] = load_words<KS>(v_buf, quad * (2 * D) + (lane & 15) * (D / 8), row * (D / 2));
+        st.s[h] = load_words<8>(s_buf, 32 * quad, row * 8);
+      } else {
+        const size_t krow = row_of_key(32 * b + 16 * h + (lane & 15)), grow = row_of_key(32 * b + 16 * h + 4 * quad);
+        st.k[h] = load_words<KS>(a.k + krow * (D / 2) + quad * (D / 8));
+        st.v[h] = load_words<KS>(a.v + grow * (D / 2) + (lane & 15) * (D / 8));
+        st.s[h] = load_words<8>((const char*)a.steps + grow * 8);
+      }
+    }
+#endif
+    return st;
+  };
+  int i0 = piece * a.piece;
+  constexpr int FOUND = 30;  // blocks of a batch: the lanes find 32, one of them is fetched in the batch before
+  auto key_of_lane = [&](int b) { return 32 * b + 16 * (lane & 1); };
+  unsigned found = 0;
+  if (BY16 && from_start) found = row_of_key(key_of_lane(i0 + (KEYS ? wave : 0) + (lane >> 1) * STEP));
+  const int q0 = constant(a.cu_q, seq), q_len = constant(a.cu_q, seq + 1) - q0, kv_len = constant(a.kv_lens, seq);
   const int rows = q_len * g, before = kv_len - q_len;
-  constexpr int TILE_ROWS = KEYS ? 16 : 64 * RT;
   if (row0 >= rows || before < 0) return;
   const Blocks all = blocks_of(a, row0, TILE_ROWS, rows, g, before);
-  int i0 = piece * a.piece, end = min(all.count, i0 + a.piece);
+  int end = min(all.count, i0 + a.piece);
   if (i0 >= all.count) {  // the sequence has no such piece: its parts say so
     for (int r = row0 + threadIdx.x; r < min(row0 + TILE_ROWS, rows); r += 256)
       *(f32x2_t*)(a.part_ml + 2 * (((size_t)(q0 + r / g) * a.nq + head * g + r % g) * a.pieces + piece)) = (f32x2_t){-INFINITY, 0.f};
@@ -372,68 +444,34 @@ __global__ __launch_bounds__(256, residents(NS)) void attention4_kernel(Attentio
   const int last_low = lowest_seen(a, last_pos);
   Walk<RT, NS, CAP> walk;
   const float unit = CAP ? a.scale : a.scale * LOG2E;
-  walk.template load_queries<T>(a, unit, head, g, q0, base, rows, before, lane);
+  walk.template load_queries<T>(a, unit, head, g_magic, q0, base, rows, before, lane);
 
-  constexpr int STEP = KEYS ? 4 : 1;
-  typedef const int __attribute__((address_space(4)))* constant_ints;
-  const int* table = a.table + (size_t)seq * a.table_width;
-  auto block_at = [&](int i) { return all.at(max(0, min(i, all.count - 1))); };  // past the end the last one, not used
-  // Rows of the pages (a row: one token of a head) of keys 32 b + 16 h + (lane & 15) and 32 b + 16 h + 4 quad. A page number from the
-  // table, wherever it points, is brought into the pool: given-back pages are masked, but asked for.
-  auto row_of = [&](int entry, int off) { return (unsigned)((max(0, min(entry, a.num_pages - 1)) * a.nkv + head) * a.page_size + off); };
-  auto pages = [&](int i) {
-    Pages p;
-    const int b = block_at(i);
-#pragma unroll
-    for (int h = 0; h < 2; ++h) {
-      int page, off;
-      if constexpr (BY16) {
-        page_of(magic, __builtin_amdgcn_readfirstlane(32 * b + 16 * h), page, off);
-        p.k[h] = ((constant_ints)table)[__builtin_amdgcn_readfirstlane(min(page, a.table_width - 1))];
-        p.g[h] = off;
-      } else {
-        page_of(magic, 32 * b + 16 * h + (lane & 15), page, off);
-        p.k[h] = row_of(table[min(page, a.table_width - 1)], off);
-        page_of(magic, 32 * b + 16 * h + 4 * quad, page, off);
-        p.g[h] = row_of(table[min(page, a.table_width - 1)], off);
-      }
-    }
-    return p;
-  };
-  auto load = [&](const Pages& p) {
-    Stage st;
-#pragma unroll
-    for (int h = 0; h < 2; ++h) {
-      if constexpr (BY16) {
-        const size_t row = (unsigned)__builtin_amdgcn_readfirstlane(row_of(p.k[h], p.g[h]));
-        st.k[h] = load_words<KS>(a.k + row * (D / 2) + (unsigned)((lane & 15) * (D / 2) + quad * (D / 8)));
-        st.v[h] = load_words<KS>(a.v + row * (D / 2) + (unsigned)(quad * (2 * D) + (lane & 15) * (D / 8)));
-        st.s[h] = load_words<8>((const char*)a.steps + row * 8 + (unsigned)(32 * quad));
-      } else {
-        st.k[h] = load_words<KS>(a.k + (size_t)(unsigned)p.k[h] * (D / 2) + quad * (D / 8));
-        st.v[h] = load_words<KS>(a.v + (size_t)(unsigned)p.g[h] * (D / 2) + (lane & 15) * (D / 8));
-        st.s[h] = load_words<8>((const char*)a.steps + (size_t)(unsigned)p.g[h] * 8);
-      }
-    }
-    return st;
-  };
+  auto block_at = [&](int i) { return from_start ? i : all.at(max(0, min(i, all.count - 1))); };  // past the end none that is used
   auto use = [&](const Stage& st, int i) {
     const int b = block_at(i);
     const bool inside = 32 * b + 31 <= first_pos && (32 * b >= last_low || 32 * b + 31 < a.keep_first);
     walk.block(a, unit, st, b, inside, lane);
   };
   if (i0 < end) {
-    Pages p0 = pages(i0), p1 = pages(i0 + STEP);
-    Stage s0 = load(p0);
-    p0 = pages(i0 + 2 * STEP);
-    for (int i = i0; i < end; i += 2 * STEP) {
-      Stage s1 = load(p1);
-      p1 = pages(i + 3 * STEP);
+    if (BY16 && !from_start) found = row_of_key(key_of_lane(block_at(i0 + (lane >> 1) * STEP)));
+    Stage s0 = load(block_at(i0), found, 0), s1;
+    unsigned later = 0;
+    int j = FOUND;  // where the batch stands
+    for (int i = i0;;) {
+      if (BY16 && j == FOUND) {  // j runs by two: a batch's rows are found while the one before is used
+        if (i != i0) found = later;
+        later = row_of_key(key_of_lane(block_at(i + (FOUND + (lane >> 1)) * STEP)));
+        j = 0;
+      }
+      s1 = load(block_at(i + STEP), found, j + 1);
       use(s0, i);
-      if (i + STEP >= end) break;
-      s0 = load(p0);
-      p0 = pages(i + 4 * STEP);
-      use(s1, i + STEP);
+      i += STEP;
+      if (i >= end) break;
+      s0 = load(block_at(i + STEP), found, j + 2);
+      use(s1, i);
+      i += STEP;
+      if (i >= end) break;
+      j += 2;
     }
   }
   walk.end();
@@ -468,7 +506,9 @@ __global__ __launch_bounds__(256, residents(NS)) void attention4_kernel(Attentio
   for (int t = 0; t < RT; ++t) {
     const int r = base + 16 * t + (lane & 15);
     if (r >= rows) continue;
-    const size_t row = (size_t)(q0 + r / g) * a.nq + head * g + r % g;
+    int token, in_group;
+    page_of(g_magic, r, token, in_group);
+    const size_t row = (size_t)(q0 + token) * a.nq + head * g + in_group;
     if (a.pieces > 1) {
       float* to = a.part_o + (row * a.pieces + piece) * D;
 #pragma unroll
@@ -534,9 +574,9 @@ __global__ __launch_bounds__(256) void attention4_merge_kernel(T* out, const flo
 
 template <int RT, int NS, bool KEYS, typename T>
 static int launch(const Attention4Args& a, hipStream_t stream) {
-  const dim3 grid(a.num_tiles * a.nkv, a.pieces);
-  const bool by16 = a.page_size % 16 == 0;
-#define GO(CAP, BY16) attention4_kernel<RT, NS, KEYS, CAP, BY16, T><<<grid, 256, 0, stream>>>(a, page_magic(a.page_size))
+  const dim3 grid(a.nkv, a.num_tiles, a.pieces);
+  const bool by16 = a.page_size % 16 == 0 && (int64_t)a.num_pages * a.nkv * a.page_size * (D / 2 > 8 ? D / 2 : 8) < (1ll << 32);
+#define GO(CAP, BY16) attention4_kernel<RT, NS, KEYS, CAP, BY16, T><<<grid, 256, 0, stream>>>(a, page_magic(a.page_size), page_magic(a.nq / a.nkv))
   if (a.softcap > 0.f) {
     if (by16) GO(true, true);
     else GO(true, false);
@@ -565,7 +605,7 @@ extern "C" int qrt_attention4(const Attention4Args* args, int dtype, int keys, i
   QRT_CHECK(a.pieces == 1 || (a.part_o && a.part_ml && a.num_merge_tokens > 0 && (int64_t)a.num_merge_tokens * a.nq < (1ll << 31)), "attention4: pieces need room for their parts");
   QRT_CHECK((a.tile_seq != nullptr) == (a.tile_row0 != nullptr) || keys, "attention4: a list of tiles has sequences and rows");
   QRT_CHECK(!keys || a.nq / a.nkv <= 16, "attention4: %d rows a token in a tile of 16", a.nq / a.nkv);
-  QRT_CHECK((int64_t)a.num_tiles * a.nkv < (1ll << 31), "attention4: too many tiles");
+  QRT_CHECK(a.num_tiles <= 65535, "attention4: %d tiles in one launch, 65535 at most", a.num_tiles);
   QRT_CHECK(((uintptr_t)a.q | (uintptr_t)a.out | (uintptr_t)a.k | (uintptr_t)a.v | (uintptr_t)a.steps) % 16 == 0, "attention4: tensors must begin at multiples of 16 bytes");
   if (a.num_tiles <= 0) return 0;
   if (dtype == QRT_F32) {

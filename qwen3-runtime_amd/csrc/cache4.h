@@ -13,15 +13,16 @@
 #pragma once
 #include "common.h"
 
-struct PageMagic {  // division by the page size without dividing
+struct PageMagic {  // division of numbers below 2^31 by the page size, or the like, without dividing
   unsigned size, by;
 };
-inline PageMagic page_magic(int page_size) {
-  return {(unsigned)page_size, (unsigned)(((1ull << 32) + page_size - 1) / page_size)};
+inline PageMagic page_magic(int size) {
+  return {(unsigned)size, size == 1 ? ~0u : (unsigned)(((1ull << 32) + size - 1) / size)};
 }
 __device__ __forceinline__ void page_of(PageMagic m, int key, int& page, int& offset) {
-  unsigned q = __umulhi((unsigned)key, m.by);  // one too many at most
+  unsigned q = __umulhi((unsigned)key, m.by);  // one too many at most; by 1, one too few at most
   int r = key - (int)(q * m.size);
   if (r < 0) r += m.size, --q;
+  if (r >= (int)m.size) r -= m.size, ++q;
   page = (int)q, offset = r;
 }
