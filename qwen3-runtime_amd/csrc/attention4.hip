@@ -100,7 +100,12 @@ __device__ __forceinline__ Words<N> load_words(const __amdgpu_buffer_rsrc_t from
 
 struct Stage {
   Words<KS> k[2], v[2];
-  Words<8> s[2];
+  unsigned s;  // lanes below 32: lo and step of key `lane`, the others: of value `lane` - 32
+};
+// What a lane makes of the pairs of its wave's 32 keys, one pair a lane, for all to read: of keys what multiplies a sum and a query's
+// sum, of values the step and the middle.
+struct Scales {
+  float kmul[32], kadd[32], vstep[32], vmid[32];
 };
 
 // Nibbles `nibble` and `nibble` + 4 of x as a pair of bfloat16, OFF + n each. Mask and exponent are kept in registers where the compiler
@@ -123,11 +128,6 @@ struct Place {
   }
 };
 
-// lo + by * step of a pair of bfloat16, in float32
-template <int BY>
-__device__ __forceinline__ float lo_plus(unsigned pair) {
-  return fmaf((float)BY, __uint_as_float(pair & 0xffff0000u), __uint_as_float(pair << 16));
-}
 constexpr float NOTHING = -3.4028235e38f;  // the reference of a row that has seen no key
 
 template <int RT, int NS, bool CAP>
@@ -139,7 +139,7 @@ struct Walk {
   float ref[RT];               // what exponents are taken against, in log2
   float l[RT], c[RT];          // this lane's part of sum e, and of sum e (lo + 8 step)
   int pos[RT], low[RT];
-  f32x4_t acc[RT][2 * KS], weights[RT];  // sum w (OFF + n); sum w, four times the same
+  f32x4_t acc[RT][2 * KS], weights[RT];  // sum w (OFF + n) since the last time the offsets were taken out; sum w since then, four times the same
 
   template <typename T>
   __device__ __forceinline__ void load_queries(const Attention4Args& a, float unit, int head, PageMagic g, int q0, int base, int rows, int before, int lane) {
@@ -188,8 +188,16 @@ struct Walk {
   }
 
   // One block of 32 keys. `inside`: every row of the wave sees all of it. `unit`: of the scores, log2 but with a cap.
-  __device__ __forceinline__ void block(const Attention4Args& a, float unit, const Stage& st, int b, bool inside, int lane) {
+  __device__ __forceinline__ void block(const Attention4Args& a, float unit, const Stage& st, Scales& scales, int b, bool inside, int lane) {
     const int quad = lane >> 4;
+    const bool of_value = lane >= 32;
+    {
+      const float step = __uint_as_float(st.s & 0xffff0000u), lo = __uint_as_float(st.s << 16);
+      float* to = (float*)&scales + (of_value ? 32 : 0) + lane;  // lane - 32 of the third array, or lane of the first
+      to[0] = step * (of_value ? 1.f : unit);
+      to[32] = fmaf(of_value ? 8.f : -(float)OFF, step, lo);
+    }
+    __builtin_amdgcn_wave_barrier();  // a wave's reads of LDS come behind its writes
     f32x4_t sc[RT][2];
 #pragma unroll
     for (int t = 0; t < RT; ++t)
@@ -208,15 +216,13 @@ struct Walk {
             sc[t][h] = __builtin_amdgcn_mfma_f32_16x16x32_bf16(__builtin_bit_cast(bf16x8_t, w), q[n][t][s], sc[t][h], 0, 0, 0);
       }
     // of rows lane & 15 and keys 16 h + 4 quad + r: score = kmul * sc + kadd * qsum
-    float kmul[2][4], kadd[2][4];
+    f32x4_t kmul[2], kadd[2], vstep[2], vmid[2];
 #pragma unroll
-    for (int h = 0; h < 2; ++h)
-#pragma unroll
-      for (int r = 0; r < 4; ++r) {
-        const unsigned x = st.s[h].w[2 * r];
-        kmul[h][r] = __uint_as_float(x & 0xffff0000u) * unit;
-        kadd[h][r] = lo_plus<-OFF>(x);
-      }
+    for (int h = 0; h < 2; ++h) {
+      kmul[h] = *(const f32x4_t*)(scales.kmul + 16 * h + 4 * quad), kadd[h] = *(const f32x4_t*)(scales.kadd + 16 * h + 4 * quad);
+      vstep[h] = *(const f32x4_t*)(scales.vstep + 16 * h + 4 * quad), vmid[h] = *(const f32x4_t*)(scales.vmid + 16 * h + 4 * quad);
+    }
+    __builtin_amdgcn_wave_barrier();
     auto score = [&](int t, int h, int r) {
       const float x = fmaf(kmul[h][r], sc[t][h][r], kadd[h][r] * qsum[t]);
       return CAP ? a.softcap * tanhf(x / a.softcap) * LOG2E : x;
@@ -280,19 +286,17 @@ struct Walk {
     for (int h = 0; h < 2; ++h)
 #pragma unroll
       for (int r = 0; r < 4; ++r) {
-        const unsigned y = st.s[h].w[2 * r + 1];
-        const float vstep = __uint_as_float(y & 0xffff0000u), vmid = lo_plus<8>(y);
 #pragma unroll
         for (int t = 0; t < RT; ++t) {
           const float e = __builtin_amdgcn_exp2f(ex[t][h][r]);
           l[t] += e;
           if (inside) {
-            c[t] = fmaf(e, vmid, c[t]);
-            ex[t][h][r] = e * vstep;
+            c[t] = fmaf(e, vmid[h][r], c[t]);
+            ex[t][h][r] = e * vstep[h][r];
           } else {  // a value that is not finite touches only rows that see it
             const bool sees = ex[t][h][r] != -INFINITY;
-            c[t] = fmaf(e, sees ? vmid : 0.f, c[t]);
-            ex[t][h][r] = sees ? e * vstep : 0.f;
+            c[t] = fmaf(e, sees ? vmid[h][r] : 0.f, c[t]);
+            ex[t][h][r] = sees ? e * vstep[h][r] : 0.f;
           }
         }
       }
@@ -333,13 +337,25 @@ struct Walk {
     }
   }
 
+  // The offsets of the codes out of the sums, which stay small so: what a sum of OFF w loses in its last places adds up over a long
+  // walk to more than a flat softmax leaves of its values (32,000 keys: 0.8 % of them).
+  __device__ __forceinline__ void center() {
+#pragma unroll
+    for (int t = 0; t < RT; ++t) {
+      const float off = -(float)(OFF + 8) * weights[t][0];
+#pragma unroll
+      for (int d = 0; d < 2 * KS; ++d) acc[t][d] += off;
+      weights[t] = (f32x4_t){0.f, 0.f, 0.f, 0.f};
+    }
+  }
+
   // The lanes' parts together: of every row its sums, and what its outputs still lack.
   __device__ __forceinline__ void end() {
+    center();
 #pragma unroll
     for (int t = 0; t < RT; ++t) {
       l[t] += __shfl_xor(l[t], 16), l[t] += __shfl_xor(l[t], 32);
       c[t] += __shfl_xor(c[t], 16), c[t] += __shfl_xor(c[t], 32);
-      c[t] = fmaf(-(float)(OFF + 8), weights[t][0], c[t]);
       if (ref[t] == NOTHING) ref[t] = -INFINITY;
     }
   }
@@ -404,13 +420,17 @@ __global__ __launch_bounds__(256, residents(RT, NS)) void attention4_kernel(Atte
         const unsigned row = (unsigned)__builtin_amdgcn_readlane((int)found, 2 * j + h);
         st.k[h] = load_words<KS>(k_buf, (lane & 15) * (D / 2) + quad * (D / 8), row * (D / 2));
         st.v[h] = load_words<KS>(v_buf, quad * (2 * D) + (lane & 15) * (D / 8), row * (D / 2));
-        st.s[h] = load_words<8>(s_buf, 32 * quad, row * 8);
       } else {
         const size_t krow = row_of_key(32 * b + 16 * h + (lane & 15)), grow = row_of_key(32 * b + 16 * h + 4 * quad);
         st.k[h] = load_words<KS>(a.k + krow * (D / 2) + quad * (D / 8));
         st.v[h] = load_words<KS>(a.v + grow * (D / 2) + (lane & 15) * (D / 8));
-        st.s[h] = load_words<8>((const char*)a.steps + grow * 8);
       }
+    }
+    if constexpr (BY16) {
+      const unsigned row0 = (unsigned)__builtin_amdgcn_readlane((int)found, 2 * j), row1 = (unsigned)__builtin_amdgcn_readlane((int)found, 2 * j + 1);
+      st.s = load_words<1>(s_buf, 8 * ((lane & 16 ? row1 : row0) + (lane & 15)) + 4 * (lane >> 5), 0).w[0];
+    } else {
+      st.s = a.steps[2 * (size_t)row_of_key(32 * b + (lane & 31)) + (lane >> 5)];
     }
 #endif
     return st;
@@ -442,6 +462,7 @@ __global__ __launch_bounds__(256, residents(RT, NS)) void attention4_kernel(Atte
     if (a.keep_first == 0) i0 = max(i0, own_first);
   }
   const int last_low = lowest_seen(a, last_pos);
+  __shared__ __align__(16) Scales scales[4];
   Walk<RT, NS, CAP> walk;
   const float unit = CAP ? a.scale : a.scale * LOG2E;
   walk.template load_queries<T>(a, unit, head, g_magic, q0, base, rows, before, lane);
@@ -450,7 +471,7 @@ __global__ __launch_bounds__(256, residents(RT, NS)) void attention4_kernel(Atte
   auto use = [&](const Stage& st, int i) {
     const int b = block_at(i);
     const bool inside = 32 * b + 31 <= first_pos && (32 * b >= last_low || 32 * b + 31 < a.keep_first);
-    walk.block(a, unit, st, b, inside, lane);
+    walk.block(a, unit, st, scales[wave], b, inside, lane);
   };
   if (i0 < end) {
     if (BY16 && !from_start) found = row_of_key(key_of_lane(block_at(i0 + (lane >> 1) * STEP)));
@@ -458,6 +479,7 @@ __global__ __launch_bounds__(256, residents(RT, NS)) void attention4_kernel(Atte
     unsigned later = 0;
     int j = FOUND;  // where the batch stands
     for (int i = i0;;) {
+      if ((i - i0) / STEP % 8 == 0) walk.center();
       if (BY16 && j == FOUND) {  // j runs by two: a batch's rows are found while the one before is used
         if (i != i0) found = later;
         later = row_of_key(key_of_lane(block_at(i + (FOUND + (lane >> 1)) * STEP)));
