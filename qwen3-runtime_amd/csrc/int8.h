@@ -43,3 +43,6 @@ __device__ __forceinline__ unsigned codes4(float a, float b, float c, float d, f
   const unsigned ab = __builtin_amdgcn_perm(ub, ua, 0x0c0c0400), cd = __builtin_amdgcn_perm(ud, uc, 0x04000c0c);
   return ab | cd;
 }
+
+int int8_tiles(const void* a, const float* a_scale, const void* w, const float* w_scale, void* c, int out_dtype, int M, int N, int width, int tile,
+               int act_kind, float limit, hipStream_t stream);

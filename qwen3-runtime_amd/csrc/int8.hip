@@ -90,8 +90,10 @@ static void launch_quantize(const T* x, int8_t* codes, float* scale, int M, int 
   const bool aligned = K % 8 == 0 && (uintptr_t)x % 16 == 0;
 #define GO(THREADS, KEEP, ALIGNED) \
   quantize_rows_kernel<T, THREADS, KEEP, ALIGNED><<<dim3((M + 256 / THREADS - 1) / (256 / THREADS)), dim3(256), 0, stream>>>(x, codes, scale, M, K, width)
+  // a wave a row needs no barrier: 1,999 rows of 2,560 columns 6.8 us by blocks
   if (!aligned) GO(256, 4, false);
   else if (width <= 1024) GO(64, 2, true);
+  else if (width <= 4096 && M >= 512) GO(64, 8, true);
   else if (width <= 4096) GO(256, 2, true);
   else GO(256, 5, true);
 #undef GO
@@ -127,23 +129,25 @@ struct Int8Rows {
   GatedEpilogue ep;
 };
 
-// The waves' share of the rows that a FUSED block turns into codes: pieces of 8 columns a lane, in registers from the loads to the codes.
-constexpr int FUSED_PIECES = 10;
-// Waves that share a row's maximum.
+// Rows that a block turns into codes itself (FUSED): up to four, a row to each of its four waves, or to two or all four of them; a lane
+// has ITS pieces of 8 columns, in registers from the loads to the codes.
+constexpr int FUSED_MOST = 10;
 constexpr int fused_parts(int M) { return M == 1 ? 4 : M == 2 ? 2 : 1; }
-constexpr int fused_steps(int M, int width) { return (width / 8 + 64 * fused_parts(M) - 1) / (64 * fused_parts(M)); }
-constexpr bool fused_takes(int M, int width) { return M <= 16 && (M * fused_parts(M) + 3) / 4 * fused_steps(M, width) <= FUSED_PIECES; }
+constexpr int fused_its(int M, int width) { return (width / 8 + 64 * fused_parts(M) - 1) / (64 * fused_parts(M)); }
+constexpr bool fused_takes(int M, int width) { return M >= 1 && M <= 4 && fused_its(M, width) <= FUSED_MOST; }
 
 // NW waves; WU units of eight weight rows (1: the operand's rows 8 to 15 repeat the others); MB blocks of 16 rows of the
 // activations (FEW: eight); GATED: half of the units are gate rows, half the up rows that belong to them.
-template <int NW, int WU, int MB, bool FEW, int U, bool GATED, bool FUSED, typename TX, typename TO>
+// ITS > 0: FUSED.
+template <int NW, int WU, int MB, bool FEW, int U, bool GATED, int ITS, typename TX, typename TO>
 __global__ __launch_bounds__(64 * NW) void int8_rows_kernel(Int8Rows p) {
+  constexpr bool FUSED = ITS > 0;
   constexpr int NT = WU == 1 ? 1 : WU / 2, AU = FEW ? 1 : 2 * MB, LOADS = WU + (FUSED ? 0 : AU), SLOT = LOADS * 1024;
   constexpr int OUTS = GATED ? 4 * WU : 8 * WU, ONCE = 2;  // outputs of a block; the cache policy of a non-temporal load
   static_assert((U - 1) * LOADS < 64, "the loads' counter holds 63");
-  static_assert(!FUSED || (NW == 4 && MB == 1), "the waves that share a row are counted for four");
+  static_assert(!FUSED || (NW == 4 && FEW), "the waves that share a row are counted for four");
   extern __shared__ __align__(16) unsigned char rows_lds[];  // [NW][U] slots, later the sums; FUSED: the rows' codes behind them
-  __shared__ unsigned most_of[FUSED ? 16 : 1];
+  __shared__ unsigned most_of[FUSED ? 4 : 1];
   const int lane = threadIdx.x & 63, wave = uniform_wave_number();
   const int r16 = lane & 15, quad = lane >> 4, sub = lane >> 3, piece = (lane & 7) ^ sub;
   const int n0 = blockIdx.x * OUTS;
@@ -153,21 +157,12 @@ __global__ __launch_bounds__(64 * NW) void int8_rows_kernel(Int8Rows p) {
   const int width = p.width, steps = width / INT8_STAGE;
 
   // FUSED: the rows come first, and are waited for behind the weights' loads
-  float v[FUSED ? FUSED_PIECES : 1][8];
-  const int parts = fused_parts(p.M), its = fused_steps(p.M, width), items = p.M * parts;
-  auto item_of = [&](int j, int& row, int& at) {  // piece j of this lane: its row (p.M or more: none) and first column
-    const int item = wave + NW * (j / its);
-    row = item / parts;
-    at = 8 * ((item % parts) * 64 + lane + 64 * parts * (j % its));
-    return item < items;
-  };
+  float v[FUSED ? ITS : 1][8];
+  const int parts = fused_parts(p.M), own_row = wave / parts, own_at = 8 * ((wave - own_row * parts) * 64 + lane);
   if constexpr (FUSED) {
 #pragma unroll
-    for (int j = 0; j < FUSED_PIECES; ++j) {
-      int row, at;
-      const bool any = item_of(j, row, at);
-      load_row8<TX, true>((const TX*)p.x + (size_t)(any ? row : 0) * p.K, any ? at : p.K, p.K, v[j]);
-    }
+    for (int j = 0; j < ITS; ++j)
+      load_row8<TX, true>((const TX*)p.x + (size_t)min(own_row, p.M - 1) * p.K, own_row < p.M ? own_at + 512 * parts * j : p.K, p.K, v[j]);
   }
   const int8_t* src[LOADS];
 #pragma unroll
@@ -193,33 +188,28 @@ __global__ __launch_bounds__(64 * NW) void int8_rows_kernel(Int8Rows p) {
   for (; fetched < U && fetched < mine; ++fetched) fetch(fetched, fetched);
 
   if constexpr (FUSED) {
-    __shared__ unsigned part_of[64];
+    __shared__ unsigned part_of[4];
     unsigned most = 0;
 #pragma unroll
-    for (int j = 0; j < FUSED_PIECES; ++j) {
+    for (int j = 0; j < ITS; ++j)
 #pragma unroll
       for (int e = 0; e < 8; ++e) most = max(most, magnitude_bits(v[j][e]));
-      if (j % its == its - 1) {  // the same in every lane
-        const unsigned m = wave_max_bits(most);
-        const int item = wave + NW * (j / its);
-        if (lane == 0 && item < items) part_of[item] = m;
-        most = 0;
-      }
-    }
+    most = wave_max_bits(most);
+    if (lane == 0) part_of[wave] = most;
     QRT_WAIT_LDS();
     QRT_BARRIER();
+    if (own_row < p.M) {
+      for (int i = 0; i < parts; ++i) most = max(most, part_of[own_row * parts + i]);
+      if (lane == 0) most_of[own_row] = most;
+      const float by = code_factor(most);
 #pragma unroll
-    for (int j = 0; j < FUSED_PIECES; ++j) {
-      int row, at;
-      if (!item_of(j, row, at) || at >= width) continue;
-      unsigned m = 0;
-      for (int i = 0; i < parts; ++i) m = max(m, part_of[row * parts + i]);
-      if (at == 0) most_of[row] = m;
-      const float by = code_factor(m);
-      typedef unsigned u32x2_t __attribute__((ext_vector_type(2)));
-      // piece c of 16 columns of a stage's row r lies at 16 (c ^ (r & 7)), as in the rings
-      unsigned char* to = own_codes + (size_t)(at >> 7) * (FEW ? 1024 : 2048) + row * 128 + 16 * (((at >> 4) & 7) ^ (row & 7)) + (at & 8);
-      *(u32x2_t*)to = (u32x2_t){codes4(v[j][0], v[j][1], v[j][2], v[j][3], by), codes4(v[j][4], v[j][5], v[j][6], v[j][7], by)};
+      for (int j = 0; j < ITS; ++j) {
+        const int at = own_at + 512 * parts * j;
+        typedef unsigned u32x2_t __attribute__((ext_vector_type(2)));
+        // piece c of 16 columns of a stage's row r lies at 16 (c ^ (r & 7)), as in the rings
+        unsigned char* to = own_codes + (size_t)(at >> 7) * 1024 + own_row * 128 + 16 * (((at >> 4) & 7) ^ own_row) + (at & 8);
+        if (at < width) *(u32x2_t*)to = (u32x2_t){codes4(v[j][0], v[j][1], v[j][2], v[j][3], by), codes4(v[j][4], v[j][5], v[j][6], v[j][7], by)};
+      }
     }
     QRT_WAIT_LDS();
     QRT_BARRIER();
@@ -239,7 +229,7 @@ __global__ __launch_bounds__(64 * NW) void int8_rows_kernel(Int8Rows p) {
     if (fetched - i == U) QRT_WAIT_LOADS((U - 1) * LOADS);
     else QRT_WAIT_LOADS(0);
     const unsigned char* at = ring + slot * SLOT;
-    const unsigned char* codes = FUSED ? own_codes + (size_t)(wave + i * NW) * (FEW ? 1024 : 2048) : at + WU * 1024;
+    const unsigned char* codes = FUSED ? own_codes + (size_t)(wave + i * NW) * 1024 : at + WU * 1024;
     i32x4_t w[NT][2], a[MB][2];
 #pragma unroll
     for (int h = 0; h < 2; ++h) {
@@ -294,18 +284,18 @@ __global__ __launch_bounds__(64 * NW) void int8_rows_kernel(Int8Rows p) {
   }
 }
 
-template <int NW, int WU, int MB, bool FEW, int U, bool GATED, bool FUSED, typename TX, typename TO>
+template <int NW, int WU, int MB, bool FEW, int U, bool GATED, int ITS, typename TX, typename TO>
 static int launch_int8_rows(const Int8Rows& p, hipStream_t stream) {
   constexpr int NT = WU == 1 ? 1 : WU / 2, AU = FEW ? 1 : 2 * MB, OUTS = GATED ? 4 * WU : 8 * WU;
-  constexpr size_t rings = (size_t)NW * U * (WU + (FUSED ? 0 : AU)) * 1024, meet = (size_t)NW * NT * MB * 1024;
-  const size_t smem = (rings > meet ? rings : meet) + (FUSED ? (size_t)p.width / INT8_STAGE * AU * 1024 : 0);
-  static_assert(rings <= 156 * 1024, "the rings of this configuration do not fit LDS");
-  QRT_CHECK(smem <= 156 * 1024, "int8_rows: %d columns need %zu bytes of LDS", p.width, smem);
-  auto kernel = int8_rows_kernel<NW, WU, MB, FEW, U, GATED, FUSED, TX, TO>;
+  constexpr size_t rings = (size_t)NW * U * (WU + (ITS ? 0 : AU)) * 1024, meet = (size_t)NW * NT * MB * 1024, most = 150 * 1024;
+  const size_t smem = (rings > meet ? rings : meet) + (ITS ? (size_t)p.width / INT8_STAGE * 1024 : 0);
+  static_assert(rings <= most, "the rings of this configuration do not fit LDS");
+  QRT_CHECK(smem <= most, "int8_rows: %d columns need %zu bytes of LDS", p.width, smem);
+  auto kernel = int8_rows_kernel<NW, WU, MB, FEW, U, GATED, ITS, TX, TO>;
   static bool allowed = false;  // once per kernel: not inside a stream capture again and again
-  if (!allowed) {
-    if (hipFuncSetAttribute((const void*)kernel, hipFuncAttributeMaxDynamicSharedMemorySize, 156 * 1024) != hipSuccess)
-      return qrt_fail("int8_rows: cannot get LDS");
+  if (smem > 64 * 1024 && !allowed) {
+    if (hipFuncSetAttribute((const void*)kernel, hipFuncAttributeMaxDynamicSharedMemorySize, (int)most) != hipSuccess)
+      return qrt_fail("int8_rows: cannot get %zu bytes of LDS", smem);
     allowed = true;
   }
   kernel<<<dim3((p.N + OUTS - 1) / OUTS), dim3(64 * NW), smem, stream>>>(p);
@@ -313,44 +303,66 @@ static int launch_int8_rows(const Int8Rows& p, hipStream_t stream) {
   return 0;
 }
 
-template <bool GATED, bool FUSED, typename TX, typename TO>
+template <bool GATED, typename TX, typename TO>
+static int fused_by_size(const Int8Rows& p, hipStream_t stream) {
+  constexpr int WU = GATED ? 2 : 1;
+  const int its = fused_its(p.M, p.width);
+  if (its <= 2) return launch_int8_rows<4, WU, 1, true, 4, GATED, 2, TX, TO>(p, stream);
+  if (its <= 5) return launch_int8_rows<4, WU, 1, true, 4, GATED, 5, TX, TO>(p, stream);
+  return launch_int8_rows<4, WU, 1, true, 4, GATED, FUSED_MOST, TX, TO>(p, stream);
+}
+template <bool GATED, typename TO>
 static int rows_by_size(const Int8Rows& p, hipStream_t stream) {
-  if constexpr (FUSED) {
-    if (p.M <= 8) return launch_int8_rows<4, GATED ? 2 : 1, 1, true, 4, GATED, true, TX, TO>(p, stream);
-    return launch_int8_rows<4, 2, 1, false, 4, GATED, true, TX, TO>(p, stream);
-  } else {
-    if (p.M <= 8) return launch_int8_rows<4, 2, 1, true, 4, GATED, false, TX, TO>(p, stream);
-    if (p.M <= 16) return launch_int8_rows<4, 2, 1, false, 4, GATED, false, TX, TO>(p, stream);
-    if (p.M <= 32) return launch_int8_rows<4, 2, 2, false, 4, GATED, false, TX, TO>(p, stream);
-    if (p.M <= 48) return launch_int8_rows<4, 4, 3, false, 3, GATED, false, TX, TO>(p, stream);
-    return launch_int8_rows<4, 4, 4, false, 3, GATED, false, TX, TO>(p, stream);
-  }
+  if (p.M <= 8) return launch_int8_rows<4, 2, 1, true, 4, GATED, 0, float, TO>(p, stream);
+  if (p.M <= 16) return launch_int8_rows<4, 2, 1, false, 4, GATED, 0, float, TO>(p, stream);
+  if (p.M <= 32) return launch_int8_rows<4, 2, 2, false, 3, GATED, 0, float, TO>(p, stream);
+  if (p.M <= 48) return launch_int8_rows<4, 4, 3, false, 2, GATED, 0, float, TO>(p, stream);
+  return launch_int8_rows<4, 4, 4, false, 2, GATED, 0, float, TO>(p, stream);
 }
 
-// Whether qrt_int8_rows turns these rows into codes itself.
-extern "C" int qrt_int8_rows_fuses(int M, int K, int width) { return M > 0 && K % 8 == 0 && fused_takes(M, width); }
-
-// c [M, N] of up to 64 rows. Either x (rows as they are, in x_dtype; qrt_int8_rows_fuses says which) or a and a_scale. act_kind < 0: no gate;
-// otherwise w is [2 N, width].
-extern "C" int qrt_int8_rows(const void* x, int x_dtype, const void* a, const float* a_scale, const void* w, const float* w_scale, void* c,
-                             int out_dtype, int M, int N, int K, int width, int act_kind, float limit, hipStream_t stream) {
-  if (check_width("int8_rows", M, K, width)) return -1;
-  QRT_CHECK(N > 0 && M <= 64, "int8_rows: bad sizes M=%d N=%d", M, N);
-  QRT_CHECK(act_kind <= QRT_ACT_CLAMPED, "int8_rows: unknown activation %d", act_kind);
-  QRT_CHECK(out_dtype == QRT_BF16 || out_dtype == QRT_F32, "int8_rows: unknown output dtype %d", out_dtype);
-  QRT_CHECK(((uintptr_t)(x ? x : a) | (uintptr_t)w) % 16 == 0, "int8_rows: operands must begin at multiples of 16 bytes");
-  QRT_CHECK(!x || qrt_int8_rows_fuses(M, K, width), "int8_rows: %d rows of %d columns come as codes", M, K);
-  QRT_CHECK(!x || x_dtype == QRT_BF16 || x_dtype == QRT_F32, "int8_rows: unknown dtype %d", x_dtype);
-  if (M == 0) return 0;
+// c [M, N] of up to 64 rows. Either x (rows as they are, in x_dtype: those that fused_takes, of a multiple of 8 columns) or a and a_scale.
+// act_kind < 0: no gate; otherwise w is [2 N, width].
+static int int8_rows(const void* x, int x_dtype, const void* a, const float* a_scale, const void* w, const float* w_scale, void* c, int out_dtype,
+                     int M, int N, int K, int width, int act_kind, float limit, hipStream_t stream) {
   const Int8Rows p{x, (const int8_t*)a, a_scale, (const int8_t*)w, w_scale, c, M, N, K, width, GatedEpilogue{act_kind, limit, nullptr}};
   const bool bf = out_dtype == QRT_BF16;
 #define GO(GATED)                                                                                                            \
   do {                                                                                                                       \
-    if (x && x_dtype == QRT_BF16) return bf ? rows_by_size<GATED, true, bf16_t, bf16_t>(p, stream) : rows_by_size<GATED, true, bf16_t, float>(p, stream); \
-    if (x) return bf ? rows_by_size<GATED, true, float, bf16_t>(p, stream) : rows_by_size<GATED, true, float, float>(p, stream);                         \
-    return bf ? rows_by_size<GATED, false, float, bf16_t>(p, stream) : rows_by_size<GATED, false, float, float>(p, stream);  \
+    if (x && x_dtype == QRT_BF16) return bf ? fused_by_size<GATED, bf16_t, bf16_t>(p, stream) : fused_by_size<GATED, bf16_t, float>(p, stream); \
+    if (x) return bf ? fused_by_size<GATED, float, bf16_t>(p, stream) : fused_by_size<GATED, float, float>(p, stream);       \
+    return bf ? rows_by_size<GATED, bf16_t>(p, stream) : rows_by_size<GATED, float>(p, stream);                              \
   } while (0)
   if (act_kind >= 0) GO(true);
   GO(false);
 #undef GO
+}
+
+// Rows up to which the weight is streamed past them; more go by tiles.
+constexpr int STREAMED_ROWS = 64;
+
+// Bytes of workspace that qrt_int8_product wants: none, or the rows' codes and scales.
+extern "C" int64_t qrt_int8_workspace(int M, int K, int width) {
+  return K % 8 == 0 && fused_takes(M, width) ? 0 : (int64_t)M * width + 4 * (((int64_t)M + 3) & ~3ll);
+}
+
+// c [M, N] (out_dtype) = rows x [M, K] (x_dtype) by w [N, width] and w_scale [N], or with a gate (act_kind >= 0) w [2 N, width], w_scale [2 N] and the activation
+// of the two. tile: a number of TILES in ops/hip.py, for more than 64 rows.
+extern "C" int qrt_int8_product(const void* x, int x_dtype, const void* w, const float* w_scale, void* c, int out_dtype, void* workspace, int M, int N,
+                                int K, int width, int tile, int act_kind, float limit, hipStream_t stream) {
+  if (check_width("int8_product", M, K, width)) return -1;
+  QRT_CHECK(N > 0 && N < (1 << 30), "int8_product: bad size N=%d", N);
+  QRT_CHECK(x_dtype == QRT_BF16 || x_dtype == QRT_F32, "int8_product: unknown dtype %d", x_dtype);
+  QRT_CHECK(out_dtype == QRT_BF16 || out_dtype == QRT_F32, "int8_product: unknown output dtype %d", out_dtype);
+  QRT_CHECK(act_kind <= QRT_ACT_CLAMPED, "int8_product: unknown activation %d", act_kind);
+  QRT_CHECK(((uintptr_t)w | (uintptr_t)c | (uintptr_t)workspace) % 16 == 0, "int8_product: operands must begin at multiples of 16 bytes");
+  const int64_t room = qrt_int8_workspace(M, K, width);
+  QRT_CHECK(room == 0 || workspace, "int8_product: %d rows of %d columns need a workspace", M, K);
+  QRT_CHECK(room > 0 || (uintptr_t)x % 16 == 0, "int8_product: rows must begin at a multiple of 16 bytes");
+  if (M == 0) return 0;
+  if (room == 0) return int8_rows(x, x_dtype, nullptr, nullptr, w, w_scale, c, out_dtype, M, N, K, width, act_kind, limit, stream);
+  int8_t* const codes = (int8_t*)workspace;
+  float* const scale = (float*)(codes + (int64_t)M * width);
+  if (qrt_quantize_rows(x, x_dtype, codes, scale, M, K, width, stream)) return -1;
+  if (M <= STREAMED_ROWS) return int8_rows(nullptr, x_dtype, codes, scale, w, w_scale, c, out_dtype, M, N, K, width, act_kind, limit, stream);
+  return int8_tiles(codes, scale, w, w_scale, c, out_dtype, M, N, width, tile, act_kind, limit, stream);
 }

@@ -203,16 +203,11 @@ static int int8_by_result(const Int8TileArgs& p, int out_dtype, hipStream_t stre
 }
 
 // c [M, N] from codes a [M, width], w [N, width] ([2 N, width] with a gate: act_kind >= 0); tile: a number of TILES in ops/hip.py.
-extern "C" int qrt_int8_tiles(const void* a, const float* a_scale, const void* w, const float* w_scale, void* c, int out_dtype, int M, int N,
-                              int width, int tile, int act_kind, float limit, hipStream_t stream) {
-  QRT_CHECK(M >= 0 && N > 0 && width > 0 && width % INT8_STAGE == 0 && width <= INT8_MOST_WIDTH, "int8_tiles: bad sizes M=%d N=%d, rows of %d", M, N, width);
-  QRT_CHECK(out_dtype == QRT_BF16 || out_dtype == QRT_F32, "int8_tiles: unknown output dtype %d", out_dtype);
-  QRT_CHECK(act_kind <= QRT_ACT_CLAMPED, "int8_tiles: unknown activation %d", act_kind);
-  QRT_CHECK(((uintptr_t)a | (uintptr_t)w | (uintptr_t)c) % 16 == 0, "int8_tiles: operands must begin at multiples of 16 bytes");
+int int8_tiles(const void* a, const float* a_scale, const void* w, const float* w_scale, void* c, int out_dtype, int M, int N, int width, int tile,
+               int act_kind, float limit, hipStream_t stream) {
   const uint64_t limit_bytes = (1ull << 32) - 128;  // offsets are 32 bits
   QRT_CHECK((uint64_t)M * width <= limit_bytes && (uint64_t)(act_kind >= 0 ? 2 : 1) * N * width <= limit_bytes,
             "int8_tiles: an operand of 4 GiB or more (M=%d N=%d, rows of %d)", M, N, width);
-  if (M == 0) return 0;
   const Int8TileArgs p{(const int8_t*)a, a_scale, (const int8_t*)w, w_scale, c, M, N, width, 0, 0, act_kind, limit};
   switch (tile) {
     case 0: return int8_by_result<256, 192, 4, 2, 2>(p, out_dtype, stream);

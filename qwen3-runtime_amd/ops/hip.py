@@ -363,6 +363,9 @@ class HipOps:
         """``residual_planes``: ``linear_for_residual`` may cut K into planes with any number of rows, and not
         only with few; for callers that hand its result to nothing but the norms and ``accumulate``."""
         self.lib = core_library()
+        # declared, the arguments travel as they are: a wrapper object for each of fifteen took 2 us a call
+        self.lib.qrt_int8_product.argtypes = [c_void_p, c_int, c_void_p, c_void_p, c_void_p, c_int, c_void_p] + [c_int] * 6 + [c_float, c_void_p]
+        self.lib.qrt_int8_workspace.argtypes, self.lib.qrt_int8_workspace.restype = [c_int] * 3, c_long
         self.residual_planes = residual_planes
 
     def _check(self, lib, code: int) -> None:
@@ -1678,43 +1681,37 @@ class HipOps:
                                                          c_int(width), _stream()))
         return codes, scale
 
-    # rows up to which a product of 8-bit integers streams the weight past them; more go by tiles
-    int8_max_rows = 64
-
     def _int8_product(self, x, w, out_f32=False, gate=None):
-        """The product of rows by an ``Int8Weight``; ``gate`` = (activation, limit): gate rows, then up rows, and the activation of the two."""
+        """The product of rows by an ``Int8Weight``; ``gate`` = (activation, limit): gate rows, then up rows, and the activation of the two.
+        Up to 64 rows go past the weight as it streams, more by tiles; up to four short ones are quantised by the kernel that multiplies them."""
         if isinstance(x, ScaledRows):
             x = x.made()
-        if x.dim() != 2 or x.dtype not in _CODE or x.shape[1] != w.shape[1]:
-            raise OpsError(f"linear: x is {tuple(x.shape)} of {x.dtype}, the weight in 8 bits is {tuple(w.shape)}")
-        _need(x, "x")
-        _need(w.values, "weight", torch.int8, (w.shape[0], w.width))
-        _need(w.scale, "weight's scales", torch.float32, (w.shape[0],))
-        if x.device != w.device:
-            raise OpsError(f"linear: x is on {x.device}, the weight on {w.device}")
-        (m, k), n, act, limit = x.shape, w.shape[0], -1, 0.0
+        values, scale, (n, k), width = w.values, w.scale, w.shape, w.width
+        dtype = x.dtype
+        if x.dim() != 2 or dtype not in _CODE or x.shape[1] != k:
+            raise OpsError(f"linear: x is {tuple(x.shape)} of {dtype}, the weight in 8 bits is {tuple(w.shape)}")
+        if not (x.is_cuda and x.is_contiguous() and x.device == values.device):
+            _need(x, "x")
+            raise OpsError(f"linear: x is on {x.device}, the weight on {values.device}")
+        m, act, limit, form = x.shape[0], -1, 0.0, "whole"
         if gate is not None:
             act, limit = ACTIVATIONS[gate[0]], gate[1]
             if act > ACTIVATIONS["clamped"] or n % 2:
                 raise OpsError(f"gated_linear: {gate[0]} of a weight {tuple(w.shape)}")
-            n //= 2
-        out = torch.empty((m, n), dtype=torch.float32 if out_f32 else x.dtype, device=x.device)
+            n, form = n // 2, "gated"
+        device, lib = x.device, self.lib
+        out = torch.empty((m, n), dtype=torch.float32 if out_f32 else dtype, device=device)
         if m == 0:
             return out
-        if self.lib.qrt_int8_rows_fuses(c_int(m), c_int(k), c_int(w.width)) and x.data_ptr() % 16 == 0:
-            rows, codes, scale = x, None, None
-        else:
-            rows, (codes, scale) = None, self.quantize_rows(x)
-        if m <= self.int8_max_rows:
-            self._check(self.lib, self.lib.qrt_int8_rows(
-                _ptr(rows), c_int(_CODE[x.dtype]), _ptr(codes), _ptr(scale), _ptr(w.values), _ptr(w.scale), _ptr(out), c_int(_CODE[out.dtype]),
-                c_int(m), c_int(n), c_int(k), c_int(w.width), c_int(act), c_float(limit), _stream()))
-        else:
-            # 128 columns of bytes are a stage, as 64 of bfloat16 are: the same bytes and the same cycles of the matrix cores
-            tile = self.choose_tile(m, n, w.width // 2, "gated" if gate is not None else "whole")[0]
-            self._check(self.lib, self.lib.qrt_int8_tiles(
-                _ptr(codes), _ptr(scale), _ptr(w.values), _ptr(w.scale), _ptr(out), c_int(_CODE[out.dtype]), c_int(m), c_int(n), c_int(w.width),
-                c_int(tile), c_int(act), c_float(limit), _stream()))
+        if x.data_ptr() % 16:
+            x = x.clone()
+        room = 0 if m <= 4 and lib.qrt_int8_workspace(m, k, width) == 0 else m * width + 16 * (m // 4 + 1)
+        work = torch.empty(room, dtype=torch.uint8, device=device).data_ptr() if room else None
+        # 128 columns of bytes are a stage, as 64 of bfloat16 are: the same bytes and the same cycles of the matrix cores
+        tile = self.choose_tile(m, n, width // 2, form)[0] if m > 64 else 0
+        if lib.qrt_int8_product(x.data_ptr(), _CODE[dtype], values.data_ptr(), scale.data_ptr(), out.data_ptr(), F32 if out_f32 else _CODE[dtype],
+                                work, m, n, k, width, tile, act, limit, _stream()):
+            raise OpsError(lib.qrt_last_error().decode())
         return out
 
     def gated_linear(self, x, w_gate_up, activation="swiglu", limit=0.0, row_scale=None):
@@ -1912,13 +1909,17 @@ class HipOps:
 
     @staticmethod
     def _check_cache4(cache, nkv, d) -> int:
-        ps, pages = cache.group.page_size, cache.k.shape[0]
+        ps, pages, steps = cache.group.page_size, cache.k.shape[0], cache.pages.get("steps", cache.k)
+        if (cache.k.dtype == cache.v.dtype == torch.uint8 and steps.dtype == torch.bfloat16 and cache.k.shape == cache.v.shape == (pages, nkv, ps, d // 2)
+                and steps.shape == (pages, nkv, ps, 4) and cache.k.is_contiguous() and cache.v.is_contiguous() and steps.is_contiguous()
+                and cache.k.is_cuda and cache.v.device == steps.device == cache.k.device and d % 32 == 0 and 32 <= d <= 256 and ps % 4 == 0):
+            return pages
         if d % 32 or not 32 <= d <= 256 or ps % 4:
             raise OpsError(f"a cache of 4 bits has heads of 32 to 256 in steps of 32 and pages of a multiple of 4 tokens, not {d} and {ps}")
         _need(cache.k, "key cache", torch.uint8, (pages, nkv, ps, d // 2))
         _need(cache.v, "value cache", torch.uint8, (pages, nkv, ps, d // 2))
-        _need(cache.pages.get("steps", cache.k), "steps of the cache", torch.bfloat16, (pages, nkv, ps, 4))
-        return pages
+        _need(steps, "steps of the cache", torch.bfloat16, (pages, nkv, ps, 4))
+        raise OpsError(f"a cache on {cache.k.device}, {cache.v.device} and {steps.device}")
 
     def kv_store(self, k, v, cache):
         """``k``, ``v`` [T, heads, D] into their places in the cache."""
@@ -2072,41 +2073,52 @@ class HipOps:
     # ---- attention over a cache of 4 bits --------------------------------------------
     def _attention4(self, q, cache, ctx, nq, nkv, d, scale, window, chunk, softcap, keep_first, sink):
         """Sequences of at most 16 rows (tokens by heads of a group) go by blocks whose waves share their keys, the others by tiles of rows;
-        a step that has both takes a launch for either."""
+        a step that has both takes a launch for either. What follows from the step's lengths is kept with its context, for its other layers."""
         pages = self._check_cache4(cache, nkv, d)
-        if q.dtype not in _CODE:
-            raise OpsError(f"queries of {q.dtype}; the attention takes bfloat16 and float32")
-        if nq % nkv or not math.isfinite(scale) or softcap < 0:
-            raise OpsError(f"{nq} query heads on {nkv} key heads, scale {scale}, cap {softcap}")
-        if (keep_first and not window) or (window and chunk) or min(window, chunk, keep_first) < 0:
-            raise OpsError("a window, beside which first keys may stay in sight, or a mask of chunks")
-        ps, g, s = cache.group.page_size, nq // nkv, ctx.num_seqs
-        table = _need(cache.group.block_table, "block table", torch.int32)
-        if table.dim() != 2 or table.shape[0] != s:
-            raise OpsError(f"block table {tuple(table.shape)} for {s} sequences")
-        if table.shape[1] * ps < ctx.max_kv_len:
+        group = cache.group
+        table, s = group.block_table, ctx.num_seqs
+        key = ("attn4", nq, nkv, d, group.page_size, window, chunk, keep_first, q.dtype, ctx.scratch.get("attn_splits"))
+        plan = ctx.scratch.get(key)
+        if plan is None:
+            if q.dtype not in _CODE:
+                raise OpsError(f"queries of {q.dtype}; the attention takes bfloat16 and float32")
+            if nq % nkv:
+                raise OpsError(f"{nq} query heads on {nkv} key heads")
+            if (keep_first and not window) or (window and chunk) or min(window, chunk, keep_first) < 0:
+                raise OpsError("a window, beside which first keys may stay in sight, or a mask of chunks")
+            if len(ctx.q_lens_host) != s or sum(ctx.q_lens_host) != ctx.num_tokens:
+                raise OpsError(f"{ctx.num_tokens} tokens in {s} sequences, of lengths {ctx.q_lens_host}")
+            few = [i for i in range(s) if ctx.q_lens_host[i] * (nq // nkv) <= 16]
+            if len(few) == s:
+                plan = [self._plan_attention4(q, ctx, None, True, nq, nkv, d, window, chunk, keep_first)]
+            else:
+                many = [i for i in range(s) if ctx.q_lens_host[i] * (nq // nkv) > 16]
+                plan = [self._plan_attention4(q, ctx, few, True, nq, nkv, d, window, chunk, keep_first)] if any(ctx.q_lens_host[i] for i in few) else []
+                plan.append(self._plan_attention4(q, ctx, many, False, nq, nkv, d, window, chunk, keep_first))
+            ctx.scratch[key] = plan
+        if not (math.isfinite(scale) and softcap >= 0):
+            raise OpsError(f"scale {scale}, cap {softcap}")
+        if table.dtype != torch.int32 or table.dim() != 2 or table.shape[0] != s or not table.is_contiguous():
+            raise OpsError(f"block table {tuple(table.shape)} of {table.dtype} for {s} sequences")
+        if table.shape[1] * group.page_size < ctx.max_kv_len:
             raise OpsError(f"block table is {table.shape[1]} pages wide, the longest sequence has {ctx.max_kv_len} tokens")
-        if len(ctx.q_lens_host) != s or sum(ctx.q_lens_host) != ctx.num_tokens:
-            raise OpsError(f"{ctx.num_tokens} tokens in {s} sequences, of lengths {ctx.q_lens_host}")
-        if not (q.device == cache.k.device == table.device):
+        if not (q.device == cache.k.device == table.device == ctx.kv_lens.device == ctx.cu_q.device):
             raise OpsError(f"queries on {q.device}, a cache on {cache.k.device}, its table on {table.device}")
         out = torch.empty((ctx.num_tokens, nq * d), dtype=q.dtype, device=q.device)
-        a = _Attn4Args()
-        a.q, a.out, a.k, a.v, a.steps = q.data_ptr(), out.data_ptr(), cache.k.data_ptr(), cache.v.data_ptr(), cache.pages["steps"].data_ptr()
-        a.cu_q = _need(ctx.cu_q, "cu_q", torch.int32, (s + 1,)).data_ptr()
-        a.kv_lens = _need(ctx.kv_lens, "kv_lens", torch.int32, (s,)).data_ptr()
-        a.table, a.table_width, a.num_pages, a.num_seqs = table.data_ptr(), table.shape[1], pages, s
-        a.nq, a.nkv, a.page_size = nq, nkv, ps
-        a.window, a.chunk, a.keep_first, a.sink, a.scale, a.softcap = window, chunk, keep_first, int(sink), scale, softcap
         if ctx.num_tokens == 0:
             return out
-        few = [i for i in range(s) if ctx.q_lens_host[i] * g <= 16]
-        if len(few) == s:
-            self._launch_attention4(a, q, ctx, None, True, d)
-        else:
-            if any(ctx.q_lens_host[i] for i in few):
-                self._launch_attention4(a, q, ctx, few, True, d)
-            self._launch_attention4(a, q, ctx, [i for i in range(s) if ctx.q_lens_host[i] * g > 16], False, d)
+        cu_q, kv_lens = _need(ctx.cu_q, "cu_q", torch.int32, (s + 1,)), _need(ctx.kv_lens, "kv_lens", torch.int32, (s,))
+        lib = attention4_library(d)
+        for fixed, keys, row_tiles, room, _tensors in plan:
+            a = _Attn4Args.from_buffer_copy(fixed)
+            a.q, a.out, a.k, a.v, a.steps = q.data_ptr(), out.data_ptr(), cache.k.data_ptr(), cache.v.data_ptr(), cache.pages["steps"].data_ptr()
+            a.cu_q, a.kv_lens, a.table = cu_q.data_ptr(), kv_lens.data_ptr(), table.data_ptr()
+            a.table_width, a.num_pages, a.page_size = table.shape[1], pages, group.page_size
+            a.sink, a.scale, a.softcap = sink, scale, softcap
+            if room:
+                parts = torch.empty((room * (d + 2),), dtype=torch.float32, device=q.device)
+                a.part_o, a.part_ml = parts.data_ptr(), parts.data_ptr() + 4 * room * d
+            self._check(lib, lib.qrt_attention4(byref(a), c_int(_CODE[q.dtype]), c_int(keys), c_int(row_tiles), _stream()))
         return out
 
     @staticmethod
@@ -2118,56 +2130,47 @@ class HipOps:
             return min(-(-kv // 32), -(-(chunk + q_len) // 32) + 1)
         return -(-kv // 32)
 
-    def _launch_attention4(self, a, q, ctx, subset, keys, d):
-        g = a.nq // a.nkv
-        bf = q.dtype == torch.bfloat16
+    def _plan_attention4(self, q, ctx, subset, keys, nq, nkv, d, window, chunk, keep_first):
+        """One launch over the sequences in ``subset`` (None: all): its arguments but for the tensors' addresses, its kernel, the rows of parts
+        it needs room for, and the device lists that the arguments name."""
+        g, bf = nq // nkv, q.dtype == torch.bfloat16
         seqs = range(ctx.num_seqs) if subset is None else subset
         q_lens = [ctx.q_lens_host[i] for i in seqs]
         kv_lens = [ctx.kv_lens_host[i] for i in seqs]
         row_tiles = 2 if bf and d <= 128 and not keys and max(q_lens) * g > 64 else 1
-        key = ("attn4_plan", g, a.nkv, keys, row_tiles, None if subset is None else tuple(subset))
-        plan = ctx.scratch.get(key)
-        if plan is None:  # the same for every layer of the step
-            tiles = tokens = None
-            n_tiles = ctx.num_seqs
-            if not keys:
-                host, n_tiles = self.plan_tiles(q_lens, kv_lens, g, 64 * row_tiles, a.nkv, self.resident_blocks, list(seqs))
-                tiles = torch.from_numpy(host).to(q.device)
-            elif subset is not None:
-                n_tiles = len(q_lens)
-                tiles = torch.tensor(list(seqs) + [0] * n_tiles, dtype=torch.int32, device=q.device)
-            if subset is not None:  # the tokens of these sequences: where a merge of pieces writes
-                cu = np.concatenate([[0], np.cumsum(ctx.q_lens_host)])
-                tokens = torch.from_numpy(np.concatenate([np.arange(cu[i], cu[i + 1]) for i in seqs]).astype(np.int32)).to(q.device)
-            plan = ctx.scratch[key] = (tiles, n_tiles, tokens)
-        tiles, n_tiles, tokens = plan
-        a.tile_seq = a.tile_row0 = a.merge_tokens = a.part_o = a.part_ml = None
+        tiles = tokens = None
+        n_tiles = ctx.num_seqs
+        if not keys:
+            host, n_tiles = self.plan_tiles(q_lens, kv_lens, g, 64 * row_tiles, nkv, self.resident_blocks, list(seqs))
+            tiles = torch.from_numpy(host).to(q.device)
+        elif subset is not None:
+            n_tiles = len(q_lens)
+            tiles = torch.tensor(list(seqs) + [0] * n_tiles, dtype=torch.int32, device=q.device)
+        if subset is not None:  # the tokens of these sequences: where a merge of pieces writes
+            cu = np.concatenate([[0], np.cumsum(ctx.q_lens_host)])
+            tokens = torch.from_numpy(np.concatenate([np.arange(cu[i], cu[i + 1]) for i in seqs]).astype(np.int32)).to(q.device)
+        a = _Attn4Args()
         if tiles is not None:
             a.tile_seq, a.tile_row0 = tiles.data_ptr(), tiles.data_ptr() + 4 * n_tiles
-        a.num_tiles = n_tiles
-        a.num_merge_tokens = ctx.num_tokens
+        a.num_tiles, a.num_seqs, a.nq, a.nkv, a.num_merge_tokens = n_tiles, ctx.num_seqs, nq, nkv, ctx.num_tokens
+        a.window, a.chunk, a.keep_first = window, chunk, keep_first
         if tokens is not None:
             a.merge_tokens, a.num_merge_tokens = tokens.data_ptr(), tokens.numel()
         # a captured step is launched for its bucket's lengths, and told the lengths of its moment beside
         lens = (ctx.scratch.get("attn_lens") if subset is None else None) or kv_lens
         most_q = max(q_lens)
-        most = self.attention4_blocks(max(kv_lens), most_q, a.window, a.chunk, a.keep_first)
-        total = sum(self.attention4_blocks(n, most_q, a.window, a.chunk, a.keep_first) for n in lens)
+        most = self.attention4_blocks(max(kv_lens), most_q, window, chunk, keep_first)
+        total = sum(self.attention4_blocks(n, most_q, window, chunk, keep_first) for n in lens)
         splits = ctx.scratch.get("attn_splits")
-        a.piece = max(-(-most // splits), -(-most // 1024)) if splits else self.choose_attention4_piece(most, total, n_tiles, a.nkv, keys)
+        a.piece = max(-(-most // splits), -(-most // 1024)) if splits else self.choose_attention4_piece(most, total, n_tiles, nkv, keys)
         a.pieces = -(-most // a.piece)
-        if a.pieces > 1:
-            parts = ctx.num_tokens * a.nq * a.pieces
-            room = torch.empty((parts * (d + 2),), dtype=torch.float32, device=q.device)
-            a.part_o, a.part_ml = room.data_ptr(), room.data_ptr() + 4 * parts * d
-        lib = attention4_library(d)
-        self._check(lib, lib.qrt_attention4(byref(a), c_int(_CODE[q.dtype]), c_int(int(keys)), c_int(row_tiles), _stream()))
+        return bytes(a), int(keys), row_tiles, ctx.num_tokens * nq * a.pieces if a.pieces > 1 else 0, (tiles, tokens)
 
     @staticmethod
     def choose_attention4_piece(most: int, total: int, tiles: int, nkv: int, keys: bool) -> int:
         """Blocks of 32 keys that one block of the launch walks."""
-        if keys:  # about 1,024 blocks of the launch, four waves of each with two blocks of keys or more, 64 pieces at most
-            return max(8, -(-total * nkv // 1024), -(-most // 64))
+        if keys:  # about 512 blocks of the launch, four waves of each with two blocks of keys or more, 64 pieces at most
+            return max(8, -(-total * nkv // 512), -(-most // 64))
         launch = tiles * nkv
         return most if launch >= 512 else max(16, -(-most // -(-512 // launch)))
 

@@ -218,20 +218,18 @@ def test_a_weight_that_is_not_finite_is_refused():
 
 
 def test_entry_points_refuse_sizes_on_the_host():
-    from ctypes import c_float, c_int, c_void_p
+    from ctypes import c_int, c_void_p
 
     from qwen3_runtime_amd.ops.hip import HipOps
 
     lib, p = HipOps().lib, c_void_p(1 << 20)  # not read: the sizes are refused
-    rows = lambda m, n, k, width, act=-1, dtype=1, x=None: lib.qrt_int8_rows(  # noqa: E731
-        x, c_int(1), p, p, p, p, p, c_int(dtype), c_int(m), c_int(n), c_int(k), c_int(width), c_int(act), c_float(0), None)
-    for bad in ((65, 16, 128, 128), (1, 0, 128, 128), (1, 16, 128, 100), (1, 16, 200, 128), (1, 16, 0, 128), (1, 16, 1 << 18, 1 << 18), (-1, 16, 128, 128)):
-        assert rows(*bad) != 0
-    assert rows(1, 16, 128, 128, act=2) != 0 and rows(1, 16, 128, 128, dtype=2) != 0 and rows(16, 16, 9728, 9728, x=p) != 0
-    tiles = lambda m, n, width, tile=0, act=-1, dtype=1: lib.qrt_int8_tiles(  # noqa: E731
-        p, p, p, p, p, c_int(dtype), c_int(m), c_int(n), c_int(width), c_int(tile), c_int(act), c_float(0), None)
-    for bad in ((1, 16, 100), (1, 0, 128), (-1, 16, 128), (1 << 20, 16, 1 << 13), (1, 16, 128, 14), (1, 16, 128, 0, 2), (1, 16, 128, 0, -1, 2)):
-        assert tiles(*bad) != 0
+    product = lambda m, n, k, width, tile=0, act=-1, dtype=1, out=1, work=p, x=p: lib.qrt_int8_product(  # noqa: E731
+        x, dtype, p, p, p, out, work, m, n, k, width, tile, act, 0.0, None)
+    for bad in ((1, 0, 128, 128), (1, 16, 128, 100), (1, 16, 200, 128), (1, 16, 0, 128), (1, 16, 1 << 18, 1 << 18), (-1, 16, 128, 128)):
+        assert product(*bad) != 0, bad
+    for bad in (dict(act=2), dict(dtype=2), dict(out=2), dict(work=None), dict(work=c_void_p(8))):
+        assert product(5, 16, 128, 128, **bad) != 0, bad
+    assert product(1, 16, 128, 128, x=c_void_p((1 << 20) + 2)) != 0
     quantize = lambda m, k, width, dtype=1: lib.qrt_quantize_rows(p, c_int(dtype), p, p, c_int(m), c_int(k), c_int(width), None)  # noqa: E731
     for bad in ((1, 129, 128), (1, 0, 128), (-1, 128, 128), (1, 128, 136), (1, 128, 128, 2)):
         assert quantize(*bad) != 0
