@@ -130,11 +130,13 @@ struct Int8Rows {
 };
 
 // Rows that a block turns into codes itself (FUSED): up to four, a row to each of its four waves, or to two or all four of them; a lane
-// has ITS pieces of 8 columns, in registers from the loads to the codes.
+// has ITS pieces of 8 columns, in registers from the loads to the codes. Every block does so again, so it pays while blocks are few: us
+// with a kernel in front and fused at 1 and 4 rows 6,144 x 2,560 7.0, 7.1 and 4.5, 5.2; 6,144 x 4,096 9.0, 9.1 and 6.0, 6.5; gated, 9,728 x 2,560
+// (1,216 blocks) 12.0, 12.1 and 11.7, 13.7, 12,288 x 4,096 (1,536) 18.5, 18.6 and 21.3, 24.1.
 constexpr int FUSED_MOST = 10;
 constexpr int fused_parts(int M) { return M == 1 ? 4 : M == 2 ? 2 : 1; }
 constexpr int fused_its(int M, int width) { return (width / 8 + 64 * fused_parts(M) - 1) / (64 * fused_parts(M)); }
-constexpr bool fused_takes(int M, int width) { return M >= 1 && M <= 4 && fused_its(M, width) <= FUSED_MOST; }
+constexpr bool fused_takes(int M, int N, int width) { return M >= 1 && M <= 4 && N <= 8 * 1100 && fused_its(M, width) <= FUSED_MOST; }
 
 // NW waves; WU units of eight weight rows (1: the operand's rows 8 to 15 repeat the others); MB blocks of 16 rows of the
 // activations (FEW: eight); GATED: half of the units are gate rows, half the up rows that belong to them.
@@ -158,7 +160,7 @@ __global__ __launch_bounds__(64 * NW) void int8_rows_kernel(Int8Rows p) {
 
   // FUSED: the rows come first, and are waited for behind the weights' loads
   float v[FUSED ? ITS : 1][8];
-  const int parts = fused_parts(p.M), own_row = wave / parts, own_at = 8 * ((wave - own_row * parts) * 64 + lane);
+  const int parts = fused_parts(p.M), code_rows = 4 / parts, own_row = wave / parts, own_at = 8 * ((wave - own_row * parts) * 64 + lane);
   if constexpr (FUSED) {
 #pragma unroll
     for (int j = 0; j < ITS; ++j)
@@ -207,7 +209,7 @@ __global__ __launch_bounds__(64 * NW) void int8_rows_kernel(Int8Rows p) {
         const int at = own_at + 512 * parts * j;
         typedef unsigned u32x2_t __attribute__((ext_vector_type(2)));
         // piece c of 16 columns of a stage's row r lies at 16 (c ^ (r & 7)), as in the rings
-        unsigned char* to = own_codes + (size_t)(at >> 7) * 1024 + own_row * 128 + 16 * (((at >> 4) & 7) ^ own_row) + (at & 8);
+        unsigned char* to = own_codes + (size_t)((at >> 7) * code_rows + own_row) * 128 + 16 * (((at >> 4) & 7) ^ own_row) + (at & 8);
         if (at < width) *(u32x2_t*)to = (u32x2_t){codes4(v[j][0], v[j][1], v[j][2], v[j][3], by), codes4(v[j][4], v[j][5], v[j][6], v[j][7], by)};
       }
     }
@@ -220,16 +222,16 @@ __global__ __launch_bounds__(64 * NW) void int8_rows_kernel(Int8Rows p) {
   for (int t = 0; t < NT; ++t)
 #pragma unroll
     for (int b = 0; b < MB; ++b) acc[t][b] = (i32x4_t){0, 0, 0, 0};
-  const int rw = WU == 1 ? r16 & 7 : r16, ra = FEW ? r16 & 7 : r16;
+  const int rw = WU == 1 ? r16 & 7 : r16, ra = FUSED ? r16 & (code_rows - 1) : FEW ? r16 & 7 : r16;
   const int w_at[2] = {rw * 128 + 16 * (quad ^ (r16 & 7)), rw * 128 + 16 * ((4 + quad) ^ (r16 & 7))};
-  const int a_at[2] = {ra * 128 + 16 * (quad ^ (r16 & 7)), ra * 128 + 16 * ((4 + quad) ^ (r16 & 7))};
+  const int a_at[2] = {ra * 128 + 16 * (quad ^ (ra & 7)), ra * 128 + 16 * ((4 + quad) ^ (ra & 7))};
   int slot = 0;
   for (int i = 0; i < mine; ++i) {
     // step i has landed when at most the U - 1 steps fetched after it are still on their way
     if (fetched - i == U) QRT_WAIT_LOADS((U - 1) * LOADS);
     else QRT_WAIT_LOADS(0);
     const unsigned char* at = ring + slot * SLOT;
-    const unsigned char* codes = FUSED ? own_codes + (size_t)(wave + i * NW) * 1024 : at + WU * 1024;
+    const unsigned char* codes = FUSED ? own_codes + (size_t)((wave + i * NW) * code_rows) * 128 : at + WU * 1024;
     i32x4_t w[NT][2], a[MB][2];
 #pragma unroll
     for (int h = 0; h < 2; ++h) {
@@ -288,7 +290,7 @@ template <int NW, int WU, int MB, bool FEW, int U, bool GATED, int ITS, typename
 static int launch_int8_rows(const Int8Rows& p, hipStream_t stream) {
   constexpr int NT = WU == 1 ? 1 : WU / 2, AU = FEW ? 1 : 2 * MB, OUTS = GATED ? 4 * WU : 8 * WU;
   constexpr size_t rings = (size_t)NW * U * (WU + (ITS ? 0 : AU)) * 1024, meet = (size_t)NW * NT * MB * 1024, most = 150 * 1024;
-  const size_t smem = (rings > meet ? rings : meet) + (ITS ? (size_t)p.width / INT8_STAGE * 1024 : 0);
+  const size_t smem = (rings > meet ? rings : meet) + (ITS ? (size_t)p.width * (4 / fused_parts(p.M)) : 0);
   static_assert(rings <= most, "the rings of this configuration do not fit LDS");
   QRT_CHECK(smem <= most, "int8_rows: %d columns need %zu bytes of LDS", p.width, smem);
   auto kernel = int8_rows_kernel<NW, WU, MB, FEW, U, GATED, ITS, TX, TO>;
@@ -315,9 +317,16 @@ template <bool GATED, typename TO>
 static int rows_by_size(const Int8Rows& p, hipStream_t stream) {
   if (p.M <= 8) return launch_int8_rows<4, 2, 1, true, 4, GATED, 0, float, TO>(p, stream);
   if (p.M <= 16) return launch_int8_rows<4, 2, 1, false, 4, GATED, 0, float, TO>(p, stream);
-  if (p.M <= 32) return launch_int8_rows<4, 2, 2, false, 3, GATED, 0, float, TO>(p, stream);
-  if (p.M <= 48) return launch_int8_rows<4, 4, 3, false, 2, GATED, 0, float, TO>(p, stream);
-  return launch_int8_rows<4, 4, 4, false, 2, GATED, 0, float, TO>(p, stream);
+  // 32 weight rows a block fetch the activations half as often, where they leave as many blocks as compute units
+  if (p.M <= 32) {
+    if (p.N * (GATED ? 2 : 1) < 32 * 512) return launch_int8_rows<4, 2, 2, false, 3, GATED, 0, float, TO>(p, stream);
+    return launch_int8_rows<4, 4, 2, false, 2, GATED, 0, float, TO>(p, stream);
+  }
+  if (p.N * (GATED ? 2 : 1) < 32 * 192) {
+    if (p.M <= 48) return launch_int8_rows<4, 2, 3, false, 2, GATED, 0, float, TO>(p, stream);
+    return launch_int8_rows<4, 2, 4, false, 2, GATED, 0, float, TO>(p, stream);
+  }
+  return launch_int8_rows<4, 4, 3, false, 2, GATED, 0, float, TO>(p, stream);
 }
 
 // c [M, N] of up to 64 rows. Either x (rows as they are, in x_dtype: those that fused_takes, of a multiple of 8 columns) or a and a_scale.
@@ -337,16 +346,17 @@ static int int8_rows(const void* x, int x_dtype, const void* a, const float* a_s
 #undef GO
 }
 
-// Rows up to which the weight is streamed past them; more go by tiles.
-constexpr int STREAMED_ROWS = 64;
+// Whether the weight is streamed past the rows; more go by tiles. us by streams and tiles at 48 and 64 rows: 6,144 x 4,096 12.5, 14.0 and 14.0, 14.0; gated
+// 9,728 x 2,560 19.7, 25.4 and 21.2, 21.2; 2,560 x 9,728 19.9, 23.0 and 26.3, 26.3.
+constexpr bool streams(int M, int N, bool gated) { return M <= 48 || (M <= 64 && N * (gated ? 2 : 1) < 32 * 192); }
 
 // Bytes of workspace that qrt_int8_product wants: none, or the rows' codes and scales.
-extern "C" int64_t qrt_int8_workspace(int M, int K, int width) {
-  return K % 8 == 0 && fused_takes(M, width) ? 0 : (int64_t)M * width + 4 * (((int64_t)M + 3) & ~3ll);
+extern "C" int64_t qrt_int8_workspace(int M, int N, int K, int width) {
+  return K % 8 == 0 && fused_takes(M, N, width) ? 0 : (int64_t)M * width + 4 * (((int64_t)M + 3) & ~3ll);
 }
 
 // c [M, N] (out_dtype) = rows x [M, K] (x_dtype) by w [N, width] and w_scale [N], or with a gate (act_kind >= 0) w [2 N, width], w_scale [2 N] and the activation
-// of the two. tile: a number of TILES in ops/hip.py, for more than 64 rows.
+// of the two. tile: a number of TILES in ops/hip.py, for more than 48 rows.
 extern "C" int qrt_int8_product(const void* x, int x_dtype, const void* w, const float* w_scale, void* c, int out_dtype, void* workspace, int M, int N,
                                 int K, int width, int tile, int act_kind, float limit, hipStream_t stream) {
   if (check_width("int8_product", M, K, width)) return -1;
@@ -355,7 +365,7 @@ extern "C" int qrt_int8_product(const void* x, int x_dtype, const void* w, const
   QRT_CHECK(out_dtype == QRT_BF16 || out_dtype == QRT_F32, "int8_product: unknown output dtype %d", out_dtype);
   QRT_CHECK(act_kind <= QRT_ACT_CLAMPED, "int8_product: unknown activation %d", act_kind);
   QRT_CHECK(((uintptr_t)w | (uintptr_t)c | (uintptr_t)workspace) % 16 == 0, "int8_product: operands must begin at multiples of 16 bytes");
-  const int64_t room = qrt_int8_workspace(M, K, width);
+  const int64_t room = qrt_int8_workspace(M, N, K, width);
   QRT_CHECK(room == 0 || workspace, "int8_product: %d rows of %d columns need a workspace", M, K);
   QRT_CHECK(room > 0 || (uintptr_t)x % 16 == 0, "int8_product: rows must begin at a multiple of 16 bytes");
   if (M == 0) return 0;
@@ -363,6 +373,6 @@ extern "C" int qrt_int8_product(const void* x, int x_dtype, const void* w, const
   int8_t* const codes = (int8_t*)workspace;
   float* const scale = (float*)(codes + (int64_t)M * width);
   if (qrt_quantize_rows(x, x_dtype, codes, scale, M, K, width, stream)) return -1;
-  if (M <= STREAMED_ROWS) return int8_rows(nullptr, x_dtype, codes, scale, w, w_scale, c, out_dtype, M, N, K, width, act_kind, limit, stream);
+  if (streams(M, N, act_kind >= 0)) return int8_rows(nullptr, x_dtype, codes, scale, w, w_scale, c, out_dtype, M, N, K, width, act_kind, limit, stream);
   return int8_tiles(codes, scale, w, w_scale, c, out_dtype, M, N, width, tile, act_kind, limit, stream);
 }

@@ -365,7 +365,7 @@ class HipOps:
         self.lib = core_library()
         # declared, the arguments travel as they are: a wrapper object for each of fifteen took 2 us a call
         self.lib.qrt_int8_product.argtypes = [c_void_p, c_int, c_void_p, c_void_p, c_void_p, c_int, c_void_p] + [c_int] * 6 + [c_float, c_void_p]
-        self.lib.qrt_int8_workspace.argtypes, self.lib.qrt_int8_workspace.restype = [c_int] * 3, c_long
+        self.lib.qrt_int8_workspace.argtypes, self.lib.qrt_int8_workspace.restype = [c_int] * 4, c_long
         self.residual_planes = residual_planes
 
     def _check(self, lib, code: int) -> None:
@@ -1683,7 +1683,7 @@ class HipOps:
 
     def _int8_product(self, x, w, out_f32=False, gate=None):
         """The product of rows by an ``Int8Weight``; ``gate`` = (activation, limit): gate rows, then up rows, and the activation of the two.
-        Up to 64 rows go past the weight as it streams, more by tiles; up to four short ones are quantised by the kernel that multiplies them."""
+        Up to 48 rows (64 by few outputs) go past the weight as it streams, more by tiles; up to four by few outputs are quantised by the kernel that multiplies them."""
         if isinstance(x, ScaledRows):
             x = x.made()
         values, scale, (n, k), width = w.values, w.scale, w.shape, w.width
@@ -1705,10 +1705,10 @@ class HipOps:
             return out
         if x.data_ptr() % 16:
             x = x.clone()
-        room = 0 if m <= 4 and lib.qrt_int8_workspace(m, k, width) == 0 else m * width + 16 * (m // 4 + 1)
+        room = 0 if m <= 4 and lib.qrt_int8_workspace(m, n, k, width) == 0 else m * width + 16 * (m // 4 + 1)
         work = torch.empty(room, dtype=torch.uint8, device=device).data_ptr() if room else None
         # 128 columns of bytes are a stage, as 64 of bfloat16 are: the same bytes and the same cycles of the matrix cores
-        tile = self.choose_tile(m, n, width // 2, form)[0] if m > 64 else 0
+        tile = self.choose_tile(m, n, width // 2, form)[0] if m > 48 else 0
         if lib.qrt_int8_product(x.data_ptr(), _CODE[dtype], values.data_ptr(), scale.data_ptr(), out.data_ptr(), F32 if out_f32 else _CODE[dtype],
                                 work, m, n, k, width, tile, act, limit, _stream()):
             raise OpsError(lib.qrt_last_error().decode())
