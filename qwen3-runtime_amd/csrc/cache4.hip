@@ -89,17 +89,160 @@ __global__ __launch_bounds__(256) void store4_kernel(Store4Args a) {
   }
 }
 
-// k, v [tokens, heads, dim] with their tokens k_stride and v_stride elements apart; slots[t] = page * page_size + offset, tokens whose
-// slot is in no page are left out.
-extern "C" int qrt_store4(const void* k, const void* v, int dtype, int64_t k_stride, int64_t v_stride, void* k_pages, void* v_pages, void* steps,
-                          const int* slots, int64_t num_pages, int tokens, int heads, int dim, int page_size, hipStream_t stream) {
+// Few tokens: q/k norm, rotation, the queries' store and the quantising store of keys and values in one kernel, a wave a head. A lane has
+// pairs of elements that turn together, as the rotation of a whole cache has them for few tokens (the same sums, the same bits of the
+// queries, keys rounded to the activations' type before they are quantised); codes meet in LDS, a byte an element, to be packed. A decode
+// step's store cost a kernel of 3 us more without it.
+struct Norm4Args {
+  const void* qkv;  // [tokens, stride]: q, k and v heads
+  int64_t stride;
+  const float* q_weight;  // null: no norm
+  const float* k_weight;
+  const float* inv_freq;  // null: no rotation
+  const int* positions;
+  void* q_out;
+  int nq, rot_pairs;
+  float eps;
+};
+
+template <typename T>
+__global__ __launch_bounds__(256) void norm_store4_kernel(Norm4Args n, Store4Args a) {
+  __shared__ __align__(8) uint8_t codes_of[4][256];
+  const int lane = threadIdx.x & 63, wave = uniform_wave_number();
+  const int heads = n.nq + 2 * a.heads, D = a.dim, half = D >> 1, rp = n.rot_pairs;
+  const int item = blockIdx.x * 4 + wave, t = item / heads, h = item - t * heads;
+  if (t >= a.tokens) return;
+  const bool is_q = h < n.nq, value = h >= n.nq + a.heads;
+  const T* src = (const T*)n.qkv + (size_t)t * n.stride + (size_t)h * D;
+  const float* w = is_q ? n.q_weight : value ? nullptr : n.k_weight;
+  const bool turns = n.inv_freq && !value;
+  // pair p: elements p and rp + p where it turns; behind those the others
+  auto first_of = [&](int p) { return p < rp ? p : p + rp; };
+  auto second_of = [&](int p) { return p < rp ? p + rp : p + half; };
+  float x1[2], x2[2], w1[2], w2[2], fr[2];
+  float ss = 0.f;
+  const float pos = turns ? (float)n.positions[t] : 0.f;
+  const int64_t slot = is_q ? 0 : a.slots[t];
+#pragma unroll
+  for (int i = 0; i < 2; ++i) {
+    const int p = lane + 64 * i;
+    x1[i] = x2[i] = fr[i] = 0.f, w1[i] = w2[i] = 1.f;
+    if (p < half) {
+      x1[i] = to_f32<T>(src[first_of(p)]), x2[i] = to_f32<T>(src[second_of(p)]);
+      if (w) w1[i] = w[first_of(p)], w2[i] = w[second_of(p)];
+      if (turns && p < rp) fr[i] = n.inv_freq[p];
+    }
+  }
+#pragma unroll
+  for (int i = 0; i < 2; ++i) ss += x1[i] * x1[i] + x2[i] * x2[i];
+  if (w) {
+    ss = wave_sum(ss);
+    const float inv = rsqrtf(ss / (float)D + n.eps);
+#pragma unroll
+    for (int i = 0; i < 2; ++i) x1[i] = x1[i] * inv * w1[i], x2[i] = x2[i] * inv * w2[i];
+  }
+  if (turns) {
+#pragma unroll
+    for (int i = 0; i < 2; ++i) {
+      if (lane + 64 * i < rp) {
+        float sn, c;
+        sincos_angle(pos * fr[i], &sn, &c);
+        const float y1 = x1[i] * c - x2[i] * sn, y2 = x2[i] * c + x1[i] * sn;
+        x1[i] = y1, x2[i] = y2;
+      }
+    }
+  }
+  if (is_q) {
+    T* to = (T*)n.q_out + ((size_t)t * n.nq + h) * D;
+#pragma unroll
+    for (int i = 0; i < 2; ++i) {
+      const int p = lane + 64 * i;
+      if (p < half) to[first_of(p)] = from_f32<T>(x1[i]), to[second_of(p)] = from_f32<T>(x2[i]);
+    }
+    return;
+  }
+  float low = INFINITY, high = -INFINITY;
+  bool bad = false;
+#pragma unroll
+  for (int i = 0; i < 2; ++i) {
+    if (lane + 64 * i >= half) continue;
+    x1[i] = to_f32<T>(from_f32<T>(x1[i])), x2[i] = to_f32<T>(from_f32<T>(x2[i]));
+    low = fminf(low, fminf(x1[i], x2[i])), high = fmaxf(high, fmaxf(x1[i], x2[i]));
+    bad |= !(fabsf(x1[i]) < INFINITY) || !(fabsf(x2[i]) < INFINITY);
+  }
+  bool broken = __builtin_amdgcn_ballot_w64(bad) != 0;
+  high = wave_max(high), low = -wave_max(-low);
+  const bf16_t lo16 = (bf16_t)low;
+  const float lo = (float)lo16;
+  const bf16_t step16 = (bf16_t)((high - lo) / 15.0f);
+  const float step = (float)step16;
+  broken |= !(step < INFINITY);
+  const bool flat = broken || !(step > 0.f);
+#pragma unroll
+  for (int i = 0; i < 2; ++i) {
+    const int p = lane + 64 * i;
+    if (p < half) {
+      codes_of[wave][first_of(p)] = flat ? 0 : (uint8_t)fminf(fmaxf(rintf((x1[i] - lo) / step), 0.f), 15.f);
+      codes_of[wave][second_of(p)] = flat ? 0 : (uint8_t)fminf(fmaxf(rintf((x2[i] - lo) / step), 0.f), 15.f);
+    }
+  }
+  __builtin_amdgcn_wave_barrier();  // a wave's reads of LDS come behind its writes
+  if (slot < 0 || slot >= a.num_slots) return;
+  const int head = h - n.nq - (value ? a.heads : 0);
+  const int64_t page = slot / a.page_size;
+  const int off = (int)(slot - page * a.page_size);
+  const int64_t row = (page * a.heads + head) * a.page_size + off;
+  if (lane == 0) {
+    a.steps[2 * row + value] = broken ? 0x7fc0u : (unsigned)__builtin_bit_cast(unsigned short, lo16) | (flat ? 0u : (unsigned)__builtin_bit_cast(unsigned short, step16) << 16);
+  }
+#pragma unroll
+  for (int i = 0; i < 2; ++i) {
+    const int b = lane + 64 * i;  // a byte of D / 2
+    if (b >= half) continue;
+    if (!value) {
+      a.k_pages[row * half + b] = codes_of[wave][2 * b] | codes_of[wave][2 * b + 1] << 4;
+    } else {
+      const int words = D / 32, c = b / words, e = 32 * (b - c * words) + c;
+      a.v_pages[(row - (off & 3)) * half + 4 * b + (off & 3)] = codes_of[wave][e] | codes_of[wave][e + 16] << 4;
+    }
+  }
+}
+
+static int check_store4(int dtype, int64_t num_pages, int tokens, int heads, int dim, int page_size, const void* k_pages, const void* v_pages, const void* steps) {
   QRT_CHECK(dtype == QRT_BF16 || dtype == QRT_F32, "store4: unknown dtype %d", dtype);
   QRT_CHECK(tokens >= 0 && heads > 0 && num_pages >= 0, "store4: bad sizes tokens=%d heads=%d", tokens, heads);
   QRT_CHECK(dim >= 32 && dim <= 256 && dim % 32 == 0, "store4: heads of 32 to 256 in steps of 32, not %d", dim);
   QRT_CHECK(page_size >= 4 && page_size % 4 == 0, "store4: pages of a multiple of 4 tokens, not %d", page_size);
+  QRT_CHECK(((uintptr_t)k_pages | (uintptr_t)v_pages | (uintptr_t)steps) % 16 == 0, "store4: pages must begin at multiples of 16 bytes");
+  return 0;
+}
+
+// qkv [tokens, stride]: nq heads of queries, nkv of keys and nkv of values. Weights may be null (no norm), inv_freq too (no rotation; otherwise rot_pairs
+// frequencies). q_out [tokens, nq, dim]. Tokens whose slot is in no page store nothing.
+extern "C" int qrt_norm_store4(const void* qkv, int dtype, int64_t stride, const float* q_weight, const float* k_weight, float eps, const float* inv_freq,
+                               const int* positions, int rot_pairs, void* q_out, void* k_pages, void* v_pages, void* steps, const int* slots, int64_t num_pages,
+                               int tokens, int nq, int nkv, int dim, int page_size, hipStream_t stream) {
+  if (check_store4(dtype, num_pages, tokens, nkv, dim, page_size, k_pages, v_pages, steps)) return -1;
+  QRT_CHECK(nq > 0 && stride >= (int64_t)(nq + 2 * nkv) * dim, "norm_store4: rows of %lld for %d + 2 * %d heads of %d", (long long)stride, nq, nkv, dim);
+  QRT_CHECK(!inv_freq || (positions && rot_pairs >= 1 && rot_pairs <= dim / 2), "norm_store4: %d pairs turn in heads of %d", rot_pairs, dim);
+  QRT_CHECK((int64_t)tokens * (nq + 2 * nkv) < (1ll << 31), "norm_store4: too many tokens for one launch (%d)", tokens);
+  if (tokens == 0) return 0;
+  const Norm4Args n{qkv, stride, q_weight, k_weight, inv_freq, positions, q_out, nq, inv_freq ? rot_pairs : dim / 2, eps};
+  const Store4Args a{nullptr, nullptr, (uint8_t*)k_pages, (uint8_t*)v_pages, (unsigned*)steps, slots, 0, 0, num_pages * page_size, tokens, nkv, dim, page_size};
+  const int blocks = (tokens * (nq + 2 * nkv) + 3) / 4;
+  if (dtype == QRT_BF16) norm_store4_kernel<bf16_t><<<blocks, 256, 0, stream>>>(n, a);
+  else norm_store4_kernel<float><<<blocks, 256, 0, stream>>>(n, a);
+  QRT_LAUNCH_CHECK("norm_store4");
+  return 0;
+}
+
+// k, v [tokens, heads, dim] with their tokens k_stride and v_stride elements apart; slots[t] = page * page_size + offset, tokens whose
+// slot is in no page are left out.
+extern "C" int qrt_store4(const void* k, const void* v, int dtype, int64_t k_stride, int64_t v_stride, void* k_pages, void* v_pages, void* steps,
+                          const int* slots, int64_t num_pages, int tokens, int heads, int dim, int page_size, hipStream_t stream) {
+  if (check_store4(dtype, num_pages, tokens, heads, dim, page_size, k_pages, v_pages, steps)) return -1;
   const int align = dtype == QRT_BF16 ? 8 : 4;
   QRT_CHECK(((uintptr_t)k | (uintptr_t)v) % 16 == 0 && k_stride % align == 0 && v_stride % align == 0, "store4: rows must begin at multiples of 16 bytes");
-  QRT_CHECK(((uintptr_t)k_pages | (uintptr_t)v_pages | (uintptr_t)steps) % 16 == 0, "store4: pages must begin at multiples of 16 bytes");
   if (tokens == 0) return 0;
   const Store4Args a{k, v, (uint8_t*)k_pages, (uint8_t*)v_pages, (unsigned*)steps, slots, k_stride, v_stride, num_pages * page_size, tokens, heads, dim, page_size};
   const int lanes = dim <= 32 ? 4 : dim <= 64 ? 8 : dim <= 128 ? 16 : 32;

@@ -116,6 +116,98 @@ extern "C" int qrt_quantize_rows(const void* x, int dtype, void* codes, float* s
   return 0;
 }
 
+// ---------------------------------------------------------------- a norm's rows as codes
+
+// residual += delta (or the sum of its planes, in their order), and the codes of the row's RMS norm, which is rounded to bfloat16 before where
+// the activations are: what add_rmsnorm and quantize_rows make, without the row between them. A block a row, all of it in registers.
+template <typename TD, int KEEP, bool ROUND>
+__global__ __launch_bounds__(256) void add_rmsnorm_codes_kernel(float* __restrict__ residual, const TD* __restrict__ delta, const float* __restrict__ weight,
+                                                                int8_t* __restrict__ codes, float* __restrict__ scale, int hidden, int width, float eps,
+                                                                int planes, size_t plane_stride) {
+  __shared__ float red[16];
+  __shared__ unsigned part[4];
+  float* x = residual + (size_t)blockIdx.x * hidden;
+  const TD* d = delta + (size_t)blockIdx.x * hidden;
+  f32x4_t v[KEEP], w[KEEP];
+  float squares = 0.f;
+#pragma unroll
+  for (int i = 0; i < KEEP; ++i) {
+    const int at = min(4 * ((int)threadIdx.x + 256 * i), hidden - 4);
+    v[i] = *(const f32x4_t*)(x + at), w[i] = *(const f32x4_t*)(weight + at);
+  }
+  if (planes > 0) {
+#pragma unroll
+    for (int i = 0; i < KEEP; ++i) {
+      const int at = min(4 * ((int)threadIdx.x + 256 * i), hidden - 4);
+      for (int p = 0; p < planes; ++p) {
+        typedef TD dvec_t __attribute__((ext_vector_type(4)));
+        const dvec_t y = *(const dvec_t*)(d + p * plane_stride + at);
+#pragma unroll
+        for (int e = 0; e < 4; ++e) v[i][e] += to_f32<TD>(y[e]);
+      }
+    }
+  }
+#pragma unroll
+  for (int i = 0; i < KEEP; ++i) {
+    const int at = 4 * ((int)threadIdx.x + 256 * i);
+    if (at >= hidden) v[i] = (f32x4_t){0.f, 0.f, 0.f, 0.f};
+    else if (planes > 0) *(f32x4_t*)(x + at) = v[i];
+    squares += (v[i][0] * v[i][0] + v[i][1] * v[i][1]) + (v[i][2] * v[i][2] + v[i][3] * v[i][3]);
+  }
+  const float by = rsqrtf(block_sum(squares, red) / (float)hidden + eps);
+  unsigned most = 0;
+#pragma unroll
+  for (int i = 0; i < KEEP; ++i)
+#pragma unroll
+    for (int e = 0; e < 4; ++e) {
+      v[i][e] = v[i][e] * by * w[i][e];
+      if (ROUND) v[i][e] = (float)(bf16_t)v[i][e];
+      most = max(most, magnitude_bits(v[i][e]));
+    }
+  most = wave_max_bits(most);
+  if ((threadIdx.x & 63) == 0) part[threadIdx.x >> 6] = most;
+  __syncthreads();
+  most = max(max(part[0], part[1]), max(part[2], part[3]));
+  const float factor = code_factor(most);
+#pragma unroll
+  for (int i = 0; i < KEEP; ++i) {
+    const int at = 4 * ((int)threadIdx.x + 256 * i);
+    if (at < width) *(unsigned*)(codes + (size_t)blockIdx.x * width + at) = codes4(v[i][0], v[i][1], v[i][2], v[i][3], factor);
+  }
+  if (threadIdx.x == 0) scale[blockIdx.x] = row_scale_of(most);
+}
+
+// Rows of up to 8,192 columns, a multiple of 4. delta may be null (planes 0).
+extern "C" int qrt_add_rmsnorm_codes(float* residual, const void* delta, int delta_dtype, const float* weight, void* codes, float* scale, int rows, int hidden,
+                                     int width, float eps, int planes, int64_t plane_stride, int round, hipStream_t stream) {
+  if (check_width("add_rmsnorm_codes", rows, hidden, width)) return -1;
+  QRT_CHECK(hidden % 4 == 0 && width <= 8192, "add_rmsnorm_codes: rows of %d", hidden);
+  QRT_CHECK(planes >= 0 && (planes == 0 || delta), "add_rmsnorm_codes: %d planes", planes);
+  QRT_CHECK(delta_dtype == QRT_BF16 || delta_dtype == QRT_F32, "add_rmsnorm_codes: unknown dtype %d", delta_dtype);
+  QRT_CHECK(((uintptr_t)residual | (uintptr_t)delta | (uintptr_t)weight | (uintptr_t)codes) % 16 == 0, "add_rmsnorm_codes: rows must begin at multiples of 16 bytes");
+  if (rows == 0) return 0;
+#define GO(TD, KEEP, ROUND) \
+  add_rmsnorm_codes_kernel<TD, KEEP, ROUND><<<rows, 256, 0, stream>>>(residual, (const TD*)delta, weight, (int8_t*)codes, scale, hidden, width, eps, planes, plane_stride)
+#define BY_WIDTH(TD, ROUND)                    \
+  do {                                         \
+    if (width <= 1024) GO(TD, 1, ROUND);       \
+    else if (width <= 2048) GO(TD, 2, ROUND);  \
+    else if (width <= 4096) GO(TD, 4, ROUND);  \
+    else GO(TD, 8, ROUND);                     \
+  } while (0)
+  if (delta_dtype == QRT_BF16) {
+    if (round) BY_WIDTH(bf16_t, true);
+    else BY_WIDTH(bf16_t, false);
+  } else {
+    if (round) BY_WIDTH(float, true);
+    else BY_WIDTH(float, false);
+  }
+#undef BY_WIDTH
+#undef GO
+  QRT_LAUNCH_CHECK("add_rmsnorm_codes");
+  return 0;
+}
+
 // ---------------------------------------------------------------- few rows
 
 struct Int8Rows {
@@ -356,8 +448,8 @@ extern "C" int64_t qrt_int8_workspace(int M, int N, int K, int width) {
 }
 
 // c [M, N] (out_dtype) = rows x [M, K] (x_dtype) by w [N, width] and w_scale [N], or with a gate (act_kind >= 0) w [2 N, width], w_scale [2 N] and the activation
-// of the two. tile: a number of TILES in ops/hip.py, for more than 48 rows.
-extern "C" int qrt_int8_product(const void* x, int x_dtype, const void* w, const float* w_scale, void* c, int out_dtype, void* workspace, int M, int N,
+// of the two. With codes_scale [M] (not null) x is codes already, [M, width]. tile: a number of TILES in ops/hip.py, for more than 48 rows.
+extern "C" int qrt_int8_product(const void* x, int x_dtype, const float* codes_scale, const void* w, const float* w_scale, void* c, int out_dtype, void* workspace, int M, int N,
                                 int K, int width, int tile, int act_kind, float limit, hipStream_t stream) {
   if (check_width("int8_product", M, K, width)) return -1;
   QRT_CHECK(N > 0 && N < (1 << 30), "int8_product: bad size N=%d", N);
@@ -365,6 +457,12 @@ extern "C" int qrt_int8_product(const void* x, int x_dtype, const void* w, const
   QRT_CHECK(out_dtype == QRT_BF16 || out_dtype == QRT_F32, "int8_product: unknown output dtype %d", out_dtype);
   QRT_CHECK(act_kind <= QRT_ACT_CLAMPED, "int8_product: unknown activation %d", act_kind);
   QRT_CHECK(((uintptr_t)w | (uintptr_t)c | (uintptr_t)workspace) % 16 == 0, "int8_product: operands must begin at multiples of 16 bytes");
+  if (codes_scale) {
+    QRT_CHECK((uintptr_t)x % 16 == 0, "int8_product: codes must begin at a multiple of 16 bytes");
+    if (M == 0) return 0;
+    if (streams(M, N, act_kind >= 0)) return int8_rows(nullptr, x_dtype, x, codes_scale, w, w_scale, c, out_dtype, M, N, K, width, act_kind, limit, stream);
+    return int8_tiles(x, codes_scale, w, w_scale, c, out_dtype, M, N, width, tile, act_kind, limit, stream);
+  }
   const int64_t room = qrt_int8_workspace(M, N, K, width);
   QRT_CHECK(room == 0 || workspace, "int8_product: %d rows of %d columns need a workspace", M, K);
   QRT_CHECK(room > 0 || (uintptr_t)x % 16 == 0, "int8_product: rows must begin at a multiple of 16 bytes");

@@ -330,6 +330,16 @@ class ScaledRows:
         return self.ops.add_rmsnorm(self.residual, None, self.weight, self.eps, self.rows.dtype)
 
 
+class CodedRows:
+    """Rows of an RMS norm as 8-bit codes [T, width] and a scale each (``HipOps.add_rmsnorm_codes``), for products of weights in 8 bits alone;
+    ``dtype`` is what the activations would have been in, and the products' results are."""
+
+    __slots__ = ("codes", "scale", "shape", "dtype")
+
+    def __init__(self, codes, scale, shape, dtype):
+        self.codes, self.scale, self.shape, self.dtype = codes, scale, shape, dtype
+
+
 class HipOps:
     # bfloat16 products with more rows than this are made by tiles or the vendor library
     own_max_rows = 64
@@ -364,7 +374,7 @@ class HipOps:
         only with few; for callers that hand its result to nothing but the norms and ``accumulate``."""
         self.lib = core_library()
         # declared, the arguments travel as they are: a wrapper object for each of fifteen took 2 us a call
-        self.lib.qrt_int8_product.argtypes = [c_void_p, c_int, c_void_p, c_void_p, c_void_p, c_int, c_void_p] + [c_int] * 6 + [c_float, c_void_p]
+        self.lib.qrt_int8_product.argtypes = [c_void_p, c_int, c_void_p, c_void_p, c_void_p, c_void_p, c_int, c_void_p] + [c_int] * 6 + [c_float, c_void_p]
         self.lib.qrt_int8_workspace.argtypes, self.lib.qrt_int8_workspace.restype = [c_int] * 4, c_long
         self.residual_planes = residual_planes
 
@@ -1681,19 +1691,41 @@ class HipOps:
                                                          c_int(width), _stream()))
         return codes, scale
 
+    def add_rmsnorm_codes(self, residual, delta, weight, eps, out_dtype):
+        """``quantize_rows(add_rmsnorm(residual, delta, weight, eps, out_dtype))`` as ``CodedRows``, in one kernel; the rows of more than 8,192
+        columns, or of no multiple of 4, as they are."""
+        if isinstance(delta, PendingProduct):
+            delta = delta.made()
+        t, h = residual.shape
+        width = -(-h // 128) * 128
+        if h % 4 or width > 8192:
+            return self.add_rmsnorm(residual, delta, weight, eps, out_dtype)
+        _need(residual, "residual", torch.float32)
+        _need(weight, "norm weight", torch.float32, (h,))
+        pd, cd, nd = (None, F32, 0) if delta is None else _planes(delta, t, h, "delta")
+        codes = torch.empty((t, width), dtype=torch.int8, device=residual.device)
+        scale = torch.empty((t,), dtype=torch.float32, device=residual.device)
+        self._check(self.lib, self.lib.qrt_add_rmsnorm_codes(
+            _ptr(residual), pd, c_int(cd), _ptr(weight), _ptr(codes), _ptr(scale), c_int(t), c_int(h), c_int(width), c_float(eps), c_int(nd),
+            c_long(t * h), c_int(int(out_dtype == torch.bfloat16)), _stream()))
+        return CodedRows(codes, scale, residual.shape, out_dtype)
+
     def _int8_product(self, x, w, out_f32=False, gate=None):
         """The product of rows by an ``Int8Weight``; ``gate`` = (activation, limit): gate rows, then up rows, and the activation of the two.
-        Up to 48 rows (64 by few outputs) go past the weight as it streams, more by tiles; up to four by few outputs are quantised by the kernel that multiplies them."""
+        Up to 48 rows (64 by few outputs) go past the weight as it streams, more by tiles; up to four by few outputs are quantised by
+        the kernel that multiplies them, ``CodedRows`` are codes already."""
         if isinstance(x, ScaledRows):
             x = x.made()
         values, scale, (n, k), width = w.values, w.scale, w.shape, w.width
-        dtype = x.dtype
-        if x.dim() != 2 or dtype not in _CODE or x.shape[1] != k:
+        dtype, coded = x.dtype, None
+        if len(x.shape) != 2 or dtype not in _CODE or x.shape[1] != k:
             raise OpsError(f"linear: x is {tuple(x.shape)} of {dtype}, the weight in 8 bits is {tuple(w.shape)}")
+        m, act, limit, form = x.shape[0], -1, 0.0, "whole"
+        if isinstance(x, CodedRows):
+            x, coded = x.codes, x.scale
         if not (x.is_cuda and x.is_contiguous() and x.device == values.device):
             _need(x, "x")
             raise OpsError(f"linear: x is on {x.device}, the weight on {values.device}")
-        m, act, limit, form = x.shape[0], -1, 0.0, "whole"
         if gate is not None:
             act, limit = ACTIVATIONS[gate[0]], gate[1]
             if act > ACTIVATIONS["clamped"] or n % 2:
@@ -1705,12 +1737,12 @@ class HipOps:
             return out
         if x.data_ptr() % 16:
             x = x.clone()
-        room = 0 if m <= 4 and lib.qrt_int8_workspace(m, n, k, width) == 0 else m * width + 16 * (m // 4 + 1)
+        room = 0 if coded is not None or (m <= 4 and lib.qrt_int8_workspace(m, n, k, width) == 0) else m * width + 16 * (m // 4 + 1)
         work = torch.empty(room, dtype=torch.uint8, device=device).data_ptr() if room else None
         # 128 columns of bytes are a stage, as 64 of bfloat16 are: the same bytes and the same cycles of the matrix cores
         tile = self.choose_tile(m, n, width // 2, form)[0] if m > 48 else 0
-        if lib.qrt_int8_product(x.data_ptr(), _CODE[dtype], values.data_ptr(), scale.data_ptr(), out.data_ptr(), F32 if out_f32 else _CODE[dtype],
-                                work, m, n, k, width, tile, act, limit, _stream()):
+        if lib.qrt_int8_product(x.data_ptr(), _CODE[dtype], None if coded is None else coded.data_ptr(), values.data_ptr(), scale.data_ptr(), out.data_ptr(),
+                                F32 if out_f32 else _CODE[dtype], work, m, n, k, width, tile, act, limit, _stream()):
             raise OpsError(lib.qrt_last_error().decode())
         return out
 
@@ -1770,6 +1802,9 @@ class HipOps:
     # every layer, instead of being computed in every layer's kernel
     rope_table_from_tokens = 256
 
+    # tokens up to which norm, rotation and the store into a cache of 4 bits are one kernel, a wave a head; more go by the kernel for many tokens
+    store4_together_tokens = 31
+
     def qk_norm_rope_store(self, qkv, nq, nkv, d, q_w, k_w, eps, inv_freq, positions, cache, ctx=None,
                            angles_key=None, value_dim=None, extra=0, value_turn=None):
         """Per-head RMSNorm of queries and keys, rotation of their first ``2 len(inv_freq)`` elements (first
@@ -1815,6 +1850,16 @@ class HipOps:
                 raise OpsError(f"turned values of {dv} take the step's context and {dv // 2} frequencies")
             a.v_rope = self.rope_table(ctx, *value_turn).data_ptr()
         pages, k = 0, None
+        if four and t <= self.store4_together_tokens:
+            cache_pages = self._check_cache4(cache, nkv, d)
+            _need(cache.group.slots, "slots", torch.int32, (t,))
+            if not (qkv.device == cache.k.device == cache.group.slots.device) or qkv.dtype not in _CODE:
+                raise OpsError(f"q, k and v of {qkv.dtype} on {qkv.device}, a cache on {cache.k.device}")
+            self._check(self.lib, self.lib.qrt_norm_store4(
+                _ptr(qkv), c_int(_CODE[qkv.dtype]), c_long(width), _ptr(q_w), _ptr(k_w), c_float(eps), _ptr(inv_freq), _ptr(positions if inv_freq is not None else None),
+                c_int(pairs if inv_freq is not None else 0), _ptr(q), _ptr(cache.k), _ptr(cache.v), _ptr(cache.pages["steps"]), _ptr(cache.group.slots),
+                c_long(cache_pages), c_int(t), c_int(nq), c_int(nkv), c_int(d), c_int(cache.group.page_size), _stream()))
+            return q
         if four:
             k = torch.empty((t, nkv * d), dtype=qkv.dtype, device=qkv.device)
             a.k_out, a.nv = k.data_ptr(), 0

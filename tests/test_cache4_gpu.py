@@ -313,24 +313,41 @@ def test_a_captured_step_is_the_eager_one():
 
 @gpu
 @pytest.mark.parametrize("dtype", [torch.bfloat16, torch.float32])
-def test_norm_rotation_and_store_together(dtype):
+@pytest.mark.parametrize("t,nq,nkv,d,pairs,norm", [(37, 6, 2, 64, 32, True), (1, 32, 8, 128, 64, True), (31, 4, 2, 96, 48, False), (5, 3, 1, 256, 32, True), (2, 2, 2, 32, None, True),
+                                                   (8, 5, 5, 160, 80, False), (100, 8, 2, 128, 64, True), (7, 2, 1, 224, 100, True), (3, 2, 1, 64, None, False)])
+def test_norm_rotation_and_store_together(t, nq, nkv, d, pairs, norm, dtype):
     """Queries as with an ordinary cache, and in the cache what the store makes of that one's keys and values."""
     from qwen3_runtime_amd.parts.base import CacheView, GroupView
     from qwen3_runtime_amd.parts.plan import CacheSpec
 
-    o, t, nq, nkv, d, ps, pages = ops(), 37, 6, 2, 64, 16, 4
-    qkv = torch.randn(t, (nq + 2 * nkv) * d, generator=gen(1)).to(dtype).to(DEV)
+    o, ps = ops(), 16
+    pages = t // ps + 3
+    qkv = torch.randn(t, (nq + 2 * nkv) * d + 8, generator=gen(1)).to(dtype).to(DEV)
     qw, kw = (1 + 0.1 * torch.randn(d, generator=gen(2))).to(DEV), (1 + 0.1 * torch.randn(d, generator=gen(3))).to(DEV)
-    freq = (1e4 ** -(torch.arange(d // 2) / (d // 2))).to(DEV)
-    pos, slots = torch.arange(t, dtype=torch.int32, device=DEV), torch.arange(5, 5 + t, dtype=torch.int32, device=DEV)
+    qw, kw = (qw, kw) if norm else (None, None)
+    freq = None if pairs is None else (1e4 ** -(torch.arange(pairs) / pairs)).to(DEV)
+    pos, slots = torch.arange(t, dtype=torch.int32, device=DEV) + 1000, torch.arange(5, 5 + t, dtype=torch.int32, device=DEV)
     whole = CacheView(CacheSpec("paged_kv", heads=nkv, head_dim=d), group=GroupView(ps, None, None, slots),
                       k=torch.zeros(pages, nkv, ps, d, dtype=dtype, device=DEV), v=torch.zeros(pages, nkv, d, ps, dtype=dtype, device=DEV))
     cache, want = empty_cache(pages, nkv, ps, d), empty_cache(pages, nkv, ps, d)
     cache.group.slots = slots
-    q = o.qk_norm_rope_store(qkv, nq, nkv, d, qw, kw, 1e-6, freq, pos, whole)
-    assert torch.equal(o.qk_norm_rope_store(qkv, nq, nkv, d, qw, kw, 1e-6, freq, pos, cache), q)
+    q = o.qk_norm_rope_store(qkv, nq, nkv, d, qw, kw, 1e-6, freq, pos, whole, extra=8)
+    assert torch.equal(o.qk_norm_rope_store(qkv, nq, nkv, d, qw, kw, 1e-6, freq, pos, cache, extra=8), q)
     at = slots.cpu().long()
     put(want, at // ps, at % ps, whole.k.cpu()[at // ps, :, at % ps], whole.v.cpu()[at // ps, :, :, at % ps], d)
+    same(cache, want)
+
+
+@gpu
+def test_few_tokens_whose_slot_is_in_no_page_store_nothing():
+    o, t, nq, nkv, d, ps = ops(), 4, 2, 1, 64, 16
+    qkv = torch.randn(t, (nq + 2 * nkv) * d, generator=gen(1)).to(DEV)
+    qkv[1, nq * d] = float("nan")
+    cache, want = empty_cache(2, nkv, ps, d), empty_cache(2, nkv, ps, d)
+    cache.group.slots = torch.tensor([-1, 3, 32, 2 ** 31 - 1], dtype=torch.int32, device=DEV)
+    o.qk_norm_rope_store(qkv, nq, nkv, d, None, None, 0.0, None, torch.zeros(t, dtype=torch.int32, device=DEV), cache)
+    k, v = qkv[1:2, nq * d: (nq + 1) * d].view(1, 1, d).cpu(), qkv[1:2, (nq + 1) * d:].view(1, 1, d).cpu()
+    put(want, torch.tensor([0]), torch.tensor([3]), k, v, d)
     same(cache, want)
 
 

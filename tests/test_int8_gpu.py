@@ -121,6 +121,32 @@ def test_gated_products(m, n, k, dtype):
 
 
 @gpu
+@pytest.mark.parametrize("planes", [0, 1, 3])
+@pytest.mark.parametrize("m,h,n", [(1, 96, 40), (5, 640, 304), (20, 2560, 301), (70, 1100, 64), (3, 8192, 32), (2, 8320, 32), (2, 102, 16)])
+@pytest.mark.parametrize("dtype", [torch.bfloat16, torch.float32])
+def test_a_norms_codes_and_their_products(m, h, n, planes, dtype):
+    """As the norm and the products behind it, apart; the norm's sums may be made in another order, which moves a code by one here and there (1 / 127 of
+    a row's largest element, of h elements)."""
+    o = ops()
+    delta = None if planes == 0 else rnd(planes, m, h, seed=4) if planes > 1 else rnd(m, h, seed=4, dtype=torch.bfloat16)
+    residual, weight, w = rnd(m, h, seed=1), 1 + rnd(h, seed=2) / 10, Int8Weight.quantize(rnd(n, h, seed=3))
+    one, other = residual.clone(), residual.clone()
+    rows = o.add_rmsnorm_codes(one, delta, weight, 1e-5, dtype)
+    plain = o.add_rmsnorm(other, delta, weight, 1e-5, dtype)
+    # planes join the stream one after the other, or their sum does
+    assert torch.allclose(one, other, rtol=0, atol=1e-5)
+    codes, scale = o.quantize_rows(plain)
+    if hasattr(rows, "codes"):
+        off = (rows.codes.int() - codes.int()).abs()
+        assert int(off.max()) <= 1 and float((off > 0).float().mean()) < 2e-3 and torch.allclose(rows.scale, scale, rtol=2 ** -7)
+    else:
+        assert h % 4 or h > 8192
+    for a, b in ((o.linear(rows, w), o.linear(plain, w)), (o.linear_for_residual(rows, w), o.linear_for_residual(plain, w)),
+                 (o.gated_linear(rows, w), o.gated_linear(plain, w)) if n % 2 == 0 else (weight, weight)):
+        assert a.dtype == b.dtype and float((a - b).double().norm()) <= 0.01 * float(b.double().norm())
+
+
+@gpu
 @pytest.mark.parametrize("m", [3, 20, 100])
 @pytest.mark.parametrize("bad", [float("nan"), float("inf"), float("-inf")])
 def test_rows_that_are_not_finite_are_nan_and_leave_the_others(m, bad):
@@ -223,13 +249,13 @@ def test_entry_points_refuse_sizes_on_the_host():
     from qwen3_runtime_amd.ops.hip import HipOps
 
     lib, p = HipOps().lib, c_void_p(1 << 20)  # not read: the sizes are refused
-    product = lambda m, n, k, width, tile=0, act=-1, dtype=1, out=1, work=p, x=p: lib.qrt_int8_product(  # noqa: E731
-        x, dtype, p, p, p, out, work, m, n, k, width, tile, act, 0.0, None)
+    product = lambda m, n, k, width, tile=0, act=-1, dtype=1, out=1, work=p, x=p, codes=None: lib.qrt_int8_product(  # noqa: E731
+        x, dtype, codes, p, p, p, out, work, m, n, k, width, tile, act, 0.0, None)
     for bad in ((1, 0, 128, 128), (1, 16, 128, 100), (1, 16, 200, 128), (1, 16, 0, 128), (1, 16, 1 << 18, 1 << 18), (-1, 16, 128, 128)):
         assert product(*bad) != 0, bad
     for bad in (dict(act=2), dict(dtype=2), dict(out=2), dict(work=None), dict(work=c_void_p(8))):
         assert product(5, 16, 128, 128, **bad) != 0, bad
-    assert product(1, 16, 128, 128, x=c_void_p((1 << 20) + 2)) != 0
+    assert product(1, 16, 128, 128, x=c_void_p((1 << 20) + 2)) != 0 and product(9, 16, 128, 128, x=c_void_p((1 << 20) + 2), codes=p) != 0
     quantize = lambda m, k, width, dtype=1: lib.qrt_quantize_rows(p, c_int(dtype), p, p, c_int(m), c_int(k), c_int(width), None)  # noqa: E731
     for bad in ((1, 129, 128), (1, 0, 128), (-1, 128, 128), (1, 128, 136), (1, 128, 128, 2)):
         assert quantize(*bad) != 0
