@@ -38,12 +38,13 @@ __device__ __forceinline__ void load_row8(const T* __restrict__ row, int at, int
   }
 }
 
-// THREADS to a row; KEEP pieces of 8 columns a thread stay in registers, wider rows are read a second time.
+// THREADS to a row (64, or a whole block); KEEP pieces of 8 columns a thread stay in registers, wider rows are read a second time.
 template <typename T, int THREADS, int KEEP, bool ALIGNED>
-__global__ __launch_bounds__(256) void quantize_rows_kernel(const T* __restrict__ x, int8_t* __restrict__ codes, float* __restrict__ scale, int M, int K, int width) {
-  __shared__ unsigned part[4];
+__global__ __launch_bounds__(THREADS > 256 ? THREADS : 256) void quantize_rows_kernel(const T* __restrict__ x, int8_t* __restrict__ codes, float* __restrict__ scale, int M, int K, int width) {
+  constexpr int WAVES = THREADS / 64;
+  __shared__ unsigned part[WAVES];
   const int t = threadIdx.x % THREADS;
-  const int row = blockIdx.x * (256 / THREADS) + threadIdx.x / THREADS;
+  const int row = THREADS < 256 ? blockIdx.x * (256 / THREADS) + threadIdx.x / THREADS : blockIdx.x;
   const T* src = x + (size_t)min(row, M - 1) * K;
   float v[KEEP][8];
   unsigned most = 0;
@@ -63,7 +64,9 @@ __global__ __launch_bounds__(256) void quantize_rows_kernel(const T* __restrict_
   if (THREADS > 64) {
     if ((threadIdx.x & 63) == 0) part[threadIdx.x >> 6] = most;
     __syncthreads();
-    most = max(max(part[0], part[1]), max(part[2], part[3]));
+    most = part[0];
+#pragma unroll
+    for (int i = 1; i < WAVES; ++i) most = max(most, part[i]);
   }
   if (row >= M) return;
   const float by = code_factor(most);
@@ -88,13 +91,16 @@ __global__ __launch_bounds__(256) void quantize_rows_kernel(const T* __restrict_
 template <typename T>
 static void launch_quantize(const T* x, int8_t* codes, float* scale, int M, int K, int width, hipStream_t stream) {
   const bool aligned = K % 8 == 0 && (uintptr_t)x % 16 == 0;
-#define GO(THREADS, KEEP, ALIGNED) \
-  quantize_rows_kernel<T, THREADS, KEEP, ALIGNED><<<dim3((M + 256 / THREADS - 1) / (256 / THREADS)), dim3(256), 0, stream>>>(x, codes, scale, M, K, width)
-  // a wave a row needs no barrier: 1,999 rows of 2,560 columns 6.8 us by blocks
+#define GO(THREADS, KEEP, ALIGNED)                                                                                                     \
+  quantize_rows_kernel<T, THREADS, KEEP, ALIGNED>                                                                                      \
+      <<<dim3(THREADS < 256 ? (M + 256 / THREADS - 1) / (256 / THREADS) : M), dim3(THREADS < 256 ? 256 : THREADS), 0, stream>>>(x, codes, scale, M, K, width)
+  // a wave a row needs no barrier: 1,999 rows of 2,560 columns 6.8 -> 4.2 us. Few long rows leave most compute units idle and are over as
+  // soon as one of them is: 1,024 threads.
   if (!aligned) GO(256, 4, false);
   else if (width <= 1024) GO(64, 2, true);
   else if (width <= 4096 && M >= 512) GO(64, 8, true);
   else if (width <= 4096) GO(256, 2, true);
+  else if (M < 256) GO(1024, 2, true);
   else GO(256, 5, true);
 #undef GO
 }
@@ -407,6 +413,11 @@ static int fused_by_size(const Int8Rows& p, hipStream_t stream) {
 }
 template <bool GATED, typename TO>
 static int rows_by_size(const Int8Rows& p, hipStream_t stream) {
+  if constexpr (!GATED) {  // blocks are no more than compute units: eight waves each
+    if (p.M <= 8 && p.N <= 4096) return launch_int8_rows<8, 2, 1, true, 4, false, 0, float, TO>(p, stream);
+    if (p.M <= 16 && p.N <= 4096) return launch_int8_rows<8, 2, 1, false, 4, false, 0, float, TO>(p, stream);
+    if (p.M <= 32 && p.N <= 4096) return launch_int8_rows<8, 2, 2, false, 3, false, 0, float, TO>(p, stream);
+  }
   if (p.M <= 8) return launch_int8_rows<4, 2, 1, true, 4, GATED, 0, float, TO>(p, stream);
   if (p.M <= 16) return launch_int8_rows<4, 2, 1, false, 4, GATED, 0, float, TO>(p, stream);
   // 32 weight rows a block fetch the activations half as often, where they leave as many blocks as compute units
