@@ -8,8 +8,8 @@
 // lanes and nothing goes through LDS. A block of 32 keys is on its way while another is multiplied, its page numbers one block before that.
 //
 // bfloat16 queries: OFF = 128, weights w in bfloat16 (their errors average out, as in every attention that multiplies
-// probabilities in 16 bits). float32 queries: q and w as three bfloat16 each (24 bits in all, whole), OFF = 16, which leaves three more bits
-// of a sum to what is wanted.
+// probabilities in 16 bits). float32 queries: q and w as three bfloat16 each (24 bits in all, whole), and OFF = -8, which leaves nothing to
+// take out: with an offset of 16 the results were 3.6e-6 from those in 64 bits, where sums in float32 are 2e-7.
 //
 // KEYS: up to 16 rows (token x head of the group); the four waves of a block take its blocks of keys in turn and meet in LDS. Otherwise a
 // wave has 16 RT rows of its own, and the four of a block read the same keys at about the same time. Either way a launch may cut the
@@ -108,23 +108,28 @@ struct Scales {
   float kmul[32], kadd[32], vstep[32], vmid[32];
 };
 
-// Nibbles `nibble` and `nibble` + 4 of x as a pair of bfloat16, OFF + n each. Mask and exponent are kept in registers where the compiler
-// does not see their values: it then takes one instruction, v_and_or_b32, for what two with literals would do.
+// Nibbles `nibble` and `nibble` + 4 of x as a pair of bfloat16, OFF + n each. OFF = 128: mask and exponent are kept in registers where the
+// compiler does not see their values: it then takes one instruction, v_and_or_b32, for what two with literals would do. OFF = -8: by way
+// of float32, five instructions a pair for two.
 template <int OFF>
-struct Place {
+struct Place;
+template <>
+struct Place<128> {
   unsigned mask, exponent;
   __device__ __forceinline__ Place() {
-    if constexpr (OFF == 128) {
-      asm("s_mov_b32 %0, 0x000f000f" : "=s"(mask));
-      asm("v_mov_b32 %0, 0x43004300" : "=v"(exponent));
-    } else {
-      asm("s_mov_b32 %0, 0x00780078" : "=s"(mask));
-      asm("v_mov_b32 %0, 0x41804180" : "=v"(exponent));
-    }
+    asm("s_mov_b32 %0, 0x000f000f" : "=s"(mask));
+    asm("v_mov_b32 %0, 0x43004300" : "=v"(exponent));
   }
+  __device__ __forceinline__ unsigned operator()(unsigned x, int nibble) const { return ((x >> (4 * nibble)) & mask) | exponent; }
+};
+template <>
+struct Place<-8> {
   __device__ __forceinline__ unsigned operator()(unsigned x, int nibble) const {
-    const unsigned y = OFF == 128 ? x >> (4 * nibble) : nibble == 0 ? x << 3 : x >> (4 * nibble - 3);
-    return (y & mask) | exponent;
+    const unsigned bytes = (nibble & 1 ? x >> 4 : x) & 0x0f0f0f0fu;
+    const int at = 8 * (nibble >> 1);
+    typedef bf16_t bf16x2_t __attribute__((ext_vector_type(2)));
+    const bf16x2_t pair = {(bf16_t)((float)(bytes >> at & 255u) - 8.f), (bf16_t)((float)(bytes >> (at + 16) & 255u) - 8.f)};
+    return __builtin_bit_cast(unsigned, pair);
   }
 };
 
@@ -132,7 +137,7 @@ constexpr float NOTHING = -3.4028235e38f;  // the reference of a row that has se
 
 template <int RT, int NS, bool CAP>
 struct Walk {
-  static constexpr int OFF = NS == 1 ? 128 : 16;
+  static constexpr int OFF = NS == 1 ? 128 : -8;
   Place<OFF> place;
   bf16x8_t q[NS][RT][KS];
   float qsum[RT];              // sum of the row's query, times the unit of the scores
@@ -317,11 +322,12 @@ struct Walk {
         }
     constexpr unsigned ONES = 0x3f803f80u;
     const u32x4_t ones = {ONES, ONES, ONES, ONES};
+    if constexpr (OFF != -8)
 #pragma unroll
-    for (int t = 0; t < RT; ++t)
+      for (int t = 0; t < RT; ++t)
 #pragma unroll
-      for (int n = 0; n < NS; ++n)
-        weights[t] = __builtin_amdgcn_mfma_f32_16x16x32_bf16(__builtin_bit_cast(bf16x8_t, ones), p[n][t], weights[t], 0, 0, 0);
+        for (int n = 0; n < NS; ++n)
+          weights[t] = __builtin_amdgcn_mfma_f32_16x16x32_bf16(__builtin_bit_cast(bf16x8_t, ones), p[n][t], weights[t], 0, 0, 0);
 #pragma unroll
     for (int w = 0; w < KS; ++w) {
       const unsigned x = st.v[0].w[w], y = st.v[1].w[w];
@@ -340,6 +346,7 @@ struct Walk {
   // The offsets of the codes out of the sums, which stay small so: what a sum of OFF w loses in its last places adds up over a long
   // walk to more than a flat softmax leaves of its values (32,000 keys: 0.8 % of them).
   __device__ __forceinline__ void center() {
+    if constexpr (OFF == -8) return;
 #pragma unroll
     for (int t = 0; t < RT; ++t) {
       const float off = -(float)(OFF + 8) * weights[t][0];

@@ -1710,20 +1710,25 @@ class HipOps:
             c_long(t * h), c_int(int(out_dtype == torch.bfloat16)), _stream()))
         return CodedRows(codes, scale, residual.shape, out_dtype)
 
+    @staticmethod
+    @functools.lru_cache(maxsize=4096)
+    def _int8_workspace(m: int, n: int, k: int, width: int) -> int:
+        return core_library().qrt_int8_workspace(m, n, k, width)
+
     def _int8_product(self, x, w, out_f32=False, gate=None):
         """The product of rows by an ``Int8Weight``; ``gate`` = (activation, limit): gate rows, then up rows, and the activation of the two.
         Up to 48 rows (64 by few outputs) go past the weight as it streams, more by tiles; up to four by few outputs are quantised by
         the kernel that multiplies them, ``CodedRows`` are codes already."""
         if isinstance(x, ScaledRows):
             x = x.made()
-        values, scale, (n, k), width = w.values, w.scale, w.shape, w.width
-        dtype, coded = x.dtype, None
-        if len(x.shape) != 2 or dtype not in _CODE or x.shape[1] != k:
-            raise OpsError(f"linear: x is {tuple(x.shape)} of {dtype}, the weight in 8 bits is {tuple(w.shape)}")
-        m, act, limit, form = x.shape[0], -1, 0.0, "whole"
+        values, (n, k), width = w.values, w.shape, w.width
+        dtype, shape, coded = x.dtype, x.shape, None
+        if len(shape) != 2 or dtype not in _CODE or shape[1] != k:
+            raise OpsError(f"linear: x is {tuple(shape)} of {dtype}, the weight in 8 bits is {tuple(w.shape)}")
+        m, act, limit, form = shape[0], -1, 0.0, "whole"
         if isinstance(x, CodedRows):
             x, coded = x.codes, x.scale
-        if not (x.is_cuda and x.is_contiguous() and x.device == values.device):
+        if x.get_device() < 0 or x.get_device() != values.get_device() or not x.is_contiguous():
             _need(x, "x")
             raise OpsError(f"linear: x is on {x.device}, the weight on {values.device}")
         if gate is not None:
@@ -1731,18 +1736,18 @@ class HipOps:
             if act > ACTIVATIONS["clamped"] or n % 2:
                 raise OpsError(f"gated_linear: {gate[0]} of a weight {tuple(w.shape)}")
             n, form = n // 2, "gated"
-        device, lib = x.device, self.lib
-        out = torch.empty((m, n), dtype=torch.float32 if out_f32 else dtype, device=device)
+        lib, code = self.lib, F32 if out_f32 else _CODE[dtype]
+        out = x.new_empty((m, n), dtype=torch.float32 if out_f32 else dtype)
         if m == 0:
             return out
         if x.data_ptr() % 16:
             x = x.clone()
-        room = 0 if coded is not None or (m <= 4 and lib.qrt_int8_workspace(m, n, k, width) == 0) else m * width + 16 * (m // 4 + 1)
-        work = torch.empty(room, dtype=torch.uint8, device=device).data_ptr() if room else None
+        room = 0 if coded is not None else self._int8_workspace(m, n, k, width)
+        work = x.new_empty(room, dtype=torch.uint8) if room else None
         # 128 columns of bytes are a stage, as 64 of bfloat16 are: the same bytes and the same cycles of the matrix cores
         tile = self.choose_tile(m, n, width // 2, form)[0] if m > 48 else 0
-        if lib.qrt_int8_product(x.data_ptr(), _CODE[dtype], None if coded is None else coded.data_ptr(), values.data_ptr(), scale.data_ptr(), out.data_ptr(),
-                                F32 if out_f32 else _CODE[dtype], work, m, n, k, width, tile, act, limit, _stream()):
+        if lib.qrt_int8_product(x.data_ptr(), _CODE[dtype], None if coded is None else coded.data_ptr(), values.data_ptr(), w.scale.data_ptr(), out.data_ptr(),
+                                code, None if work is None else work.data_ptr(), m, n, k, width, tile, act, limit, _stream()):
             raise OpsError(lib.qrt_last_error().decode())
         return out
 
@@ -1957,7 +1962,7 @@ class HipOps:
         ps, pages, steps = cache.group.page_size, cache.k.shape[0], cache.pages.get("steps", cache.k)
         if (cache.k.dtype == cache.v.dtype == torch.uint8 and steps.dtype == torch.bfloat16 and cache.k.shape == cache.v.shape == (pages, nkv, ps, d // 2)
                 and steps.shape == (pages, nkv, ps, 4) and cache.k.is_contiguous() and cache.v.is_contiguous() and steps.is_contiguous()
-                and cache.k.is_cuda and cache.v.device == steps.device == cache.k.device and d % 32 == 0 and 32 <= d <= 256 and ps % 4 == 0):
+                and cache.k.get_device() == cache.v.get_device() == steps.get_device() >= 0 and d % 32 == 0 and 32 <= d <= 256 and ps % 4 == 0):
             return pages
         if d % 32 or not 32 <= d <= 256 or ps % 4:
             raise OpsError(f"a cache of 4 bits has heads of 32 to 256 in steps of 32 and pages of a multiple of 4 tokens, not {d} and {ps}")
@@ -2147,9 +2152,9 @@ class HipOps:
             raise OpsError(f"block table {tuple(table.shape)} of {table.dtype} for {s} sequences")
         if table.shape[1] * group.page_size < ctx.max_kv_len:
             raise OpsError(f"block table is {table.shape[1]} pages wide, the longest sequence has {ctx.max_kv_len} tokens")
-        if not (q.device == cache.k.device == table.device == ctx.kv_lens.device == ctx.cu_q.device):
+        if not (q.get_device() == cache.k.get_device() == table.get_device() == ctx.kv_lens.get_device() == ctx.cu_q.get_device()):
             raise OpsError(f"queries on {q.device}, a cache on {cache.k.device}, its table on {table.device}")
-        out = torch.empty((ctx.num_tokens, nq * d), dtype=q.dtype, device=q.device)
+        out = q.new_empty((ctx.num_tokens, nq * d))
         if ctx.num_tokens == 0:
             return out
         cu_q, kv_lens = _need(ctx.cu_q, "cu_q", torch.int32, (s + 1,)), _need(ctx.kv_lens, "kv_lens", torch.int32, (s,))
@@ -2161,7 +2166,7 @@ class HipOps:
             a.table_width, a.num_pages, a.page_size = table.shape[1], pages, group.page_size
             a.sink, a.scale, a.softcap = sink, scale, softcap
             if room:
-                parts = torch.empty((room * (d + 2),), dtype=torch.float32, device=q.device)
+                parts = q.new_empty((room * (d + 2),), dtype=torch.float32)
                 a.part_o, a.part_ml = parts.data_ptr(), parts.data_ptr() + 4 * room * d
             self._check(lib, lib.qrt_attention4(byref(a), c_int(_CODE[q.dtype]), c_int(keys), c_int(row_tiles), _stream()))
         return out
