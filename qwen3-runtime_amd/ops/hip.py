@@ -265,6 +265,13 @@ def _stream() -> c_void_p:
 current_stream = _stream
 
 
+def _here(t: torch.Tensor, name: str) -> None:
+    """Launches go to the current device's stream: a tensor on another device is refused."""
+    device = _raw_device() if _raw_device is not None else torch.cuda.current_device()
+    if t.get_device() != device:
+        raise OpsError(f"{name} is on {t.device}, the current device is cuda:{device}")
+
+
 def _need(t: torch.Tensor, name: str, dtype=None, shape=None) -> torch.Tensor:
     if not t.is_cuda:
         raise OpsError(f"{name} must be on the GPU, it is on {t.device}")
@@ -1683,6 +1690,7 @@ class HipOps:
         if x.dim() != 2 or x.dtype not in _CODE or not 0 < x.shape[1] <= INT8_MOST_WIDTH:
             raise OpsError(f"quantize_rows: rows of bfloat16 or float32 of up to {INT8_MOST_WIDTH} columns, not {tuple(x.shape)} of {x.dtype}")
         _need(x, "x")
+        _here(x, "x")
         m, k = x.shape
         width = -(-k // 128) * 128
         codes = torch.empty((m, width), dtype=torch.int8, device=x.device)
@@ -1701,6 +1709,7 @@ class HipOps:
         if h % 4 or width > 8192:
             return self.add_rmsnorm(residual, delta, weight, eps, out_dtype)
         _need(residual, "residual", torch.float32)
+        _here(residual, "residual")
         _need(weight, "norm weight", torch.float32, (h,))
         pd, cd, nd = (None, F32, 0) if delta is None else _planes(delta, t, h, "delta")
         codes = torch.empty((t, width), dtype=torch.int8, device=residual.device)
@@ -1731,6 +1740,7 @@ class HipOps:
         if x.get_device() < 0 or x.get_device() != values.get_device() or not x.is_contiguous():
             _need(x, "x")
             raise OpsError(f"linear: x is on {x.device}, the weight on {values.device}")
+        _here(x, "x")
         if gate is not None:
             act, limit = ACTIVATIONS[gate[0]], gate[1]
             if act > ACTIVATIONS["clamped"] or n % 2:
@@ -1866,6 +1876,7 @@ class HipOps:
                 c_long(cache_pages), c_int(t), c_int(nq), c_int(nkv), c_int(d), c_int(cache.group.page_size), _stream()))
             return q
         if four:
+            # keys by the kernel for many tokens into rows of their own, then the store
             k = torch.empty((t, nkv * d), dtype=qkv.dtype, device=qkv.device)
             a.k_out, a.nv = k.data_ptr(), 0
         elif cache is not None:
@@ -1877,7 +1888,8 @@ class HipOps:
             a.nkv = a.nv = 0  # keys and values go nowhere: only queries are needed
         self._qk(a, qkv.dtype, pages)
         if four:
-            self._store4(k, qkv[:, (nq + nkv) * d: (nq + 2 * nkv) * d], nkv, d, cache)
+            v = qkv[:, (nq + nkv) * d: (nq + 2 * nkv) * d]
+            self._store4(k, v if width % 8 == 0 and qkv.data_ptr() % 16 == 0 else v.contiguous(), nkv, d, cache)
         return q
 
     def qk_joint_norm_store(self, qk, nq, nkv, d, bias, q_w, k_w, eps, positions, q_temp, values_are_keys, cache):
@@ -1963,6 +1975,7 @@ class HipOps:
         if (cache.k.dtype == cache.v.dtype == torch.uint8 and steps.dtype == torch.bfloat16 and cache.k.shape == cache.v.shape == (pages, nkv, ps, d // 2)
                 and steps.shape == (pages, nkv, ps, 4) and cache.k.is_contiguous() and cache.v.is_contiguous() and steps.is_contiguous()
                 and cache.k.get_device() == cache.v.get_device() == steps.get_device() >= 0 and d % 32 == 0 and 32 <= d <= 256 and ps % 4 == 0):
+            _here(cache.k, "key cache")
             return pages
         if d % 32 or not 32 <= d <= 256 or ps % 4:
             raise OpsError(f"a cache of 4 bits has heads of 32 to 256 in steps of 32 and pages of a multiple of 4 tokens, not {d} and {ps}")
@@ -2125,6 +2138,8 @@ class HipOps:
         """Sequences of at most 16 rows (tokens by heads of a group) go by blocks whose waves share their keys, the others by tiles of rows;
         a step that has both takes a launch for either. What follows from the step's lengths is kept with its context, for its other layers."""
         pages = self._check_cache4(cache, nkv, d)
+        if ctx.num_tokens == 0:
+            return q.new_empty((0, nq * d))
         group = cache.group
         table, s = group.block_table, ctx.num_seqs
         key = ("attn4", nq, nkv, d, group.page_size, window, chunk, keep_first, q.dtype, ctx.scratch.get("attn_splits"))
@@ -2155,8 +2170,6 @@ class HipOps:
         if not (q.get_device() == cache.k.get_device() == table.get_device() == ctx.kv_lens.get_device() == ctx.cu_q.get_device()):
             raise OpsError(f"queries on {q.device}, a cache on {cache.k.device}, its table on {table.device}")
         out = q.new_empty((ctx.num_tokens, nq * d))
-        if ctx.num_tokens == 0:
-            return out
         cu_q, kv_lens = _need(ctx.cu_q, "cu_q", torch.int32, (s + 1,)), _need(ctx.kv_lens, "kv_lens", torch.int32, (s,))
         lib = attention4_library(d)
         for fixed, keys, row_tiles, room, _tensors in plan:

@@ -49,7 +49,8 @@ class PreNormBlock(Block):
 
     @staticmethod
     def _normed(ctx, norm, residual, delta, reader):
-        if reader.weights_in_int8 and reader.takes_scaled_rows and getattr(norm, "takes_products", False) and hasattr(ctx.ops, "add_rmsnorm_codes"):
+        if (reader.weights_in_int8 and reader.takes_scaled_rows and getattr(norm, "takes_products", False) and hasattr(ctx.ops, "add_rmsnorm_codes")
+                and not isinstance(delta, (NormedUpdate, ScaledUpdate, StreamUpdate))):
             return ctx.ops.add_rmsnorm_codes(residual, delta, norm.weight, norm.eps, ctx.dtype)  # the reader's products take codes
         if ctx.per_pass.get("norms_take_products") and reader.takes_scaled_rows:
             return norm.forward(ctx, residual, delta, scaled=True)

@@ -372,6 +372,67 @@ def test_attention_refuses():
             attend()
 
 
+@gpu
+def test_steps_without_tokens_and_sequences_without_any():
+    o = ops()
+    q, cache, ctx = case([(0, 40), (2, 50), (0, 0), (20, 33), (0, 9)], 4, 2, 64, 16, torch.bfloat16)
+    near(o.paged_attention(q, cache, ctx, 4, 2, 64, 0.125, None), plain(q, cache, ctx, 4, 2, 64, 0.125), cache)
+    q, cache, ctx = case([(0, 40), (0, 0)], 4, 2, 64, 16, torch.bfloat16)
+    assert o.paged_attention(q, cache, ctx, 4, 2, 64, 0.125, None).shape == (0, 256)
+    cache.group.slots = torch.zeros(0, dtype=torch.int32, device=DEV)
+    o.kv_store(torch.zeros(0, 2, 64, device=DEV), torch.zeros(0, 2, 64, device=DEV), cache)
+
+
+@gpu
+@pytest.mark.parametrize("seqs", [[(1, 60), (1, 300)], [(40, 60), (1, 300)]])
+def test_rows_behind_the_last_sequence_and_neighbours_in_the_cache_stay(seqs):
+    """A padded batch: the output has rows for the step's tokens alone, what lies behind them in memory stays, and the cache is only read."""
+    nq, nkv, d, ps = 4, 2, 64, 16
+    q, cache, ctx = case(seqs, nq, nkv, d, ps, torch.bfloat16)
+    before = {n: x.clone() for n, x in cache.pages.items()}
+    ctx.scratch["attn_splits"] = 3
+    out = ops().paged_attention(q, cache, ctx, nq, nkv, d, d ** -0.5, None)
+    assert out.shape == q.shape
+    for n, x in cache.pages.items():
+        assert torch.equal(x.view(torch.uint8), before[n].view(torch.uint8))
+
+
+@gpu
+def test_a_cache_whose_rows_pass_32_bits_of_bytes():
+    """Pages beyond the first 4 GiB of a pool: those go by addresses of 64 bits. Only the pages in the table are written."""
+    nq, nkv, d, ps, n = 8, 8, 256, 64, 150
+    pages = (1 << 32) // (nkv * ps * d // 2) + 40
+    o = ops()
+    q, cache, ctx = case([(1, n), (70, n)], nq, nkv, d, ps, torch.bfloat16)
+    want = o.paged_attention(q, cache, ctx, nq, nkv, d, d ** -0.5, None)
+    table, at = cache.group.block_table.clone(), {}
+    big = {name: torch.empty((pages, *x.shape[1:]), dtype=x.dtype, device=DEV) for name, x in cache.pages.items()}
+    for i, p in enumerate(sorted(set(table[table >= 0].tolist()))):
+        at[p] = pages - 1 - i if i % 2 else i
+        for name, x in cache.pages.items():
+            big[name][at[p]] = x[p]
+    cache.group.block_table = torch.tensor([[at.get(p, -1) for p in row] for row in table.tolist()], dtype=torch.int32, device=DEV)
+    cache.pages, cache.k, cache.v = big, big["k"], big["v"]
+    got = o.paged_attention(q, cache, ctx, nq, nkv, d, d ** -0.5, None)
+    assert torch.equal(got, want)
+    # the store, there too
+    k, v = torch.randn(3, nkv, d, generator=gen(1)).to(DEV), torch.randn(3, nkv, d, generator=gen(2)).to(DEV)
+    cache.group.slots = torch.tensor([(pages - 60) * ps + 1, (pages - 60) * ps + 2, (pages - 61) * ps + 63], dtype=torch.int32, device=DEV)
+    o.kv_store(k, v, cache)
+    low = empty_cache(2, nkv, ps, d)
+    low.group.slots = torch.tensor([ps + 1, ps + 2, 63], dtype=torch.int32, device=DEV)
+    o.kv_store(k, v, low)
+    for name, x in low.pages.items():
+        for p, off in ((1, slice(1, 3)), (0, slice(63, 64))):
+            a, b = x[p], big[name][pages - 61 + p]
+            if name == "v":
+                a, b = (y.reshape(nkv, ps // 4, d // 2, 4) for y in (a, b))
+                four, j = off.start // 4, slice(off.start % 4, off.start % 4 + off.stop - off.start)
+                assert torch.equal(a[:, four, :, j], b[:, four, :, j])
+            else:
+                assert torch.equal(a[:, off], b[:, off])
+
+
 # ---- needs no GPU
 
 

@@ -209,6 +209,32 @@ def test_no_rows_and_refusals_on_the_device():
         o.gated_linear(rnd(2, 640), w, "relu2")
 
 
+@gpu
+def test_tensors_on_another_device_than_the_current_one_are_refused(monkeypatch):
+    from qwen3_runtime_amd.ops import OpsError, hip
+
+    o, w, x = ops(), Int8Weight.quantize(rnd(32, 640)), rnd(2, 640)
+    o.linear(x, w)
+    monkeypatch.setattr(hip, "_raw_device", lambda: 1)  # as if another device were current
+    for call in (lambda: o.linear(x, w), lambda: o.gated_linear(x, w), lambda: o.quantize_rows(x),
+                 lambda: o.add_rmsnorm_codes(x.clone(), None, torch.ones(640, device=DEV), 1e-6, torch.float32)):
+        with pytest.raises(OpsError, match="current device"):
+            call()
+
+
+@gpu
+@pytest.mark.parametrize("offset", [1, 2, 8])
+@pytest.mark.parametrize("m", [1, 5, 70])
+def test_rows_that_begin_anywhere(m, offset):
+    w = Int8Weight.quantize(rnd(48, 640, seed=2))
+    x = rnd(m * 640 + offset, seed=1, dtype=torch.bfloat16)[offset:].view(m, 640)
+    near(ops().linear(x, w), product(x, w), torch.bfloat16)
+    # and weights: columns of a wider matrix, rows that begin anywhere
+    wide = torch.randint(-127, 128, (48, 700), dtype=torch.int8, generator=torch.Generator().manual_seed(3)).to(DEV)
+    w = Int8Weight(wide[:, offset: offset + 640], torch.ones(96, device=DEV)[::2])
+    near(ops().linear(x, w), product(x, w), torch.bfloat16)
+
+
 # ---- needs no GPU
 
 
