@@ -23,7 +23,16 @@ constexpr int KS = D / 32;  // steps of 32 elements: words a lane holds of 16 ke
 typedef float f32x2_t __attribute__((ext_vector_type(2)));
 constexpr float LOG2E = 1.4426950408889634f;
 
-struct Attention4Args {
+// What follows from a step's lengths, the same for all its layers.
+struct Attention4Plan {
+  const int* tile_seq;      // null: tile i is sequence i from its first row
+  const int* tile_row0;     // null: from the first row
+  const int* merge_tokens;  // null: all
+  int num_merge_tokens, num_tiles, num_seqs, nq, nkv;
+  int window, chunk, keep_first;
+  int piece, pieces;  // blocks of 32 keys in a piece; how many pieces the launch has room for
+};
+struct Attention4Args : Attention4Plan {
   const void* q;
   void* out;
   const uint8_t* k;
@@ -32,16 +41,10 @@ struct Attention4Args {
   const int* cu_q;
   const int* kv_lens;
   const int* table;
-  const int* tile_seq;   // null: tile i is sequence i from its first row
-  const int* tile_row0;  // null: from the first row
-  float* part_o;         // [rows, pieces, D], not divided by the sums
-  float* part_ml;        // [rows, pieces, 2]
-  const int* merge_tokens;  // null: all
-  int num_merge_tokens;
-  int table_width, num_tiles, num_pages, num_seqs, nq, nkv, page_size;
-  int window, chunk, keep_first, sink;
+  float* part_o;   // [rows, pieces, D], not divided by the sums
+  float* part_ml;  // [rows, pieces, 2]
+  int table_width, num_pages, page_size, sink;
   float scale, softcap;
-  int piece, pieces;  // blocks of 32 keys in a piece; how many pieces the launch has room for
 };
 
 // The blocks of 32 keys that rows [base, base + rows_of_tile) of a sequence see: first those of the kept first tokens, then a run.
@@ -622,16 +625,20 @@ static int launch(const Attention4Args& a, hipStream_t stream) {
   return 0;
 }
 
-// keys: tiles of up to 16 rows, the waves of a block share its keys; otherwise tiles of 64 row_tiles rows.
-extern "C" int qrt_attention4(const Attention4Args* args, int dtype, int keys, int row_tiles, hipStream_t stream) {
-  const Attention4Args& a = *args;
+// keys: tiles of up to 16 rows, the waves of a block share its keys; otherwise tiles of 64 row_tiles rows. parts: room for the pieces' sums, behind whose
+// ml_at bytes come their maxima and weights (not needed for one piece).
+extern "C" int qrt_attention4(const Attention4Plan* plan, const void* q, void* out, const void* k, const void* v, const void* steps, const int* cu_q,
+                              const int* kv_lens, const int* table, void* parts, int64_t ml_at, int table_width, int num_pages, int page_size, int sink,
+                              float scale, float softcap, int dtype, int keys, int row_tiles, hipStream_t stream) {
+  const Attention4Args a{*plan, q, out, (const uint8_t*)k, (const uint8_t*)v, (const unsigned*)steps, cu_q, kv_lens, table, (float*)parts,
+                         (float*)((char*)parts + ml_at), table_width, num_pages, page_size, sink, scale, softcap};
   QRT_CHECK(dtype == QRT_BF16 || dtype == QRT_F32, "attention4: unknown dtype %d", dtype);
   QRT_CHECK(a.nq > 0 && a.nkv > 0 && a.nq % a.nkv == 0, "attention4: %d query heads on %d key heads", a.nq, a.nkv);
   QRT_CHECK(a.page_size >= 4 && a.page_size % 4 == 0 && a.num_pages > 0 && a.table_width > 0, "attention4: pages of a multiple of 4 tokens, not %d", a.page_size);
   QRT_CHECK((int64_t)a.num_pages * a.nkv * a.page_size < (1ll << 31), "attention4: a pool of %d pages of %d tokens and %d heads has too many rows", a.num_pages, a.page_size, a.nkv);
   QRT_CHECK(a.window >= 0 && a.chunk >= 0 && a.keep_first >= 0 && !(a.window && a.chunk) && !(a.keep_first && !a.window), "attention4: bad mask");
   QRT_CHECK(a.piece > 0 && a.pieces > 0 && a.pieces <= MOST_PIECES, "attention4: bad pieces %d of %d", a.pieces, a.piece);
-  QRT_CHECK(a.pieces == 1 || (a.part_o && a.part_ml && a.num_merge_tokens > 0 && (int64_t)a.num_merge_tokens * a.nq < (1ll << 31)), "attention4: pieces need room for their parts");
+  QRT_CHECK(a.pieces == 1 || (a.part_o && ml_at > 0 && ml_at % 16 == 0 && a.num_merge_tokens > 0 && (int64_t)a.num_merge_tokens * a.nq < (1ll << 31)), "attention4: pieces need room for their parts");
   QRT_CHECK((a.tile_seq != nullptr) == (a.tile_row0 != nullptr) || keys, "attention4: a list of tiles has sequences and rows");
   QRT_CHECK(!keys || a.nq / a.nkv <= 16, "attention4: %d rows a token in a tile of 16", a.nq / a.nkv);
   QRT_CHECK(a.num_tiles <= 65535, "attention4: %d tiles in one launch, 65535 at most", a.num_tiles);

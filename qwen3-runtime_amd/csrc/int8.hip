@@ -227,19 +227,22 @@ struct Int8Rows {
   GatedEpilogue ep;
 };
 
-// Rows that a block turns into codes itself (FUSED): up to four, a row to each of its four waves, or to two or all four of them; a lane
-// has ITS pieces of 8 columns, in registers from the loads to the codes. Every block does so again, so it pays while blocks are few: us
+// Rows that a block turns into codes itself (FUSED): up to eight, one or two to each of its four waves, or one to two or all four of them; a
+// lane has ITS pieces of 8 columns of each, in registers from the loads to the codes. Every block does so again, so it pays while blocks and rows are few: us
 // with a kernel in front and fused at 1 and 4 rows 6,144 x 2,560 7.0, 7.1 and 4.5, 5.2; 6,144 x 4,096 9.0, 9.1 and 6.0, 6.5; gated, 9,728 x 2,560
 // (1,216 blocks) 12.0, 12.1 and 11.7, 13.7, 12,288 x 4,096 (1,536) 18.5, 18.6 and 21.3, 24.1.
+// Five to eight rows of 1,024 columns 4.0 to 4.1 fused by 2,560 outputs and some 4.7 not, of 2,560 columns 6.5 and 5.9; 16 rows of 1,024 5.8 and 5.1.
 constexpr int FUSED_MOST = 10;
 constexpr int fused_parts(int M) { return M == 1 ? 4 : M == 2 ? 2 : 1; }
 constexpr int fused_its(int M, int width) { return (width / 8 + 64 * fused_parts(M) - 1) / (64 * fused_parts(M)); }
-constexpr bool fused_takes(int M, int N, int width) { return M >= 1 && M <= 4 && N <= 8 * 1100 && fused_its(M, width) <= FUSED_MOST; }
+constexpr bool fused_takes(int M, int N, int width) {
+  return M >= 1 && (M <= 4 ? N <= 8 * 1100 && fused_its(M, width) <= FUSED_MOST : M <= 8 && N <= 4096 && fused_its(M, width) <= 2);
+}
 
 // NW waves; WU units of eight weight rows (1: the operand's rows 8 to 15 repeat the others); MB blocks of 16 rows of the
 // activations (FEW: eight); GATED: half of the units are gate rows, half the up rows that belong to them.
-// ITS > 0: FUSED.
-template <int NW, int WU, int MB, bool FEW, int U, bool GATED, int ITS, typename TX, typename TO>
+// ITS > 0: FUSED, ROWS rows of the activations a wave (or a part of one).
+template <int NW, int WU, int MB, bool FEW, int U, bool GATED, int ROWS, int ITS, typename TX, typename TO>
 __global__ __launch_bounds__(64 * NW) void int8_rows_kernel(Int8Rows p) {
   constexpr bool FUSED = ITS > 0;
   constexpr int NT = WU == 1 ? 1 : WU / 2, AU = FEW ? 1 : 2 * MB, LOADS = WU + (FUSED ? 0 : AU), SLOT = LOADS * 1024;
@@ -247,7 +250,7 @@ __global__ __launch_bounds__(64 * NW) void int8_rows_kernel(Int8Rows p) {
   static_assert((U - 1) * LOADS < 64, "the loads' counter holds 63");
   static_assert(!FUSED || (NW == 4 && FEW), "the waves that share a row are counted for four");
   extern __shared__ __align__(16) unsigned char rows_lds[];  // [NW][U] slots, later the sums; FUSED: the rows' codes behind them
-  __shared__ unsigned most_of[FUSED ? 4 : 1];
+  __shared__ unsigned most_of[FUSED ? 4 * ROWS : 1];
   const int lane = threadIdx.x & 63, wave = uniform_wave_number();
   const int r16 = lane & 15, quad = lane >> 4, sub = lane >> 3, piece = (lane & 7) ^ sub;
   const int n0 = blockIdx.x * OUTS;
@@ -257,12 +260,16 @@ __global__ __launch_bounds__(64 * NW) void int8_rows_kernel(Int8Rows p) {
   const int width = p.width, steps = width / INT8_STAGE;
 
   // FUSED: the rows come first, and are waited for behind the weights' loads
-  float v[FUSED ? ITS : 1][8];
-  const int parts = fused_parts(p.M), code_rows = 4 / parts, own_row = wave / parts, own_at = 8 * ((wave - own_row * parts) * 64 + lane);
+  float v[FUSED ? ROWS * ITS : 1][8];
+  const int parts = fused_parts(p.M), code_rows = 4 * ROWS / parts, own_row = wave / parts, own_at = 8 * ((wave - own_row * parts) * 64 + lane);
   if constexpr (FUSED) {
 #pragma unroll
-    for (int j = 0; j < ITS; ++j)
-      load_row8<TX, true>((const TX*)p.x + (size_t)min(own_row, p.M - 1) * p.K, own_row < p.M ? own_at + 512 * parts * j : p.K, p.K, v[j]);
+    for (int k = 0; k < ROWS; ++k)
+#pragma unroll
+      for (int j = 0; j < ITS; ++j) {
+        const int row = own_row + 4 * k;
+        load_row8<TX, true>((const TX*)p.x + (size_t)min(row, p.M - 1) * p.K, row < p.M ? own_at + 512 * parts * j : p.K, p.K, v[k * ITS + j]);
+      }
   }
   const int8_t* src[LOADS];
 #pragma unroll
@@ -289,26 +296,36 @@ __global__ __launch_bounds__(64 * NW) void int8_rows_kernel(Int8Rows p) {
 
   if constexpr (FUSED) {
     __shared__ unsigned part_of[4];
-    unsigned most = 0;
+    unsigned most[ROWS];
 #pragma unroll
-    for (int j = 0; j < ITS; ++j)
+    for (int k = 0; k < ROWS; ++k) {
+      most[k] = 0;
 #pragma unroll
-      for (int e = 0; e < 8; ++e) most = max(most, magnitude_bits(v[j][e]));
-    most = wave_max_bits(most);
-    if (lane == 0) part_of[wave] = most;
-    QRT_WAIT_LDS();
-    QRT_BARRIER();
-    if (own_row < p.M) {
-      for (int i = 0; i < parts; ++i) most = max(most, part_of[own_row * parts + i]);
-      if (lane == 0) most_of[own_row] = most;
-      const float by = code_factor(most);
+      for (int j = 0; j < ITS; ++j)
+#pragma unroll
+        for (int e = 0; e < 8; ++e) most[k] = max(most[k], magnitude_bits(v[k * ITS + j][e]));
+      most[k] = wave_max_bits(most[k]);
+    }
+    if (ROWS == 1 && parts > 1) {
+      if (lane == 0) part_of[wave] = most[0];
+      QRT_WAIT_LDS();
+      QRT_BARRIER();
+      for (int i = 0; i < parts; ++i) most[0] = max(most[0], part_of[own_row * parts + i]);
+    }
+#pragma unroll
+    for (int k = 0; k < ROWS; ++k) {
+      const int row = own_row + 4 * k;
+      if (row >= p.M) continue;
+      if (lane == 0) most_of[row] = most[k];
+      const float by = code_factor(most[k]);
 #pragma unroll
       for (int j = 0; j < ITS; ++j) {
         const int at = own_at + 512 * parts * j;
+        const float(&x)[8] = v[k * ITS + j];
         typedef unsigned u32x2_t __attribute__((ext_vector_type(2)));
         // piece c of 16 columns of a stage's row r lies at 16 (c ^ (r & 7)), as in the rings
-        unsigned char* to = own_codes + (size_t)((at >> 7) * code_rows + own_row) * 128 + 16 * (((at >> 4) & 7) ^ own_row) + (at & 8);
-        if (at < width) *(u32x2_t*)to = (u32x2_t){codes4(v[j][0], v[j][1], v[j][2], v[j][3], by), codes4(v[j][4], v[j][5], v[j][6], v[j][7], by)};
+        unsigned char* to = own_codes + (size_t)((at >> 7) * code_rows + row) * 128 + 16 * (((at >> 4) & 7) ^ (row & 7)) + (at & 8);
+        if (at < width) *(u32x2_t*)to = (u32x2_t){codes4(x[0], x[1], x[2], x[3], by), codes4(x[4], x[5], x[6], x[7], by)};
       }
     }
     QRT_WAIT_LDS();
@@ -384,14 +401,14 @@ __global__ __launch_bounds__(64 * NW) void int8_rows_kernel(Int8Rows p) {
   }
 }
 
-template <int NW, int WU, int MB, bool FEW, int U, bool GATED, int ITS, typename TX, typename TO>
+template <int NW, int WU, int MB, bool FEW, int U, bool GATED, int ROWS, int ITS, typename TX, typename TO>
 static int launch_int8_rows(const Int8Rows& p, hipStream_t stream) {
   constexpr int NT = WU == 1 ? 1 : WU / 2, AU = FEW ? 1 : 2 * MB, OUTS = GATED ? 4 * WU : 8 * WU;
   constexpr size_t rings = (size_t)NW * U * (WU + (ITS ? 0 : AU)) * 1024, meet = (size_t)NW * NT * MB * 1024, most = 150 * 1024;
-  const size_t smem = (rings > meet ? rings : meet) + (ITS ? (size_t)p.width * (4 / fused_parts(p.M)) : 0);
+  const size_t smem = (rings > meet ? rings : meet) + (ITS ? (size_t)p.width * (4 * ROWS / fused_parts(p.M)) : 0);
   static_assert(rings <= most, "the rings of this configuration do not fit LDS");
   QRT_CHECK(smem <= most, "int8_rows: %d columns need %zu bytes of LDS", p.width, smem);
-  auto kernel = int8_rows_kernel<NW, WU, MB, FEW, U, GATED, ITS, TX, TO>;
+  auto kernel = int8_rows_kernel<NW, WU, MB, FEW, U, GATED, ROWS, ITS, TX, TO>;
   static bool allowed = false;  // once per kernel: not inside a stream capture again and again
   if (smem > 64 * 1024 && !allowed) {
     if (hipFuncSetAttribute((const void*)kernel, hipFuncAttributeMaxDynamicSharedMemorySize, (int)most) != hipSuccess)
@@ -407,29 +424,30 @@ template <bool GATED, typename TX, typename TO>
 static int fused_by_size(const Int8Rows& p, hipStream_t stream) {
   constexpr int WU = GATED ? 2 : 1;
   const int its = fused_its(p.M, p.width);
-  if (its <= 2) return launch_int8_rows<4, WU, 1, true, 4, GATED, 2, TX, TO>(p, stream);
-  if (its <= 5) return launch_int8_rows<4, WU, 1, true, 4, GATED, 5, TX, TO>(p, stream);
-  return launch_int8_rows<4, WU, 1, true, 4, GATED, FUSED_MOST, TX, TO>(p, stream);
+  if (p.M > 4) return launch_int8_rows<4, WU, 1, true, 4, GATED, 2, 2, TX, TO>(p, stream);
+  if (its <= 2) return launch_int8_rows<4, WU, 1, true, 4, GATED, 1, 2, TX, TO>(p, stream);
+  if (its <= 5) return launch_int8_rows<4, WU, 1, true, 4, GATED, 1, 5, TX, TO>(p, stream);
+  return launch_int8_rows<4, WU, 1, true, 4, GATED, 1, FUSED_MOST, TX, TO>(p, stream);
 }
 template <bool GATED, typename TO>
 static int rows_by_size(const Int8Rows& p, hipStream_t stream) {
   if constexpr (!GATED) {  // blocks are no more than compute units: eight waves each
-    if (p.M <= 8 && p.N <= 4096) return launch_int8_rows<8, 2, 1, true, 4, false, 0, float, TO>(p, stream);
-    if (p.M <= 16 && p.N <= 4096) return launch_int8_rows<8, 2, 1, false, 4, false, 0, float, TO>(p, stream);
-    if (p.M <= 32 && p.N <= 4096) return launch_int8_rows<8, 2, 2, false, 3, false, 0, float, TO>(p, stream);
+    if (p.M <= 8 && p.N <= 4096) return launch_int8_rows<8, 2, 1, true, 4, false, 1, 0, float, TO>(p, stream);
+    if (p.M <= 16 && p.N <= 4096) return launch_int8_rows<8, 2, 1, false, 4, false, 1, 0, float, TO>(p, stream);
+    if (p.M <= 32 && p.N <= 4096) return launch_int8_rows<8, 2, 2, false, 3, false, 1, 0, float, TO>(p, stream);
   }
-  if (p.M <= 8) return launch_int8_rows<4, 2, 1, true, 4, GATED, 0, float, TO>(p, stream);
-  if (p.M <= 16) return launch_int8_rows<4, 2, 1, false, 4, GATED, 0, float, TO>(p, stream);
+  if (p.M <= 8) return launch_int8_rows<4, 2, 1, true, 4, GATED, 1, 0, float, TO>(p, stream);
+  if (p.M <= 16) return launch_int8_rows<4, 2, 1, false, 4, GATED, 1, 0, float, TO>(p, stream);
   // 32 weight rows a block fetch the activations half as often, where they leave as many blocks as compute units
   if (p.M <= 32) {
-    if (p.N * (GATED ? 2 : 1) < 32 * 512) return launch_int8_rows<4, 2, 2, false, 3, GATED, 0, float, TO>(p, stream);
-    return launch_int8_rows<4, 4, 2, false, 2, GATED, 0, float, TO>(p, stream);
+    if (p.N * (GATED ? 2 : 1) < 32 * 512) return launch_int8_rows<4, 2, 2, false, 3, GATED, 1, 0, float, TO>(p, stream);
+    return launch_int8_rows<4, 4, 2, false, 2, GATED, 1, 0, float, TO>(p, stream);
   }
   if (p.N * (GATED ? 2 : 1) < 32 * 192) {
-    if (p.M <= 48) return launch_int8_rows<4, 2, 3, false, 2, GATED, 0, float, TO>(p, stream);
-    return launch_int8_rows<4, 2, 4, false, 2, GATED, 0, float, TO>(p, stream);
+    if (p.M <= 48) return launch_int8_rows<4, 2, 3, false, 2, GATED, 1, 0, float, TO>(p, stream);
+    return launch_int8_rows<4, 2, 4, false, 2, GATED, 1, 0, float, TO>(p, stream);
   }
-  return launch_int8_rows<4, 4, 3, false, 2, GATED, 0, float, TO>(p, stream);
+  return launch_int8_rows<4, 4, 3, false, 2, GATED, 1, 0, float, TO>(p, stream);
 }
 
 // c [M, N] of up to 64 rows. Either x (rows as they are, in x_dtype: those that fused_takes, of a multiple of 8 columns) or a and a_scale.

@@ -64,14 +64,11 @@ class _AttnArgs(Structure):
     ]
 
 
-class _Attn4Args(Structure):
+class _Attn4Plan(Structure):
     _fields_ = [
-        ("q", c_void_p), ("out", c_void_p), ("k", c_void_p), ("v", c_void_p), ("steps", c_void_p),
-        ("cu_q", c_void_p), ("kv_lens", c_void_p), ("table", c_void_p), ("tile_seq", c_void_p), ("tile_row0", c_void_p),
-        ("part_o", c_void_p), ("part_ml", c_void_p), ("merge_tokens", c_void_p), ("num_merge_tokens", c_int),
-        ("table_width", c_int), ("num_tiles", c_int), ("num_pages", c_int), ("num_seqs", c_int), ("nq", c_int), ("nkv", c_int),
-        ("page_size", c_int), ("window", c_int), ("chunk", c_int), ("keep_first", c_int), ("sink", c_int),
-        ("scale", c_float), ("softcap", c_float), ("piece", c_int), ("pieces", c_int),
+        ("tile_seq", c_void_p), ("tile_row0", c_void_p), ("merge_tokens", c_void_p), ("num_merge_tokens", c_int),
+        ("num_tiles", c_int), ("num_seqs", c_int), ("nq", c_int), ("nkv", c_int), ("window", c_int), ("chunk", c_int), ("keep_first", c_int),
+        ("piece", c_int), ("pieces", c_int),
     ]
 
 
@@ -220,7 +217,9 @@ _attn4: dict[int, ctypes.CDLL] = {}
 def attention4_library(head_dim: int) -> ctypes.CDLL:
     """The attention over a cache of 4 bits, for one head size."""
     if head_dim not in _attn4:
-        _attn4[head_dim] = _load(f"attn4_d{head_dim}")
+        lib = _load(f"attn4_d{head_dim}")
+        lib.qrt_attention4.argtypes = [c_void_p] * 10 + [c_long] + [c_int] * 4 + [c_float] * 2 + [c_int] * 3 + [c_void_p]
+        _attn4[head_dim] = lib
     return _attn4[head_dim]
 
 
@@ -382,6 +381,7 @@ class HipOps:
         self.lib = core_library()
         # declared, the arguments travel as they are: a wrapper object for each of fifteen took 2 us a call
         self.lib.qrt_int8_product.argtypes = [c_void_p, c_int, c_void_p, c_void_p, c_void_p, c_void_p, c_int, c_void_p] + [c_int] * 6 + [c_float, c_void_p]
+        self.lib.qrt_store4.argtypes = [c_void_p, c_void_p, c_int, c_long, c_long] + [c_void_p] * 4 + [c_long] + [c_int] * 4 + [c_void_p]
         self.lib.qrt_int8_workspace.argtypes, self.lib.qrt_int8_workspace.restype = [c_int] * 4, c_long
         self.residual_planes = residual_planes
 
@@ -1963,11 +1963,11 @@ class HipOps:
         """Keys and values of tokens, rows of ``nkv * d`` with any stride, into a cache of 4 bits."""
         pages = self._check_cache4(cache, nkv, d)
         slots = _need(cache.group.slots, "slots", torch.int32, (k.shape[0],))
-        if not (k.device == v.device == cache.k.device == slots.device) or k.dtype not in _CODE:
+        if not (k.get_device() == v.get_device() == cache.k.get_device() == slots.get_device()) or k.dtype not in _CODE:
             raise OpsError(f"keys {k.dtype} on {k.device}, values on {v.device}, a cache on {cache.k.device}")
         self._check(self.lib, self.lib.qrt_store4(
-            _ptr(k), _ptr(v), c_int(_CODE[k.dtype]), c_long(k.stride(0)), c_long(v.stride(0)), _ptr(cache.k), _ptr(cache.v),
-            _ptr(cache.pages["steps"]), _ptr(slots), c_long(pages), c_int(k.shape[0]), c_int(nkv), c_int(d), c_int(cache.group.page_size), _stream()))
+            k.data_ptr(), v.data_ptr(), _CODE[k.dtype], k.stride(0), v.stride(0), cache.k.data_ptr(), cache.v.data_ptr(), cache.pages["steps"].data_ptr(),
+            slots.data_ptr(), pages, k.shape[0], nkv, d, cache.group.page_size, _stream()))
 
     @staticmethod
     def _check_cache4(cache, nkv, d) -> int:
@@ -2163,25 +2163,30 @@ class HipOps:
             ctx.scratch[key] = plan
         if not (math.isfinite(scale) and softcap >= 0):
             raise OpsError(f"scale {scale}, cap {softcap}")
-        if table.dtype != torch.int32 or table.dim() != 2 or table.shape[0] != s or not table.is_contiguous():
-            raise OpsError(f"block table {tuple(table.shape)} of {table.dtype} for {s} sequences")
-        if table.shape[1] * group.page_size < ctx.max_kv_len:
-            raise OpsError(f"block table is {table.shape[1]} pages wide, the longest sequence has {ctx.max_kv_len} tokens")
-        if not (q.get_device() == cache.k.get_device() == table.get_device() == ctx.kv_lens.get_device() == ctx.cu_q.get_device()):
+        cu_q, kv_lens = ctx.cu_q, ctx.kv_lens
+        checked = ctx.scratch.get("attn4_tensors")  # the step's own tensors are looked at once
+        if checked is None or checked[0] is not table or checked[1] is not cu_q or checked[2] is not kv_lens:
+            if table.dtype != torch.int32 or table.dim() != 2 or table.shape[0] != s or not table.is_contiguous():
+                raise OpsError(f"block table {tuple(table.shape)} of {table.dtype} for {s} sequences")
+            if table.shape[1] * group.page_size < ctx.max_kv_len:
+                raise OpsError(f"block table is {table.shape[1]} pages wide, the longest sequence has {ctx.max_kv_len} tokens")
+            _need(cu_q, "cu_q", torch.int32, (s + 1,))
+            _need(kv_lens, "kv_lens", torch.int32, (s,))
+            if not (table.get_device() == kv_lens.get_device() == cu_q.get_device()):
+                raise OpsError(f"a block table on {table.device}, lengths on {kv_lens.device} and {cu_q.device}")
+            ctx.scratch["attn4_tensors"] = checked = (table, cu_q, kv_lens)
+        if not q.get_device() == cache.k.get_device() == table.get_device():
             raise OpsError(f"queries on {q.device}, a cache on {cache.k.device}, its table on {table.device}")
         out = q.new_empty((ctx.num_tokens, nq * d))
-        cu_q, kv_lens = _need(ctx.cu_q, "cu_q", torch.int32, (s + 1,)), _need(ctx.kv_lens, "kv_lens", torch.int32, (s,))
-        lib = attention4_library(d)
+        lib, code, stream = attention4_library(d), _CODE[q.dtype], _stream()
         for fixed, keys, row_tiles, room, _tensors in plan:
-            a = _Attn4Args.from_buffer_copy(fixed)
-            a.q, a.out, a.k, a.v, a.steps = q.data_ptr(), out.data_ptr(), cache.k.data_ptr(), cache.v.data_ptr(), cache.pages["steps"].data_ptr()
-            a.cu_q, a.kv_lens, a.table = cu_q.data_ptr(), kv_lens.data_ptr(), table.data_ptr()
-            a.table_width, a.num_pages, a.page_size = table.shape[1], pages, group.page_size
-            a.sink, a.scale, a.softcap = sink, scale, softcap
+            parts = 0
             if room:
-                parts = q.new_empty((room * (d + 2),), dtype=torch.float32)
-                a.part_o, a.part_ml = parts.data_ptr(), parts.data_ptr() + 4 * room * d
-            self._check(lib, lib.qrt_attention4(byref(a), c_int(_CODE[q.dtype]), c_int(keys), c_int(row_tiles), _stream()))
+                parts = q.new_empty((room * (d + 2),), dtype=torch.float32).data_ptr()
+            if lib.qrt_attention4(fixed, q.data_ptr(), out.data_ptr(), cache.k.data_ptr(), cache.v.data_ptr(), cache.pages["steps"].data_ptr(), cu_q.data_ptr(),
+                                  kv_lens.data_ptr(), table.data_ptr(), parts, 4 * room * d, table.shape[1], pages, group.page_size, sink, scale, softcap, code,
+                                  keys, row_tiles, stream):
+                raise OpsError(lib.qrt_last_error().decode())
         return out
 
     @staticmethod
@@ -2212,7 +2217,7 @@ class HipOps:
         if subset is not None:  # the tokens of these sequences: where a merge of pieces writes
             cu = np.concatenate([[0], np.cumsum(ctx.q_lens_host)])
             tokens = torch.from_numpy(np.concatenate([np.arange(cu[i], cu[i + 1]) for i in seqs]).astype(np.int32)).to(q.device)
-        a = _Attn4Args()
+        a = _Attn4Plan()
         if tiles is not None:
             a.tile_seq, a.tile_row0 = tiles.data_ptr(), tiles.data_ptr() + 4 * n_tiles
         a.num_tiles, a.num_seqs, a.nq, a.nkv, a.num_merge_tokens = n_tiles, ctx.num_seqs, nq, nkv, ctx.num_tokens

@@ -459,9 +459,9 @@ def test_spec_of_a_cache_of_4_bits():
 
 
 def test_entry_points_refuse_on_the_host():
-    from ctypes import byref, c_int, c_long, c_void_p
+    from ctypes import c_int, c_long, c_void_p
 
-    from qwen3_runtime_amd.ops.hip import HipOps, _Attn4Args, attention4_library
+    from qwen3_runtime_amd.ops.hip import HipOps, _Attn4Plan, attention4_library
 
     lib, p = HipOps().lib, c_void_p(1 << 20)  # not read: the sizes are refused
     store = lambda t=1, heads=2, d=64, ps=16, dtype=1, stride=128, k=p: lib.qrt_store4(  # noqa: E731
@@ -470,13 +470,11 @@ def test_entry_points_refuse_on_the_host():
         assert store(**bad) != 0, bad
     lib = attention4_library(64)
 
-    def attend(dtype=1, keys=1, row_tiles=1, **fields):
-        a = _Attn4Args()
-        for n in ("q", "out", "k", "v", "steps", "cu_q", "kv_lens", "table"):
-            setattr(a, n, 1 << 20)
-        for n, x in dict(dict(num_tiles=1, nq=4, nkv=2, page_size=16, num_pages=3, table_width=2, num_seqs=1, piece=1, pieces=1, scale=1.0), **fields).items():
+    def attend(dtype=1, keys=1, row_tiles=1, page_size=16, num_pages=3, table_width=2, q=1 << 20, **fields):
+        a, at = _Attn4Plan(), 1 << 20
+        for n, x in dict(dict(num_tiles=1, nq=4, nkv=2, num_seqs=1, piece=1, pieces=1), **fields).items():
             setattr(a, n, x)
-        return lib.qrt_attention4(byref(a), c_int(dtype), c_int(keys), c_int(row_tiles), None)
+        return lib.qrt_attention4(bytes(a), q, at, at, at, at, at, at, at, 0, 0, table_width, num_pages, page_size, 0, 1.0, 0.0, dtype, keys, row_tiles, None)
 
     for bad in (dict(nq=3), dict(nkv=0), dict(page_size=6), dict(num_pages=0), dict(table_width=0), dict(window=-1), dict(window=2, chunk=2), dict(keep_first=1),
                 dict(piece=0), dict(pieces=0), dict(pieces=2), dict(dtype=3), dict(nq=34), dict(keys=0, row_tiles=3), dict(keys=0, row_tiles=2, dtype=0), dict(q=(1 << 20) + 2),
