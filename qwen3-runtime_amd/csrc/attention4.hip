@@ -11,9 +11,19 @@
 // probabilities in 16 bits). float32 queries: q and w as three bfloat16 each (24 bits in all, whole), and OFF = -8, which leaves nothing to
 // take out: with an offset of 16 the results were 3.6e-6 from those in 64 bits, where sums in float32 are 2e-7.
 //
-// KEYS: up to 16 rows (token x head of the group); the four waves of a block take its blocks of keys in turn and meet in LDS. Otherwise a
-// wave has 16 RT rows of its own, and the four of a block read the same keys at about the same time. Either way a launch may cut the
-// keys into pieces of one length, which a second kernel joins. Sums, maxima and outputs are float32.
+// A wave has 16 RT rows (token x head of the group) of its own. Of a block's four waves GROUPS share the same rows, take the blocks of keys in
+// turn and meet in LDS at the end; the rows are 4 / GROUPS bands of 16 RT, whose waves read the same keys at about the same time. Many groups
+// make many blocks of few rows, which fills the chip and evens out what a causal mask leaves; few groups meet less often. us with 4, 2 and
+// 1 groups, 32 heads on 8 of 128, a prompt read at once: 300 tokens (304 blocks of 4 groups) 11.5, 12.1, 15.3; 512 (512) 12.8, 14.7, 21.3;
+// 700 (704) 22.2, 19.4, 27.4; 2,048 (2,048) 67.7, 59.0, 70.3; two of 2,048 (4,096) 140, 119, 115.
+// RT = 2 takes the codes out of their words half as often a row: from some 400 blocks on, as many as the chip holds, that is what counts (400 tokens
+// of 4,096 49.6 and 60.1 us), before that the blocks are (128 tokens 8.7 and 5.9). A launch may cut the keys into pieces of one length as well,
+// which a second kernel joins. Sums, maxima and outputs are float32.
+//
+// What bounds it: many rows, the vector instructions: some 240 a block of 32 keys and 32 rows beside 34 of the matrix cores, issued in 60 % of the
+// cycles at 2,048 tokens (0.58 PFLOP/s). Taken out on the way there: a branch an element that the compiler had made of one condition
+// (93 us -> 71), and arguments held in scalar registers, which it kept in a vector register's lanes (71 -> 64). One row a head over 32,000 tokens: 34.8 MB in
+// 12.8 us, 2.7 TB/s, four blocks of keys a wave between a start and a meeting that take most of it, and a merge of 4 us.
 #include "common.h"
 #include "cache4.h"
 
@@ -45,7 +55,18 @@ struct Attention4Args : Attention4Plan {
   float* part_ml;  // [rows, pieces, 2]
   int table_width, num_pages, page_size, sink;
   float scale, softcap;
+  PageMagic page, group;  // division by the page size, and by the query heads of a key head
 };
+#ifdef __HIP_DEVICE_COMPILE__
+// The kernel's arguments, read where they are wanted: held from the start they took so many scalar registers that the loop over keys moved
+// forty of them a block in and out of a vector register's lanes.
+typedef const Attention4Args __attribute__((address_space(4)))* Arguments;
+__device__ __forceinline__ Arguments arguments() {
+  Arguments a = (Arguments)__builtin_amdgcn_kernarg_segment_ptr();
+  asm volatile("" : "+s"(a));
+  return a;
+}
+#endif
 
 // The blocks of 32 keys that rows [base, base + rows_of_tile) of a sequence see: first those of the kept first tokens, then a run.
 struct Blocks {
@@ -254,7 +275,7 @@ struct Walk {
 #pragma unroll
           for (int r = 0; r < 4; ++r) {
             const int key = 32 * b + 16 * h + 4 * quad + r;
-            const bool sees = key <= pos[t] && (key >= low[t] || key < a.keep_first);
+            const bool sees = (unsigned)(key - low[t]) <= (unsigned)(pos[t] - low[t]) || key < min(a.keep_first, pos[t] + 1);
             ex[t][h][r] = sees ? ex[t][h][r] : -INFINITY;
           }
     }
@@ -290,24 +311,32 @@ struct Walk {
       }
     }
     bf16x8_t p[NS][RT];
+    if (inside) {
 #pragma unroll
-    for (int h = 0; h < 2; ++h)
+      for (int t = 0; t < RT; ++t)
 #pragma unroll
-      for (int r = 0; r < 4; ++r) {
+        for (int h = 0; h < 2; ++h)
 #pragma unroll
-        for (int t = 0; t < RT; ++t) {
-          const float e = __builtin_amdgcn_exp2f(ex[t][h][r]);
-          l[t] += e;
-          if (inside) {
+          for (int r = 0; r < 4; ++r) {
+            const float e = __builtin_amdgcn_exp2f(ex[t][h][r]);
+            l[t] += e;
             c[t] = fmaf(e, vmid[h][r], c[t]);
             ex[t][h][r] = e * vstep[h][r];
-          } else {  // a value that is not finite touches only rows that see it
+          }
+    } else {  // a value that is not finite touches only rows that see it
+#pragma unroll
+      for (int t = 0; t < RT; ++t)
+#pragma unroll
+        for (int h = 0; h < 2; ++h)
+#pragma unroll
+          for (int r = 0; r < 4; ++r) {
             const bool sees = ex[t][h][r] != -INFINITY;
+            const float e = __builtin_amdgcn_exp2f(ex[t][h][r]);
+            l[t] += e;
             c[t] = fmaf(e, sees ? vmid[h][r] : 0.f, c[t]);
             ex[t][h][r] = sees ? e * vstep[h][r] : 0.f;
           }
-        }
-      }
+    }
 #pragma unroll
     for (int t = 0; t < RT; ++t)
 #pragma unroll
@@ -386,32 +415,32 @@ __device__ __forceinline__ float inverse_sum(float m, float l, bool sink) {
   return l == 0.f ? 0.f : 1.f / l;
 }
 
-// Waves a SIMD holds: three where a wave has few rows of up to 128 elements, one where queries and sums alone take most of half the registers.
+// Waves a SIMD holds: one where queries and sums alone take most of half the registers, else two (three, of the kernels that could: level).
 constexpr int residents(int RT, int NS) { return NS == 3 && D > 160 ? 1 : 2; }
 
 // BY16: pages of a multiple of 16 tokens, so that 16 keys lie in one page and where they begin is the same for the whole wave, and pools of
 // less than 4 GiB. A lane finds the page of 16 keys, 32 blocks of 32 at a time, and the loads take it from there into a scalar: finding
 // pages with scalar instructions, block after block, took a hundred of them a block.
-template <int RT, int NS, bool KEYS, bool CAP, bool BY16, typename T>
-__global__ __launch_bounds__(256, residents(RT, NS)) void attention4_kernel(Attention4Args a, PageMagic magic, PageMagic g_magic) {
+template <int RT, int NS, int GROUPS, int BANDS, bool CAP, bool BY16, typename T>
+__global__ __launch_bounds__(64 * GROUPS * BANDS, residents(RT, NS)) void attention4_kernel(Attention4Args a) {
   const int lane = threadIdx.x & 63, wave = uniform_wave_number(), quad = lane >> 4;
   const int head = blockIdx.x, tile = blockIdx.y, piece = blockIdx.z;
-  constexpr int TILE_ROWS = KEYS ? 16 : 64 * RT, STEP = KEYS ? 4 : 1;
+  constexpr int TILE_ROWS = 16 * RT * BANDS;
+  const int group = wave / BANDS, band = wave % BANDS;
   // What the launch's shapes hang on is read through the scalar cache: the page numbers of the first keys, which without a window do not
   // wait for the lengths, and these come together.
   typedef const int __attribute__((address_space(4)))* constant_ints;
   auto constant = [](const int* p, int i) { return ((constant_ints)p)[__builtin_amdgcn_readfirstlane(i)]; };
   const int seq = a.tile_seq ? constant(a.tile_seq, tile) : tile, row0 = a.tile_row0 ? constant(a.tile_row0, tile) : 0;
-  const int g = g_magic.size;
+  const int g = a.group.size;
   const bool from_start = !a.window && !a.chunk;
-  const int* table = a.table + (size_t)seq * a.table_width;
   // A row: one token of a head. A page number from the table, wherever it points, is brought into the pool: given-back pages are
   // masked, but asked for.
-  auto row_of = [&](int entry, int off) { return (unsigned)((max(0, min(entry, a.num_pages - 1)) * a.nkv + head) * a.page_size + off); };
-  auto row_of_key = [&](int key) {
+  auto row_of_key = [&](const auto& a, int key) {
     int page, off;
-    page_of(magic, key, page, off);
-    return row_of(table[min(page, a.table_width - 1)], off);
+    page_of(PageMagic{a.page.size, a.page.by}, key, page, off);
+    const int entry = (a.table + (size_t)seq * a.table_width)[min(page, a.table_width - 1)];
+    return (unsigned)((max(0, min(entry, a.num_pages - 1)) * a.nkv + head) * a.page_size + off);
   };
 #ifdef __HIP_DEVICE_COMPILE__
   constexpr int RAW = 0x00020000;  // a buffer of bytes
@@ -431,7 +460,7 @@ __global__ __launch_bounds__(256, residents(RT, NS)) void attention4_kernel(Atte
         st.k[h] = load_words<KS>(k_buf, (lane & 15) * (D / 2) + quad * (D / 8), row * (D / 2));
         st.v[h] = load_words<KS>(v_buf, quad * (2 * D) + (lane & 15) * (D / 8), row * (D / 2));
       } else {
-        const size_t krow = row_of_key(32 * b + 16 * h + (lane & 15)), grow = row_of_key(32 * b + 16 * h + 4 * quad);
+        const size_t krow = row_of_key(a, 32 * b + 16 * h + (lane & 15)), grow = row_of_key(a, 32 * b + 16 * h + 4 * quad);
         st.k[h] = load_words<KS>(a.k + krow * (D / 2) + quad * (D / 8));
         st.v[h] = load_words<KS>(a.v + grow * (D / 2) + (lane & 15) * (D / 8));
       }
@@ -440,7 +469,7 @@ __global__ __launch_bounds__(256, residents(RT, NS)) void attention4_kernel(Atte
       const unsigned row0 = (unsigned)__builtin_amdgcn_readlane((int)found, 2 * j), row1 = (unsigned)__builtin_amdgcn_readlane((int)found, 2 * j + 1);
       st.s = load_words<1>(s_buf, 8 * ((lane & 16 ? row1 : row0) + (lane & 15)) + 4 * (lane >> 5), 0).w[0];
     } else {
-      st.s = a.steps[2 * (size_t)row_of_key(32 * b + (lane & 31)) + (lane >> 5)];
+      st.s = a.steps[2 * (size_t)row_of_key(a, 32 * b + (lane & 31)) + (lane >> 5)];
     }
 #endif
     return st;
@@ -449,33 +478,32 @@ __global__ __launch_bounds__(256, residents(RT, NS)) void attention4_kernel(Atte
   constexpr int FOUND = 30;  // blocks of a batch: the lanes find 32, one of them is fetched in the batch before
   auto key_of_lane = [&](int b) { return 32 * b + 16 * (lane & 1); };
   unsigned found = 0;
-  if (BY16 && from_start) found = row_of_key(key_of_lane(i0 + (KEYS ? wave : 0) + (lane >> 1) * STEP));
+  if (BY16 && from_start) found = row_of_key(a, key_of_lane(i0 + group + (lane >> 1) * GROUPS));
   const int q0 = constant(a.cu_q, seq), q_len = constant(a.cu_q, seq + 1) - q0, kv_len = constant(a.kv_lens, seq);
   const int rows = q_len * g, before = kv_len - q_len;
   if (row0 >= rows || before < 0) return;
   const Blocks all = blocks_of(a, row0, TILE_ROWS, rows, g, before);
   int end = min(all.count, i0 + a.piece);
   if (i0 >= all.count) {  // the sequence has no such piece: its parts say so
-    for (int r = row0 + threadIdx.x; r < min(row0 + TILE_ROWS, rows); r += 256)
+    for (int r = row0 + threadIdx.x; r < min(row0 + TILE_ROWS, rows); r += 64 * GROUPS * BANDS)
       *(f32x2_t*)(a.part_ml + 2 * (((size_t)(q0 + r / g) * a.nq + head * g + r % g) * a.pieces + piece)) = (f32x2_t){-INFINITY, 0.f};
     return;
   }
-  const int base = KEYS ? row0 : row0 + wave * 16 * RT;
+  const int base = row0 + band * 16 * RT;
   const int last_pos = before + (min(base + 16 * RT, rows) - 1) / g, first_pos = before + base / g;
-  if (KEYS) {
-    i0 += wave;
-  } else {
-    if (base >= rows) return;
+  if (BANDS > 1) {
+    if (GROUPS == 1 && base >= rows) return;
     // this wave's own rows may see less than the tile's
-    end = min(end, all.kept + max(0, (last_pos >> 5) + 1 - all.first));
+    end = base < rows ? min(end, all.kept + max(0, (last_pos >> 5) + 1 - all.first)) : 0;
     const int own_first = all.kept + (lowest_seen(a, first_pos) >> 5) - all.first;
     if (a.keep_first == 0) i0 = max(i0, own_first);
   }
+  i0 += group;
   const int last_low = lowest_seen(a, last_pos);
-  __shared__ __align__(16) Scales scales[4];
+  __shared__ __align__(16) Scales scales[GROUPS * BANDS];
   Walk<RT, NS, CAP> walk;
   const float unit = CAP ? a.scale : a.scale * LOG2E;
-  walk.template load_queries<T>(a, unit, head, g_magic, q0, base, rows, before, lane);
+  walk.template load_queries<T>(a, unit, head, a.group, q0, base, rows, before, lane);
 
   auto block_at = [&](int i) { return from_start ? i : all.at(max(0, min(i, all.count - 1))); };  // past the end none that is used
   auto use = [&](const Stage& st, int i) {
@@ -484,75 +512,99 @@ __global__ __launch_bounds__(256, residents(RT, NS)) void attention4_kernel(Atte
     walk.block(a, unit, st, scales[wave], b, inside, lane);
   };
   if (i0 < end) {
-    if (BY16 && !from_start) found = row_of_key(key_of_lane(block_at(i0 + (lane >> 1) * STEP)));
+    if (BY16 && !from_start) found = row_of_key(a, key_of_lane(block_at(i0 + (lane >> 1) * GROUPS)));
     Stage s0 = load(block_at(i0), found, 0), s1;
     unsigned later = 0;
     int j = FOUND;  // where the batch stands
     for (int i = i0;;) {
-      if ((i - i0) / STEP % 8 == 0) walk.center();
+      if ((i - i0) / GROUPS % 8 == 0) walk.center();
       if (BY16 && j == FOUND) {  // j runs by two: a batch's rows are found while the one before is used
         if (i != i0) found = later;
-        later = row_of_key(key_of_lane(block_at(i + (FOUND + (lane >> 1)) * STEP)));
+#ifdef __HIP_DEVICE_COMPILE__
+        later = row_of_key(*arguments(), key_of_lane(block_at(i + (FOUND + (lane >> 1)) * GROUPS)));
+#endif
         j = 0;
       }
-      s1 = load(block_at(i + STEP), found, j + 1);
+      s1 = load(block_at(i + GROUPS), found, j + 1);
       use(s0, i);
-      i += STEP;
+      i += GROUPS;
       if (i >= end) break;
-      s0 = load(block_at(i + STEP), found, j + 2);
+      s0 = load(block_at(i + GROUPS), found, j + 2);
       use(s1, i);
-      i += STEP;
+      i += GROUPS;
       if (i >= end) break;
       j += 2;
     }
   }
   walk.end();
-  if constexpr (KEYS) {
-    __shared__ float row_m[4][16], row_l[4][16], row_c[4][16];
-    __shared__ f32x4_t meet[3][2 * KS][64];
-    if (quad == 0) row_m[wave][lane] = walk.ref[0], row_l[wave][lane] = walk.l[0], row_c[wave][lane] = walk.c[0];
+  if constexpr (GROUPS > 1) {
+    // the groups' sums meet in the first one, some of the outputs at a time
+    constexpr int TURN = 2 * KS <= 8 || BANDS == 1 ? 2 * KS : KS;
+    __shared__ float row_m[GROUPS][BANDS][RT][16], row_l[GROUPS][BANDS][RT][16], row_c[GROUPS][BANDS][RT][16];
+    __shared__ f32x4_t meet[GROUPS - 1][BANDS][TURN][64];
+    if (quad == 0)
+#pragma unroll
+      for (int t = 0; t < RT; ++t)
+        row_m[group][band][t][lane] = walk.ref[t], row_l[group][band][t][lane] = walk.l[t], row_c[group][band][t][lane] = walk.c[t];
     __syncthreads();
     const int r = lane & 15;
-    const float m = fmaxf(fmaxf(row_m[0][r], row_m[1][r]), fmaxf(row_m[2][r], row_m[3][r]));
-    float l = 0.f, c = 0.f;
 #pragma unroll
-    for (int w = 0; w < 4; ++w) {
-      const float by = row_m[w][r] == -INFINITY ? 0.f : __builtin_amdgcn_exp2f(row_m[w][r] - m);
-      // a wave without a block has no sums; one whose scores are all NaN has sums that are
-      l += row_m[w][r] == -INFINITY ? row_l[w][r] : row_l[w][r] * by;
-      c += row_m[w][r] == -INFINITY ? row_c[w][r] : row_c[w][r] * by;
-      if (w == wave && row_m[w][r] != -INFINITY)
+    for (int t = 0; t < RT; ++t) {
+      float m = -INFINITY, l = 0.f, c = 0.f;
 #pragma unroll
-        for (int d = 0; d < 2 * KS; ++d) walk.acc[0][d] *= by;
+      for (int w = 0; w < GROUPS; ++w) m = fmaxf(m, row_m[w][band][t][r]);
+#pragma unroll
+      for (int w = 0; w < GROUPS; ++w) {
+        const float own = row_m[w][band][t][r], by = own == -INFINITY ? 0.f : __builtin_amdgcn_exp2f(own - m);
+        // a group without a block has no sums; one whose scores are all NaN has sums that are
+        l += own == -INFINITY ? row_l[w][band][t][r] : row_l[w][band][t][r] * by;
+        c += own == -INFINITY ? row_c[w][band][t][r] : row_c[w][band][t][r] * by;
+        if (w == group && own != -INFINITY)
+#pragma unroll
+          for (int d = 0; d < 2 * KS; ++d) walk.acc[t][d] *= by;
+      }
+#pragma unroll
+      for (int d0 = 0; d0 < 2 * KS; d0 += TURN) {
+        if (t + d0 > 0) __syncthreads();  // what met before is read
+        if (group > 0)
+#pragma unroll
+          for (int d = 0; d < TURN; ++d) meet[group - 1][band][d][lane] = walk.acc[t][d0 + d];
+        __syncthreads();
+        if (group == 0)
+#pragma unroll
+          for (int d = 0; d < TURN; ++d) {
+            f32x4_t others = meet[GROUPS - 2][band][d][lane];
+#pragma unroll
+            for (int w = GROUPS - 3; w >= 0; --w) others = meet[w][band][d][lane] + others;
+            walk.acc[t][d0 + d] += others;
+          }
+      }
+      walk.ref[t] = m, walk.l[t] = l, walk.c[t] = c;
     }
-    if (wave > 0)
-#pragma unroll
-      for (int d = 0; d < 2 * KS; ++d) meet[wave - 1][d][lane] = walk.acc[0][d];
-    __syncthreads();
-    if (wave > 0) return;
-#pragma unroll
-    for (int d = 0; d < 2 * KS; ++d) walk.acc[0][d] += meet[0][d][lane] + (meet[1][d][lane] + meet[2][d][lane]);
-    walk.ref[0] = m, walk.l[0] = l, walk.c[0] = c;
+    if (group > 0) return;
   }
+#ifdef __HIP_DEVICE_COMPILE__
+  const Arguments e = arguments();
 #pragma unroll
   for (int t = 0; t < RT; ++t) {
     const int r = base + 16 * t + (lane & 15);
     if (r >= rows) continue;
     int token, in_group;
-    page_of(g_magic, r, token, in_group);
-    const size_t row = (size_t)(q0 + token) * a.nq + head * g + in_group;
-    if (a.pieces > 1) {
-      float* to = a.part_o + (row * a.pieces + piece) * D;
+    page_of(PageMagic{e->group.size, e->group.by}, r, token, in_group);
+    const size_t row = (size_t)(q0 + token) * e->nq + head * (int)e->group.size + in_group;
+    if (e->pieces > 1) {
+      float* to = e->part_o + (row * e->pieces + piece) * D;
 #pragma unroll
       for (int d = 0; d < 2 * KS; ++d) *(f32x4_t*)(to + 16 * d + 4 * quad) = walk.acc[t][d] + walk.c[t];
-      if (quad == 0) *(f32x2_t*)(a.part_ml + 2 * (row * a.pieces + piece)) = (f32x2_t){walk.ref[t], walk.l[t]};
+      if (quad == 0) *(f32x2_t*)(e->part_ml + 2 * (row * e->pieces + piece)) = (f32x2_t){walk.ref[t], walk.l[t]};
     } else {
-      const float by = inverse_sum(walk.ref[t], walk.l[t], a.sink);
-      T* to = (T*)a.out + row * D;
+      const float by = inverse_sum(walk.ref[t], walk.l[t], e->sink);
+      T* to = (T*)e->out + row * D;
 #pragma unroll
       for (int d = 0; d < 2 * KS; ++d) store_out4<T>(to + 16 * d + 4 * quad, (walk.acc[t][d] + walk.c[t]) * by);
     }
   }
+#endif
 }
 
 // The pieces of a row, a block a row: weights of all pieces first, then their sums, every group of D / 4 threads a share of the pieces
@@ -604,11 +656,11 @@ __global__ __launch_bounds__(256) void attention4_merge_kernel(T* out, const flo
   store_out4<T>(out + row * D + 4 * threadIdx.x, o * inverse_sum(m, l, sink));
 }
 
-template <int RT, int NS, bool KEYS, typename T>
+template <int RT, int NS, int GROUPS, int BANDS, typename T>
 static int launch(const Attention4Args& a, hipStream_t stream) {
   const dim3 grid(a.nkv, a.num_tiles, a.pieces);
   const bool by16 = a.page_size % 16 == 0 && (int64_t)a.num_pages * a.nkv * a.page_size * (D / 2 > 8 ? D / 2 : 8) < (1ll << 32);
-#define GO(CAP, BY16) attention4_kernel<RT, NS, KEYS, CAP, BY16, T><<<grid, 256, 0, stream>>>(a, page_magic(a.page_size), page_magic(a.nq / a.nkv))
+#define GO(CAP, BY16) attention4_kernel<RT, NS, GROUPS, BANDS, CAP, BY16, T><<<grid, 64 * GROUPS * BANDS, 0, stream>>>(a)
   if (a.softcap > 0.f) {
     if (by16) GO(true, true);
     else GO(true, false);
@@ -625,34 +677,39 @@ static int launch(const Attention4Args& a, hipStream_t stream) {
   return 0;
 }
 
-// keys: tiles of up to 16 rows, the waves of a block share its keys; otherwise tiles of 64 row_tiles rows. parts: room for the pieces' sums, behind whose
-// ml_at bytes come their maxima and weights (not needed for one piece).
+// A tile is 64 / groups * row_tiles rows of a sequence. parts: room for the pieces' sums, behind whose ml_at bytes come their maxima and weights (not
+// needed for one piece).
 extern "C" int qrt_attention4(const Attention4Plan* plan, const void* q, void* out, const void* k, const void* v, const void* steps, const int* cu_q,
                               const int* kv_lens, const int* table, void* parts, int64_t ml_at, int table_width, int num_pages, int page_size, int sink,
-                              float scale, float softcap, int dtype, int keys, int row_tiles, hipStream_t stream) {
-  const Attention4Args a{*plan, q, out, (const uint8_t*)k, (const uint8_t*)v, (const unsigned*)steps, cu_q, kv_lens, table, (float*)parts,
-                         (float*)((char*)parts + ml_at), table_width, num_pages, page_size, sink, scale, softcap};
+                              float scale, float softcap, int dtype, int groups, int row_tiles, hipStream_t stream) {
+  Attention4Args a{*plan, q, out, (const uint8_t*)k, (const uint8_t*)v, (const unsigned*)steps, cu_q, kv_lens, table, (float*)parts,
+                         (float*)((char*)parts + ml_at), table_width, num_pages, page_size, sink, scale, softcap, {}, {}};
   QRT_CHECK(dtype == QRT_BF16 || dtype == QRT_F32, "attention4: unknown dtype %d", dtype);
   QRT_CHECK(a.nq > 0 && a.nkv > 0 && a.nq % a.nkv == 0, "attention4: %d query heads on %d key heads", a.nq, a.nkv);
   QRT_CHECK(a.page_size >= 4 && a.page_size % 4 == 0 && a.num_pages > 0 && a.table_width > 0, "attention4: pages of a multiple of 4 tokens, not %d", a.page_size);
+  a.page = page_magic(a.page_size), a.group = page_magic(a.nq / a.nkv);
   QRT_CHECK((int64_t)a.num_pages * a.nkv * a.page_size < (1ll << 31), "attention4: a pool of %d pages of %d tokens and %d heads has too many rows", a.num_pages, a.page_size, a.nkv);
   QRT_CHECK(a.window >= 0 && a.chunk >= 0 && a.keep_first >= 0 && !(a.window && a.chunk) && !(a.keep_first && !a.window), "attention4: bad mask");
   QRT_CHECK(a.piece > 0 && a.pieces > 0 && a.pieces <= MOST_PIECES, "attention4: bad pieces %d of %d", a.pieces, a.piece);
   QRT_CHECK(a.pieces == 1 || (a.part_o && ml_at > 0 && ml_at % 16 == 0 && a.num_merge_tokens > 0 && (int64_t)a.num_merge_tokens * a.nq < (1ll << 31)), "attention4: pieces need room for their parts");
-  QRT_CHECK((a.tile_seq != nullptr) == (a.tile_row0 != nullptr) || keys, "attention4: a list of tiles has sequences and rows");
-  QRT_CHECK(!keys || a.nq / a.nkv <= 16, "attention4: %d rows a token in a tile of 16", a.nq / a.nkv);
+  QRT_CHECK(a.tile_seq || !a.tile_row0, "attention4: a list of tiles has sequences and rows");
   QRT_CHECK(a.num_tiles <= 65535, "attention4: %d tiles in one launch, 65535 at most", a.num_tiles);
   QRT_CHECK(((uintptr_t)a.q | (uintptr_t)a.out | (uintptr_t)a.k | (uintptr_t)a.v | (uintptr_t)a.steps) % 16 == 0, "attention4: tensors must begin at multiples of 16 bytes");
   if (a.num_tiles <= 0) return 0;
+#define ROWS(RT, NS, T)                                        \
+  do {                                                         \
+    if (groups == 4) return launch<RT, NS, 4, 1, T>(a, stream); \
+    if (groups == 2) return launch<RT, NS, 2, 2, T>(a, stream); \
+    if (groups == 1) return launch<RT, NS, 1, 4, T>(a, stream); \
+  } while (0)
   if (dtype == QRT_F32) {
-    if (keys) return launch<1, 3, true, float>(a, stream);
-    QRT_CHECK(row_tiles == 1, "attention4: float32 rows go by one tile a wave");
-    return launch<1, 3, false, float>(a, stream);
+    if (row_tiles == 1) ROWS(1, 3, float);
+  } else if constexpr (D <= 128) {
+    if (row_tiles == 2) ROWS(2, 1, bf16_t);
+    if (row_tiles == 1 && groups == 4) return launch<1, 1, 4, 1, bf16_t>(a, stream);
+  } else {
+    if (row_tiles == 1) ROWS(1, 1, bf16_t);
   }
-  if (keys) return launch<1, 1, true, bf16_t>(a, stream);
-  if (row_tiles == 1) return launch<1, 1, false, bf16_t>(a, stream);
-  if constexpr (D <= 128) {
-    if (row_tiles == 2) return launch<2, 1, false, bf16_t>(a, stream);
-  }
-  return qrt_fail("attention4: no kernel with %d row tiles a wave", row_tiles);
+#undef ROWS
+  return qrt_fail("attention4: no kernel with %d groups and %d row tiles a wave", groups, row_tiles);
 }

@@ -2135,8 +2135,8 @@ class HipOps:
 
     # ---- attention over a cache of 4 bits --------------------------------------------
     def _attention4(self, q, cache, ctx, nq, nkv, d, scale, window, chunk, softcap, keep_first, sink):
-        """Sequences of at most 16 rows (tokens by heads of a group) go by blocks whose waves share their keys, the others by tiles of rows;
-        a step that has both takes a launch for either. What follows from the step's lengths is kept with its context, for its other layers."""
+        """Sequences of at most 16 rows (tokens by heads of a group) are a tile each, the others go by tiles of rows from a list; a step
+        that has both takes a launch for either. What follows from the step's lengths is kept with its context, for its other layers."""
         pages = self._check_cache4(cache, nkv, d)
         if ctx.num_tokens == 0:
             return q.new_empty((0, nq * d))
@@ -2179,13 +2179,13 @@ class HipOps:
             raise OpsError(f"queries on {q.device}, a cache on {cache.k.device}, its table on {table.device}")
         out = q.new_empty((ctx.num_tokens, nq * d))
         lib, code, stream = attention4_library(d), _CODE[q.dtype], _stream()
-        for fixed, keys, row_tiles, room, _tensors in plan:
+        for fixed, groups, row_tiles, room, _tensors in plan:
             parts = 0
             if room:
                 parts = q.new_empty((room * (d + 2),), dtype=torch.float32).data_ptr()
             if lib.qrt_attention4(fixed, q.data_ptr(), out.data_ptr(), cache.k.data_ptr(), cache.v.data_ptr(), cache.pages["steps"].data_ptr(), cu_q.data_ptr(),
                                   kv_lens.data_ptr(), table.data_ptr(), parts, 4 * room * d, table.shape[1], pages, group.page_size, sink, scale, softcap, code,
-                                  keys, row_tiles, stream):
+                                  groups, row_tiles, stream):
                 raise OpsError(lib.qrt_last_error().decode())
         return out
 
@@ -2205,11 +2205,11 @@ class HipOps:
         seqs = range(ctx.num_seqs) if subset is None else subset
         q_lens = [ctx.q_lens_host[i] for i in seqs]
         kv_lens = [ctx.kv_lens_host[i] for i in seqs]
-        row_tiles = 2 if bf and d <= 128 and not keys and max(q_lens) * g > 64 else 1
+        row_tiles, groups = (1, 4) if keys else self.choose_attention4_rows([n * g for n in q_lens], nkv, bf and d <= 128)
         tiles = tokens = None
         n_tiles = ctx.num_seqs
         if not keys:
-            host, n_tiles = self.plan_tiles(q_lens, kv_lens, g, 64 * row_tiles, nkv, self.resident_blocks, list(seqs))
+            host, n_tiles = self.plan_tiles(q_lens, kv_lens, g, 16 * row_tiles * (4 // groups), nkv, 0, list(seqs))
             tiles = torch.from_numpy(host).to(q.device)
         elif subset is not None:
             n_tiles = len(q_lens)
@@ -2232,15 +2232,36 @@ class HipOps:
         splits = ctx.scratch.get("attn_splits")
         a.piece = max(-(-most // splits), -(-most // 1024)) if splits else self.choose_attention4_piece(most, total, n_tiles, nkv, keys)
         a.pieces = -(-most // a.piece)
-        return bytes(a), int(keys), row_tiles, ctx.num_tokens * nq * a.pieces if a.pieces > 1 else 0, (tiles, tokens)
+        return bytes(a), groups, row_tiles, ctx.num_tokens * nq * a.pieces if a.pieces > 1 else 0, (tiles, tokens)
+
+    @staticmethod
+    def choose_attention4_rows(rows, nkv: int, two: bool) -> tuple[int, int]:
+        """Tiles of 16 rows a wave holds (two of them where there is such a kernel, ``two``), and into how many groups that take the
+        keys in turn a block's four waves are split, for sequences of ``rows`` rows. Figures at csrc/attention4.hip."""
+        def blocks(row_tiles, groups):
+            tile = 16 * row_tiles * (4 // groups)
+            return sum(-(-r // tile) for r in rows) * nkv
+
+        row_tiles, groups = 2 if two and blocks(2, 4) >= 384 else 1, 4
+        if two and row_tiles == 1:
+            return row_tiles, groups
+        # bands that the rows do not fill are waves without work
+        for most in (512, 1750):
+            if blocks(row_tiles, groups) > most and 3 * blocks(row_tiles, groups // 2) <= 2 * blocks(row_tiles, groups):
+                groups //= 2
+            else:
+                break
+        return row_tiles, groups
 
     @staticmethod
     def choose_attention4_piece(most: int, total: int, tiles: int, nkv: int, keys: bool) -> int:
         """Blocks of 32 keys that one block of the launch walks."""
         if keys:  # about 512 blocks of the launch, four waves of each with two blocks of keys or more, 64 pieces at most
             return max(8, -(-total * nkv // 512), -(-most // 64))
+        # one piece from 192 blocks on, 256 blocks below: us in 1, 2 and 4 pieces 256 blocks (128 tokens of 4,096) 25.7, 30.0, 31.9; 128 (eight
+        # times 8 of up to 3,000) 21.2, 18.8, 18.1; 16 (8 of 8,000) in 8, 16 and 32 13.1, 11.4, 13.2
         launch = tiles * nkv
-        return most if launch >= 512 else max(16, -(-most // -(-512 // launch)))
+        return most if launch >= 192 else max(16, -(-most // -(-256 // launch)))
 
     resident_blocks = 512  # blocks of the prompt kernels the chip holds at once: 2 on each of 256 CUs
 

@@ -246,6 +246,50 @@ def test_masks_caps_and_sinks(option, splits, dtype):
     near(ops().paged_attention(q, cache, ctx, nq, nkv, d, d ** -0.5, window, **more), want, cache)
 
 
+FORMS = [(torch.bfloat16, 64, 1, 4), (torch.bfloat16, 64, 2, 4), (torch.bfloat16, 128, 2, 2), (torch.bfloat16, 96, 2, 1), (torch.bfloat16, 160, 1, 4),
+         (torch.bfloat16, 256, 1, 2), (torch.bfloat16, 192, 1, 1), (torch.float32, 64, 1, 4), (torch.float32, 32, 1, 2), (torch.float32, 128, 1, 2),
+         (torch.float32, 256, 1, 2), (torch.float32, 96, 1, 1)]
+
+
+@gpu
+@pytest.mark.parametrize("splits", [1, 3])
+@pytest.mark.parametrize("option", [{}, {"window": 37}, {"window": 50, "keep_first": 3}, {"chunk": 48}, {"softcap": 3.0, "sink": True}])
+@pytest.mark.parametrize("ps", [16, 12])
+@pytest.mark.parametrize("dtype,d,row_tiles,groups", FORMS)
+def test_every_split_of_rows_and_keys(dtype, d, row_tiles, groups, ps, option, splits, monkeypatch):
+    """Which of them a step takes follows from its sizes; here each has to take lengths that leave bands without rows and groups without keys."""
+    from qwen3_runtime_amd.ops.hip import HipOps
+
+    monkeypatch.setattr(HipOps, "choose_attention4_rows", staticmethod(lambda rows, nkv, two: (row_tiles, groups)))
+    q, cache, ctx = case([(9, 9), (23, 131), (70, 70), (17, 300), (1, 65), (16 * 64 // 3, 400)], 6, 2, d, ps, dtype, seed=d + groups, window=option.get("window"))
+    ctx.scratch["attn_splits"] = splits
+    near(ops().paged_attention(q, cache, ctx, 6, 2, d, d ** -0.5, option.get("window"), **{k: v for k, v in option.items() if k != "window"}),
+         plain(q, cache, ctx, 6, 2, d, d ** -0.5, **option), cache)
+
+
+@gpu
+@pytest.mark.parametrize("seqs,nkv,form", [([(20, 20)] * 40, 4, (1, 4)), ([(30, 41)] * 60, 4, (2, 4)), ([(64, 70)] * 60, 4, (2, 2)), ([(33, 33)] * 500, 4, (2, 1))])
+def test_steps_that_take_each_split_by_their_sizes(seqs, nkv, form):
+    from qwen3_runtime_amd.ops.hip import HipOps
+
+    assert HipOps.choose_attention4_rows([2 * n for n, _ in seqs], nkv, True) == form
+    q, cache, ctx = case(seqs, 2 * nkv, nkv, 32, 16, torch.bfloat16, seed=len(seqs))
+    near(ops().paged_attention(q, cache, ctx, 2 * nkv, nkv, 32, 32 ** -0.5, None), plain(q, cache, ctx, 2 * nkv, nkv, 32, 32 ** -0.5), cache)
+
+
+def test_how_rows_are_split():
+    from qwen3_runtime_amd.ops.hip import HipOps
+
+    choose = HipOps.choose_attention4_rows
+    assert choose([17], 1, True) == (1, 4) and choose([17], 1, False) == (1, 4)
+    for rows, nkv in (([40] * 3000, 8), ([100000], 8), ([24] * 4000, 4), ([17, 90000], 2)):
+        for two in (True, False):
+            row_tiles, groups = choose(rows, nkv, two)
+            assert groups in (1, 2, 4) and row_tiles == (2 if two else 1)
+    assert choose([24] * 4000, 4, True) == (2, 4)  # rows that fill one band have no use for a second
+    assert choose([24] * 4000, 4, False)[1] == 2
+
+
 @gpu
 @pytest.mark.parametrize("dtype", [torch.bfloat16, torch.float32])
 @pytest.mark.parametrize("value", [float("nan"), float("inf")])
