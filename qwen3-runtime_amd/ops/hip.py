@@ -13,7 +13,9 @@ weights, bfloat16 with more rows to its tiles through LDS; what those do not
 take (K no multiple of 64, weight rows no multiple of 16, operands off 16
 bytes), and what fills the vendor BLAS's own tiles beyond 2,048 rows (with
 4,096 columns of K beyond 1,536), goes to that through ``torch.matmul``, as the reference leaves its products to
-cuBLAS (qwen3_runtime/models/qwen3.py:76-77,134-135).
+cuBLAS (qwen3_runtime/models/qwen3.py:76-77,134-135). Weights in 8 bits
+(``Int8Weight``) go to the library's own kernels with any number of rows, and so
+does a cache of 4 bits: its store and its attention.
 """
 
 from __future__ import annotations
@@ -1985,7 +1987,8 @@ class HipOps:
         raise OpsError(f"a cache on {cache.k.device}, {cache.v.device} and {steps.device}")
 
     def kv_store(self, k, v, cache):
-        """``k``, ``v`` [T, heads, D] into their places in the cache."""
+        """``k``, ``v`` [T, heads, D] into their places in the cache (``cache.group.slots``, each place at most once in a call; a token
+        whose place is in no page is left out)."""
         t, nkv, d = k.shape
         _need(k, "k")
         _need(v, "v", k.dtype, (t, nkv, d))

@@ -117,6 +117,30 @@ def test_store(t, nkv, d, ps, dtype):
 
 
 @gpu
+@pytest.mark.parametrize("t", [29, 400])
+def test_codes_of_vectors_of_any_magnitude(t):
+    """Quotients as a division rounds them: magnitudes from 2^-120 to 2^120, quotients at halves of whole numbers and next to them."""
+    g = gen(t)
+    nkv, d, ps = 2, 64, 16
+    x = torch.randn(2, t, nkv, d, generator=g)
+    ties = torch.arange(d) % 31 / 2 + torch.randint(-1, 2, (2, t // 2, nkv, d), generator=g) * 2.0 ** -22
+    ties[..., 0], ties[..., 1] = 0.0, 15.0
+    x[:, : t // 2] = ties * (1 + torch.randint(0, 128, (2, t // 2, nkv, 1), generator=g) / 128)
+    x = x * 2.0 ** torch.randint(-120, 121, (2, t, nkv, 1), generator=g).float()
+    cache, want = empty_cache(-(-t // ps), nkv, ps, d), empty_cache(-(-t // ps), nkv, ps, d)
+    at = torch.arange(t)
+    cache.group.slots = at.to(torch.int32).to(DEV)
+    ops().kv_store(x[0].to(DEV), x[1].to(DEV), cache)
+    put(want, at // ps, at % ps, x[0], x[1], d)
+    same(cache, want)
+    qkv = torch.cat([torch.zeros(t, d), x[0].reshape(t, -1), x[1].reshape(t, -1)], 1)  # without a norm or a turn: few tokens by the other kernel
+    cache = empty_cache(-(-t // ps), nkv, ps, d)
+    cache.group.slots = at.to(torch.int32).to(DEV)
+    ops().qk_norm_rope_store(qkv.to(DEV), 1, nkv, d, None, None, 1e-6, None, at.to(torch.int32).to(DEV), cache)
+    same(cache, want)
+
+
+@gpu
 def test_store_leaves_out_slots_in_no_page_and_marks_what_is_not_finite():
     t, nkv, d, ps = 9, 2, 128, 16
     k, v = torch.randn(t, nkv, d, generator=gen(1)), torch.randn(t, nkv, d, generator=gen(2))
