@@ -77,9 +77,14 @@ __device__ __forceinline__ int lowest_seen(const Attention4Args& a, int pos) {
   if (a.window) return max(0, pos - a.window + 1);
   return a.chunk ? pos - pos % a.chunk : 0;
 }
-__device__ __forceinline__ Blocks blocks_of(const Attention4Args& a, int base, int tile_rows, int rows, int g, int before) {
-  const int last = before + (min(base + tile_rows, rows) - 1) / g;
-  const int low = lowest_seen(a, before + base / g);
+__device__ __forceinline__ int token_of_row(const Attention4Args& a, int row) {
+  int token, in_group;
+  page_of(a.group, row, token, in_group);
+  return token;
+}
+__device__ __forceinline__ Blocks blocks_of(const Attention4Args& a, int base, int tile_rows, int rows, int before) {
+  const int last = before + token_of_row(a, min(base + tile_rows, rows) - 1);
+  const int low = lowest_seen(a, before + token_of_row(a, base));
   Blocks b;
   b.first = low >> 5;
   b.kept = min((a.keep_first + 31) >> 5, b.first);
@@ -482,7 +487,7 @@ __global__ __launch_bounds__(64 * GROUPS * BANDS, residents(RT, NS)) void attent
   const int q0 = constant(a.cu_q, seq), q_len = constant(a.cu_q, seq + 1) - q0, kv_len = constant(a.kv_lens, seq);
   const int rows = q_len * g, before = kv_len - q_len;
   if (row0 >= rows || before < 0) return;
-  const Blocks all = blocks_of(a, row0, TILE_ROWS, rows, g, before);
+  const Blocks all = blocks_of(a, row0, TILE_ROWS, rows, before);
   int end = min(all.count, i0 + a.piece);
   if (i0 >= all.count) {  // the sequence has no such piece: its parts say so
     for (int r = row0 + threadIdx.x; r < min(row0 + TILE_ROWS, rows); r += 64 * GROUPS * BANDS)
@@ -490,7 +495,7 @@ __global__ __launch_bounds__(64 * GROUPS * BANDS, residents(RT, NS)) void attent
     return;
   }
   const int base = row0 + band * 16 * RT;
-  const int last_pos = before + (min(base + 16 * RT, rows) - 1) / g, first_pos = before + base / g;
+  const int last_pos = before + token_of_row(a, min(base + 16 * RT, rows) - 1), first_pos = before + token_of_row(a, base);
   if (BANDS > 1) {
     if (GROUPS == 1 && base >= rows) return;
     // this wave's own rows may see less than the tile's
@@ -500,20 +505,23 @@ __global__ __launch_bounds__(64 * GROUPS * BANDS, residents(RT, NS)) void attent
   }
   i0 += group;
   const int last_low = lowest_seen(a, last_pos);
+  auto block_at = [&](int i) { return from_start ? i : all.at(max(0, min(i, all.count - 1))); };  // past the end none that is used
+  Stage s0, s1;  // the first block is on its way while the queries are made ready
+  if (i0 < end) {
+    if (BY16 && !from_start) found = row_of_key(a, key_of_lane(block_at(i0 + (lane >> 1) * GROUPS)));
+    s0 = load(block_at(i0), found, 0);
+  }
   __shared__ __align__(16) Scales scales[GROUPS * BANDS];
   Walk<RT, NS, CAP> walk;
   const float unit = CAP ? a.scale : a.scale * LOG2E;
   walk.template load_queries<T>(a, unit, head, a.group, q0, base, rows, before, lane);
 
-  auto block_at = [&](int i) { return from_start ? i : all.at(max(0, min(i, all.count - 1))); };  // past the end none that is used
   auto use = [&](const Stage& st, int i) {
     const int b = block_at(i);
     const bool inside = 32 * b + 31 <= first_pos && (32 * b >= last_low || 32 * b + 31 < a.keep_first);
     walk.block(a, unit, st, scales[wave], b, inside, lane);
   };
   if (i0 < end) {
-    if (BY16 && !from_start) found = row_of_key(a, key_of_lane(block_at(i0 + (lane >> 1) * GROUPS)));
-    Stage s0 = load(block_at(i0), found, 0), s1;
     unsigned later = 0;
     int j = FOUND;  // where the batch stands
     for (int i = i0;;) {
