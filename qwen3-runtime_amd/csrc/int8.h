@@ -45,4 +45,4 @@ __device__ __forceinline__ unsigned codes4(float a, float b, float c, float d, f
 }
 
 int int8_tiles(const void* a, const float* a_scale, const void* w, const float* w_scale, void* c, int out_dtype, int M, int N, int width, int tile,
-               int act_kind, float limit, hipStream_t stream);
+               int parts, int act_kind, float limit, hipStream_t stream);

@@ -132,6 +132,7 @@ template <typename TD, int KEEP, bool ROUND>
 __global__ __launch_bounds__(256) void add_rmsnorm_codes_kernel(float* __restrict__ residual, const TD* __restrict__ delta, const float* __restrict__ weight,
                                                                 int8_t* __restrict__ codes, float* __restrict__ scale, int hidden, int width, float eps,
                                                                 int planes, size_t plane_stride) {
+  constexpr int AHEAD = KEEP > 4 ? 2 : 4;
   __shared__ float red[16];
   __shared__ unsigned part[4];
   float* x = residual + (size_t)blockIdx.x * hidden;
@@ -143,17 +144,21 @@ __global__ __launch_bounds__(256) void add_rmsnorm_codes_kernel(float* __restric
     const int at = min(4 * ((int)threadIdx.x + 256 * i), hidden - 4);
     v[i] = *(const f32x4_t*)(x + at), w[i] = *(const f32x4_t*)(weight + at);
   }
-  if (planes > 0) {
+  typedef TD dvec_t __attribute__((ext_vector_type(4)));
+  for (int p = 0; p < planes; p += AHEAD) {  // a load that waits for the one before costs a microsecond
+    dvec_t y[AHEAD][KEEP];
 #pragma unroll
-    for (int i = 0; i < KEEP; ++i) {
-      const int at = min(4 * ((int)threadIdx.x + 256 * i), hidden - 4);
-      for (int p = 0; p < planes; ++p) {
-        typedef TD dvec_t __attribute__((ext_vector_type(4)));
-        const dvec_t y = *(const dvec_t*)(d + p * plane_stride + at);
+    for (int q = 0; q < AHEAD; ++q)
 #pragma unroll
-        for (int e = 0; e < 4; ++e) v[i][e] += to_f32<TD>(y[e]);
-      }
-    }
+      for (int i = 0; i < KEEP; ++i)
+        y[q][i] = *(const dvec_t*)(d + min(p + q, planes - 1) * plane_stride + min(4 * ((int)threadIdx.x + 256 * i), hidden - 4));
+#pragma unroll
+    for (int q = 0; q < AHEAD; ++q)
+      if (p + q < planes)
+#pragma unroll
+        for (int i = 0; i < KEEP; ++i)
+#pragma unroll
+          for (int e = 0; e < 4; ++e) v[i][e] += to_f32<TD>(y[q][i][e]);
   }
 #pragma unroll
   for (int i = 0; i < KEEP; ++i) {
@@ -473,15 +478,15 @@ static int int8_rows(const void* x, int x_dtype, const void* a, const float* a_s
 // 9,728 x 2,560 19.7, 25.4 and 21.2, 21.2; 2,560 x 9,728 19.9, 23.0 and 26.3, 26.3.
 constexpr bool streams(int M, int N, bool gated) { return M <= 48 || (M <= 64 && N * (gated ? 2 : 1) < 32 * 192); }
 
-// Bytes of workspace that qrt_int8_product wants: none, or the rows' codes and scales.
+static int64_t codes_room(int M, int width) { return (int64_t)M * width + 4 * (((int64_t)M + 3) & ~3ll); }
+
+// Bytes of workspace that qrt_int8_product wants: none, or the rows' codes and scales; always these with parts of K.
 extern "C" int64_t qrt_int8_workspace(int M, int N, int K, int width) {
-  return K % 8 == 0 && fused_takes(M, N, width) ? 0 : (int64_t)M * width + 4 * (((int64_t)M + 3) & ~3ll);
+  return K % 8 == 0 && fused_takes(M, N, width) ? 0 : codes_room(M, width);
 }
 
-// c [M, N] (out_dtype) = rows x [M, K] (x_dtype) by w [N, width] and w_scale [N], or with a gate (act_kind >= 0) w [2 N, width], w_scale [2 N] and the activation
-// of the two. With codes_scale [M] (not null) x is codes already, [M, width]. tile: a number of TILES in ops/hip.py, for more than 48 rows.
-extern "C" int qrt_int8_product(const void* x, int x_dtype, const float* codes_scale, const void* w, const float* w_scale, void* c, int out_dtype, void* workspace, int M, int N,
-                                int K, int width, int tile, int act_kind, float limit, hipStream_t stream) {
+static int int8_product(const void* x, int x_dtype, const float* codes_scale, const void* w, const float* w_scale, void* c, int out_dtype, void* workspace, int M, int N,
+                        int K, int width, int tile, int parts, int act_kind, float limit, hipStream_t stream) {
   if (check_width("int8_product", M, K, width)) return -1;
   QRT_CHECK(N > 0 && N < (1 << 30), "int8_product: bad size N=%d", N);
   QRT_CHECK(x_dtype == QRT_BF16 || x_dtype == QRT_F32, "int8_product: unknown dtype %d", x_dtype);
@@ -491,10 +496,10 @@ extern "C" int qrt_int8_product(const void* x, int x_dtype, const float* codes_s
   if (codes_scale) {
     QRT_CHECK((uintptr_t)x % 16 == 0, "int8_product: codes must begin at a multiple of 16 bytes");
     if (M == 0) return 0;
-    if (streams(M, N, act_kind >= 0)) return int8_rows(nullptr, x_dtype, x, codes_scale, w, w_scale, c, out_dtype, M, N, K, width, act_kind, limit, stream);
-    return int8_tiles(x, codes_scale, w, w_scale, c, out_dtype, M, N, width, tile, act_kind, limit, stream);
+    if (parts == 1 && streams(M, N, act_kind >= 0)) return int8_rows(nullptr, x_dtype, x, codes_scale, w, w_scale, c, out_dtype, M, N, K, width, act_kind, limit, stream);
+    return int8_tiles(x, codes_scale, w, w_scale, c, out_dtype, M, N, width, tile, parts, act_kind, limit, stream);
   }
-  const int64_t room = qrt_int8_workspace(M, N, K, width);
+  const int64_t room = parts == 1 ? qrt_int8_workspace(M, N, K, width) : codes_room(M, width);
   QRT_CHECK(room == 0 || workspace, "int8_product: %d rows of %d columns need a workspace", M, K);
   QRT_CHECK(room > 0 || (uintptr_t)x % 16 == 0, "int8_product: rows must begin at a multiple of 16 bytes");
   if (M == 0) return 0;
@@ -502,6 +507,19 @@ extern "C" int qrt_int8_product(const void* x, int x_dtype, const float* codes_s
   int8_t* const codes = (int8_t*)workspace;
   float* const scale = (float*)(codes + (int64_t)M * width);
   if (qrt_quantize_rows(x, x_dtype, codes, scale, M, K, width, stream)) return -1;
-  if (streams(M, N, act_kind >= 0)) return int8_rows(nullptr, x_dtype, codes, scale, w, w_scale, c, out_dtype, M, N, K, width, act_kind, limit, stream);
-  return int8_tiles(codes, scale, w, w_scale, c, out_dtype, M, N, width, tile, act_kind, limit, stream);
+  if (parts == 1 && streams(M, N, act_kind >= 0)) return int8_rows(nullptr, x_dtype, codes, scale, w, w_scale, c, out_dtype, M, N, K, width, act_kind, limit, stream);
+  return int8_tiles(codes, scale, w, w_scale, c, out_dtype, M, N, width, tile, parts, act_kind, limit, stream);
+}
+
+// c [M, N] (out_dtype) = rows x [M, K] (x_dtype) by w [N, width] and w_scale [N], or with a gate (act_kind >= 0) w [2 N, width], w_scale [2 N] and the activation
+// of the two. With codes_scale [M] (not null) x is codes already, [M, width]. tile: a number of TILES in ops/hip.py, for more than 48 rows.
+extern "C" int qrt_int8_product(const void* x, int x_dtype, const float* codes_scale, const void* w, const float* w_scale, void* c, int out_dtype, void* workspace, int M, int N,
+                                int K, int width, int tile, int act_kind, float limit, hipStream_t stream) {
+  return int8_product(x, x_dtype, codes_scale, w, w_scale, c, out_dtype, workspace, M, N, K, width, tile, 1, act_kind, limit, stream);
+}
+// The same without a gate, by tiles whatever M: planes c [parts, M, N] in float32 whose sum is the product, two parts of K or more.
+extern "C" int qrt_int8_planes(const void* x, int x_dtype, const float* codes_scale, const void* w, const float* w_scale, void* c, void* workspace, int M, int N, int K, int width,
+                               int tile, int parts, hipStream_t stream) {
+  QRT_CHECK(parts > 1, "int8_planes: %d parts of K", parts);
+  return int8_product(x, x_dtype, codes_scale, w, w_scale, c, QRT_F32, workspace, M, N, K, width, tile, parts, -1, 0.f, stream);
 }

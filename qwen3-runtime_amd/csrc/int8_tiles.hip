@@ -19,6 +19,7 @@ struct Int8TileArgs {
   void* C;
   int M, N, width;
   int mtiles, ntiles;
+  int parts;  // of K, a plane [M, N] each
   int kind;
   float limit;
 };
@@ -47,17 +48,22 @@ __global__ __launch_bounds__(64 * WM * WN, 2) void int8_tiles_kernel(Int8TileArg
   const int r16 = lane & 15, quad = lane >> 4;
 
   // Blocks reach the XCDs in turn: each gets a run of neighbouring tiles, down bands of some 2,048 rows, column by column.
-  const int total = p.mtiles * p.ntiles, stages = p.width / INT8_STAGE;
-  int m0, n0;
+  const int total = p.mtiles * p.ntiles * p.parts;
+  int m0, n0, part, s0, stages;
   unsigned aoff[T::AL], woff[T::WL];  // rows past the end repeat the last one and are not stored
   auto locate = [&](int tile) {
     const int xcd = tile & 7;
-    const int id = xcd * (total >> 3) + min(xcd, total & 7) + (tile >> 3);
+    int id = xcd * (total >> 3) + min(xcd, total & 7) + (tile >> 3);
+    part = id / (p.mtiles * p.ntiles);
+    id -= part * p.mtiles * p.ntiles;
     constexpr int BAND = 2048 / BM;
     const int band = id / (BAND * p.ntiles), in_band = id - band * BAND * p.ntiles;
     const int high = min(BAND, p.mtiles - band * BAND);
     m0 = (band * BAND + in_band % high) * BM;
     n0 = in_band / high * (GATED ? BN / 2 : BN);
+    const int all = p.width / INT8_STAGE, each = (all + p.parts - 1) / p.parts;
+    s0 = min(all, part * each);
+    stages = min(all, s0 + each) - s0;
 #pragma unroll
     for (int j = 0; j < T::AL; ++j)
       aoff[j] = (unsigned)min(m0 + T::row_of(j, T::AU, wave, lane), p.M - 1) * (unsigned)p.width + T::piece_of(lane);
@@ -79,7 +85,7 @@ __global__ __launch_bounds__(64 * WM * WN, 2) void int8_tiles_kernel(Int8TileArg
   locate(tile);
   while (true) {
     i32x4_t acc[TM][TN];
-    T::template products<0>(a_buf, w_buf, aoff, woff, 0, stages, tiles_lds, fetched, acc);
+    T::template products<0>(a_buf, w_buf, aoff, woff, s0, stages, tiles_lds, fetched, acc);
     QRT_WAIT_LDS();
     QRT_BARRIER();  // nobody reads the ring any more
     // acc[i][j][r]: row 16 i + r16 of the wave's result, row 16 j + 4 quad + r of its weights
@@ -94,13 +100,13 @@ __global__ __launch_bounds__(64 * WM * WN, 2) void int8_tiles_kernel(Int8TileArg
 #pragma unroll
       for (int r = 0; r < 4; ++r)
         sw[j][r] = p.w_scale[GATED ? min(nw + 8 * j + 4 * (quad & 1) + r, p.N - 1) + (quad & 2 ? p.N : 0) : min(nw + 16 * j + 4 * quad + r, p.N - 1)];
+    TO* C = (TO*)p.C + (size_t)part * p.M * p.N;
     const bool more = tile + (int)gridDim.x < total;
     tile += gridDim.x;
     if (more) {
       locate(tile);
-      T::template fetch_first<0>(a_buf, w_buf, aoff, woff, 0, stages, tiles_lds, 0, FIRST);
+      T::template fetch_first<0>(a_buf, w_buf, aoff, woff, s0, stages, tiles_lds, 0, FIRST);
     }
-    TO* C = (TO*)p.C;
     constexpr int PITCH = 2 * COLS + 16;
     unsigned char* own = result + wave * ROWS * PITCH;
 #pragma unroll
@@ -181,7 +187,7 @@ static int launch_int8_tiles(Int8TileArgs p, hipStream_t stream) {
   const int outs = GATED ? BN / 2 : BN;
   p.mtiles = (p.M + BM - 1) / BM;
   p.ntiles = (p.N + outs - 1) / outs;
-  const int64_t blocks = (int64_t)p.mtiles * p.ntiles;
+  const int64_t blocks = (int64_t)p.mtiles * p.ntiles * p.parts;
   QRT_CHECK(blocks < (1 << 30), "int8_tiles: too many tiles for one launch (M=%d N=%d)", p.M, p.N);
   auto kernel = int8_tiles_kernel<BM, BN, WM, WN, S, GATED, TO>;
   static bool allowed = false;  // once per kernel: not inside a stream capture again and again
@@ -206,13 +212,17 @@ static int int8_by_result(const Int8TileArgs& p, int out_dtype, hipStream_t stre
   return launch_int8_tiles<BM, BN, WM, WN, S, false, bf16_t>(p, stream);
 }
 
-// c [M, N] from codes a [M, width], w [N, width] ([2 N, width] with a gate: act_kind >= 0); tile: a number of TILES in ops/hip.py.
+// c [M, N] from codes a [M, width], w [N, width] ([2 N, width] with a gate: act_kind >= 0), or with parts > 1 (no gate, float32) planes [parts, M, N];
+// tile: a number of TILES in ops/hip.py.
 int int8_tiles(const void* a, const float* a_scale, const void* w, const float* w_scale, void* c, int out_dtype, int M, int N, int width, int tile,
-               int act_kind, float limit, hipStream_t stream) {
+               int parts, int act_kind, float limit, hipStream_t stream) {
   const uint64_t limit_bytes = (1ull << 32) - 128;  // offsets are 32 bits
   QRT_CHECK((uint64_t)M * width <= limit_bytes && (uint64_t)(act_kind >= 0 ? 2 : 1) * N * width <= limit_bytes,
             "int8_tiles: an operand of 4 GiB or more (M=%d N=%d, rows of %d)", M, N, width);
-  const Int8TileArgs p{(const int8_t*)a, a_scale, (const int8_t*)w, w_scale, c, M, N, width, 0, 0, act_kind, limit};
+  QRT_CHECK(parts == 1 || (parts > 1 && parts <= 64 && act_kind < 0 && out_dtype == QRT_F32), "int8_tiles: %d parts of K need no gate and float32 output", parts);
+  const int stages = width / INT8_STAGE, each = (stages + parts - 1) / parts;
+  QRT_CHECK(each * (parts - 1) < stages, "int8_tiles: %d parts of %d stages leave one without any", parts, stages);
+  const Int8TileArgs p{(const int8_t*)a, a_scale, (const int8_t*)w, w_scale, c, M, N, width, 0, 0, parts, act_kind, limit};
   switch (tile) {
     case 0: return int8_by_result<256, 192, 4, 2, 2>(p, out_dtype, stream);
     case 1: return int8_by_result<256, 160, 4, 2, 3>(p, out_dtype, stream);

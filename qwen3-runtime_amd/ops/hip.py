@@ -383,6 +383,7 @@ class HipOps:
         self.lib = core_library()
         # declared, the arguments travel as they are: a wrapper object for each of fifteen took 2 us a call
         self.lib.qrt_int8_product.argtypes = [c_void_p, c_int, c_void_p, c_void_p, c_void_p, c_void_p, c_int, c_void_p] + [c_int] * 6 + [c_float, c_void_p]
+        self.lib.qrt_int8_planes.argtypes = [c_void_p, c_int] + [c_void_p] * 5 + [c_int] * 6 + [c_void_p]
         self.lib.qrt_store4.argtypes = [c_void_p, c_void_p, c_int, c_long, c_long] + [c_void_p] * 4 + [c_long] + [c_int] * 4 + [c_void_p]
         self.lib.qrt_int8_workspace.argtypes, self.lib.qrt_int8_workspace.restype = [c_int] * 4, c_long
         self.residual_planes = residual_planes
@@ -1591,9 +1592,10 @@ class HipOps:
 
         May return the result in planes ``[P, T, N]`` float32 whose sum it is (``add_rmsnorm``
         adds them): a product with few rows and few weight rows then cuts K over several blocks
-        per row tile, which fills the chip (160 row tiles for 256 compute units at the 4B size)."""
+        per row tile, which fills the chip (160 row tiles for 256 compute units at the 4B size). Products of an ``Int8Weight``
+        do so from 33 rows on."""
         if isinstance(w, Int8Weight):
-            return self._int8_product(x, w, out_f32=True)
+            return self._int8_product(x, w, out_f32=True, planes=self.residual_planes)
         m, k = x.shape
         n = w.shape[0]
         if (self.residual_planes and x.dtype == torch.float32 and w.dtype == torch.float32 and w.shape == (n, k)
@@ -1721,15 +1723,20 @@ class HipOps:
             c_long(t * h), c_int(int(out_dtype == torch.bfloat16)), _stream()))
         return CodedRows(codes, scale, residual.shape, out_dtype)
 
+    # more rows than this for the residual are cut along K into planes, by tiles. us with the norm that adds them up, without planes and with: 2,560 x 9,728
+    # at 32, 64, 128, 512 and 2,048 rows 17.5, 16.7; 22.0, 18.3; 33.5, 21.6; 46.3, 34.6; 81, 74; 2,560 x 4,096 12.0, 13.3; 14.3, 14.5; 19.7, 15.7; 30.0, 27.5
+    # and one plane; 4,096 x 4,096 at 128 and 256 rows 19.9, 19.2 and 21.7, 22.6
+    int8_planes_over_rows = 32
+
     @staticmethod
     @functools.lru_cache(maxsize=4096)
     def _int8_workspace(m: int, n: int, k: int, width: int) -> int:
         return core_library().qrt_int8_workspace(m, n, k, width)
 
-    def _int8_product(self, x, w, out_f32=False, gate=None):
+    def _int8_product(self, x, w, out_f32=False, gate=None, planes=False):
         """The product of rows by an ``Int8Weight``; ``gate`` = (activation, limit): gate rows, then up rows, and the activation of the two.
         Up to 48 rows (64 by few outputs) go past the weight as it streams, more by tiles; up to four by few outputs are quantised by
-        the kernel that multiplies them, ``CodedRows`` are codes already."""
+        the kernel that multiplies them, ``CodedRows`` are codes already. ``planes``: the result may come as planes along K."""
         if isinstance(x, ScaledRows):
             x = x.made()
         values, (n, k), width = w.values, w.shape, w.width
@@ -1748,18 +1755,25 @@ class HipOps:
             if act > ACTIVATIONS["clamped"] or n % 2:
                 raise OpsError(f"gated_linear: {gate[0]} of a weight {tuple(w.shape)}")
             n, form = n // 2, "gated"
-        lib, code = self.lib, F32 if out_f32 else _CODE[dtype]
-        out = x.new_empty((m, n), dtype=torch.float32 if out_f32 else dtype)
+        lib, code, parts = self.lib, F32 if out_f32 else _CODE[dtype], 1
+        if planes and m > self.int8_planes_over_rows:
+            tile, parts = self.choose_tile(m, n, width // 2, "planes")
+        out = x.new_empty((m, n) if parts == 1 else (parts, m, n), dtype=torch.float32 if out_f32 else dtype)
         if m == 0:
             return out
         if x.data_ptr() % 16:
             x = x.clone()
-        room = 0 if coded is not None else self._int8_workspace(m, n, k, width)
+        room = 0 if coded is not None else self._int8_workspace(m, n, k, width) if parts == 1 else m * width + 4 * m + 16
         work = x.new_empty(room, dtype=torch.uint8) if room else None
         # 128 columns of bytes are a stage, as 64 of bfloat16 are: the same bytes and the same cycles of the matrix cores
-        tile = self.choose_tile(m, n, width // 2, form)[0] if m > 48 else 0
-        if lib.qrt_int8_product(x.data_ptr(), _CODE[dtype], None if coded is None else coded.data_ptr(), values.data_ptr(), w.scale.data_ptr(), out.data_ptr(),
-                                code, None if work is None else work.data_ptr(), m, n, k, width, tile, act, limit, _stream()):
+        scales, room = None if coded is None else coded.data_ptr(), None if work is None else work.data_ptr()
+        if parts > 1:
+            failed = lib.qrt_int8_planes(x.data_ptr(), _CODE[dtype], scales, values.data_ptr(), w.scale.data_ptr(), out.data_ptr(), room, m, n, k, width, tile, parts, _stream())
+        else:
+            tile = self.choose_tile(m, n, width // 2, form)[0] if m > 48 else 0
+            failed = lib.qrt_int8_product(x.data_ptr(), _CODE[dtype], scales, values.data_ptr(), w.scale.data_ptr(), out.data_ptr(), code, room, m, n, k, width, tile,
+                                          act, limit, _stream())
+        if failed:
             raise OpsError(lib.qrt_last_error().decode())
         return out
 

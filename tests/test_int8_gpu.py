@@ -147,6 +147,32 @@ def test_a_norms_codes_and_their_products(m, h, n, planes, dtype):
 
 
 @gpu
+@pytest.mark.parametrize("coded", [False, True])
+@pytest.mark.parametrize("m,n,k", [(33, 304, 1280), (48, 301, 2560), (70, 1024, 9728), (130, 96, 4100), (600, 256, 2300)])
+def test_products_for_the_residual_in_planes(m, n, k, coded):
+    """The planes' whole sums meet in float32: each is rounded three times, and their sum once more a plane, all relative to the magnitudes of the planes."""
+    from qwen3_runtime_amd.ops.hip import CodedRows, HipOps
+
+    o = HipOps(residual_planes=True)
+    x, w = rnd(m, k, seed=m, dtype=torch.bfloat16), Int8Weight.quantize(rnd(n, k, seed=n))
+    got = o.linear_for_residual(CodedRows(*o.quantize_rows(x), x.shape, x.dtype) if coded else x, w)
+    assert (got.dim() == 3) == (k >= 2048) and got.dtype == torch.float32  # a plane has eight stages of 128 columns or more
+    got = got.view(-1, m, n)
+    parts = got.shape[0]
+    want = product(x, w)
+    assert bool(((got.double().sum(0) - want).abs() <= STEP[torch.float32] * got.double().abs().sum(0)).all())
+    # the norm behind adds them up, one after the other or their sum: as many roundings as there are planes either way
+    if n % 4 == 0:
+        ours, again = rnd(m, n, seed=5), rnd(m, n, seed=5)
+        o.add_rmsnorm_codes(ours, got, rnd(n, seed=6), 1e-6, torch.bfloat16)
+        o.add_rmsnorm(again, got, rnd(n, seed=6), 1e-6, torch.bfloat16)
+        assert torch.allclose(ours, again, rtol=0, atol=2 * parts * 2.0 ** -24 * float((got.abs().sum(0) + rnd(m, n, seed=5).abs()).max()))
+    # few rows, and a caller that takes no planes, get the whole
+    assert o.linear_for_residual(x[:32].contiguous(), w).shape == (32, n)
+    assert ops().linear_for_residual(x, w).shape == (m, n)
+
+
+@gpu
 @pytest.mark.parametrize("m", [3, 20, 100])
 @pytest.mark.parametrize("bad", [float("nan"), float("inf"), float("-inf")])
 def test_rows_that_are_not_finite_are_nan_and_leave_the_others(m, bad):
@@ -267,6 +293,19 @@ def test_a_weight_that_is_not_finite_is_refused():
         Int8Weight.quantize(w)
     with pytest.raises(ValueError):
         Int8Weight.quantize(torch.ones(3, 4, dtype=torch.int32))
+
+
+def test_planes_refuse_on_the_host():
+    from ctypes import c_void_p
+
+    from qwen3_runtime_amd.ops.hip import HipOps
+
+    lib, p = HipOps().lib, c_void_p(1 << 20)  # not read: the sizes are refused
+    planes = lambda m, n, k, width, tile=12, parts=2, x=p, work=p: lib.qrt_int8_planes(x, 1, p, p, p, p, work, m, n, k, width, tile, parts, None)  # noqa: E731
+    for bad in (dict(parts=1), dict(parts=0), dict(parts=-2), dict(parts=65), dict(parts=5), dict(parts=3), dict(tile=14), dict(x=c_void_p(8))):
+        assert planes(40, 64, 512, 512, **bad) != 0, bad
+    for bad in ((40, 0, 512, 512), (40, 64, 512, 500), (-1, 64, 512, 512)):
+        assert planes(*bad) != 0, bad
 
 
 def test_entry_points_refuse_sizes_on_the_host():
