@@ -16,14 +16,14 @@
 // make many blocks of few rows, which fills the chip and evens out what a causal mask leaves; few groups meet less often. us with 4, 2 and
 // 1 groups, 32 heads on 8 of 128, a prompt read at once: 300 tokens (304 blocks of 4 groups) 11.5, 12.1, 15.3; 512 (512) 12.8, 14.7, 21.3;
 // 700 (704) 22.2, 19.4, 27.4; 2,048 (2,048) 67.7, 59.0, 70.3; two of 2,048 (4,096) 140, 119, 115.
-// RT = 2 takes the codes out of their words half as often a row: from some 400 blocks on, as many as the chip holds, that is what counts (400 tokens
+// RT = 2 takes the codes out of their words half as often a row: from 384 blocks on, nearly as many as the chip holds, that is what counts (400 tokens
 // of 4,096 49.6 and 60.1 us), before that the blocks are (128 tokens 8.7 and 5.9). A launch may cut the keys into pieces of one length as well,
 // which a second kernel joins. Sums, maxima and outputs are float32.
 //
 // What bounds it: many rows, the vector instructions: some 240 a block of 32 keys and 32 rows beside 34 of the matrix cores, issued in 60 % of the
 // cycles at 2,048 tokens (0.58 PFLOP/s). Taken out on the way there: a branch an element that the compiler had made of one condition
 // (93 us -> 71), and arguments held in scalar registers, which it kept in a vector register's lanes (71 -> 64). One row a head over 32,000 tokens: 34.8 MB in
-// 12.8 us, 2.7 TB/s, four blocks of keys a wave between a start and a meeting that take most of it, and a merge of 4 us.
+// some 11 us, 3.2 TB/s, eight blocks of keys a wave between a start of three trips to memory and a meeting, and a merge of 3.5 us.
 #include "common.h"
 #include "cache4.h"
 

@@ -216,8 +216,10 @@ class DecodeGraph:
                 # the bucket's length, not the batch's, now fixes every launch shape (key splits too);
                 # where the lengths are very unequal the attention kernel is told them as they are
                 # now, to choose the length of its pieces by
+                lens = [runner.cache.length(e.request_id) + 1 for e in entries]
+                self.ctx.scratch["lens_at_capture"] = lens
                 if self.unequal:
-                    self.ctx.scratch["attn_lens"] = [runner.cache.length(e.request_id) + 1 for e in entries]
+                    self.ctx.scratch["attn_lens"] = lens
                 self.cache_views, self.embedding_views = runner._cache_views(self.ctx.groups)
             dev = self.views_dev
             runner.last_row_slots = dev["row_slots"]

@@ -2242,12 +2242,14 @@ class HipOps:
         if tokens is not None:
             a.merge_tokens, a.num_merge_tokens = tokens.data_ptr(), tokens.numel()
         # a captured step is launched for its bucket's lengths, and told the lengths of its moment beside
-        lens = (ctx.scratch.get("attn_lens") if subset is None else None) or kv_lens
+        # (which grow from step to step, so somewhat longer ones are counted on)
+        lens = ctx.scratch.get("lens_at_capture") if subset is None else None
+        lens = [min(n + n // 8 + 32, top) for n, top in zip(lens, kv_lens)] if lens else kv_lens
         most_q = max(q_lens)
         most = self.attention4_blocks(max(kv_lens), most_q, window, chunk, keep_first)
-        total = sum(self.attention4_blocks(n, most_q, window, chunk, keep_first) for n in lens)
+        blocks = [self.attention4_blocks(n, most_q, window, chunk, keep_first) for n in lens]
         splits = ctx.scratch.get("attn_splits")
-        a.piece = max(-(-most // splits), -(-most // 1024)) if splits else self.choose_attention4_piece(most, total, n_tiles, nkv, keys)
+        a.piece = max(-(-most // splits), -(-most // 1024)) if splits else self.choose_attention4_piece(most, blocks, n_tiles, nkv, keys)
         a.pieces = -(-most // a.piece)
         return bytes(a), groups, row_tiles, ctx.num_tokens * nq * a.pieces if a.pieces > 1 else 0, (tiles, tokens)
 
@@ -2271,13 +2273,19 @@ class HipOps:
         return row_tiles, groups
 
     @staticmethod
-    def choose_attention4_piece(most: int, total: int, tiles: int, nkv: int, keys: bool) -> int:
-        """Blocks of 32 keys that one block of the launch walks."""
-        if keys:  # about 512 blocks of the launch, four waves of each with two blocks of keys or more, 64 pieces at most
-            return max(8, -(-total * nkv // 512), -(-most // 64))
+    def choose_attention4_piece(most: int, blocks, tiles: int, nkv: int, keys: bool) -> int:
+        """Blocks of 32 keys that one block of the launch walks, of sequences that have ``blocks`` and in time up to ``most``."""
+        launch = tiles * nkv
+        if keys:
+            # us in one piece, in 256 blocks of the launch and in 512, 32 heads on 8 of 128: 512 tokens 7.0, -, 8.3; 8 x 512 7.1, -, 8.5; 24 x 1,000 11.2, 13.8, 14.1; 32 x 2,048 17.2, -, 19.7;
+            # 700 8.3, -, 8.5; 8 x 2,048 16.1, 11.0, 11.8; 16,000 -, 11.9, 13.9; 32,000 -, 14.6, 15.9; 16 x 4,000 27.8, 19.6, 18.8; 32 of 500 to 6,000 -, 32.6,
+            # 23.6: a piece costs its part of a merge, and a block that walks more than some 32 blocks of keys ends late, but where all do:
+            # 48 x 3,000 34.5 in one and 37.0 in two pieces
+            now, each = max(blocks), sum(blocks) * nkv
+            piece = max(8, min(-(-each // 256), max(32, -(-each // 512))), -(-most // 32))
+            return max(1, most) if now <= max(20, min(launch // 4, 64), piece + piece // 2) else piece
         # one piece from 192 blocks on, 256 blocks below: us in 1, 2 and 4 pieces 256 blocks (128 tokens of 4,096) 25.7, 30.0, 31.9; 128 (eight
         # times 8 of up to 3,000) 21.2, 18.8, 18.1; 16 (8 of 8,000) in 8, 16 and 32 13.1, 11.4, 13.2
-        launch = tiles * nkv
         return most if launch >= 192 else max(16, -(-most // -(-256 // launch)))
 
     resident_blocks = 512  # blocks of the prompt kernels the chip holds at once: 2 on each of 256 CUs

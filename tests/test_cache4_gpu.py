@@ -301,6 +301,20 @@ def test_steps_that_take_each_split_by_their_sizes(seqs, nkv, form):
     near(ops().paged_attention(q, cache, ctx, 2 * nkv, nkv, 32, 32 ** -0.5, None), plain(q, cache, ctx, 2 * nkv, nkv, 32, 32 ** -0.5), cache)
 
 
+def test_how_keys_are_cut():
+    """Pieces hold every block of the longest sequence, and are no more than the merge has room for."""
+    from qwen3_runtime_amd.ops.hip import HipOps
+
+    choose = HipOps.choose_attention4_piece
+    for blocks in ([1], [20], [21], [64] * 8, [500] * 16, [1, 2, 3000], [40] * 300, [100000]):
+        for most in (max(blocks), 2 * max(blocks)):
+            for keys in (True, False):
+                piece = choose(most, blocks, len(blocks), 8, keys)
+                assert piece >= 1 and -(-most // piece) <= 1024
+    assert choose(16, [16], 1, 8, True) == 16 and choose(128, [76] * 64, 64, 8, True) == 128  # one piece: no merge
+    assert choose(1000, [1000], 1, 8, True) == 32 and choose(128, [66] * 8, 8, 8, True) < 32
+
+
 def test_how_rows_are_split():
     from qwen3_runtime_amd.ops.hip import HipOps
 
