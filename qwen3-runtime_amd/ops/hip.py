@@ -2197,11 +2197,10 @@ class HipOps:
         out = q.new_empty((ctx.num_tokens, nq * d))
         lib, code, stream = attention4_library(d), _CODE[q.dtype], _stream()
         for fixed, groups, row_tiles, room, _tensors in plan:
-            parts = 0
-            if room:
-                parts = q.new_empty((room * (d + 2),), dtype=torch.float32).data_ptr()
+            # held until the launches are made: the call leaves the interpreter to other threads
+            parts = q.new_empty((room * (d + 2),), dtype=torch.float32) if room else None
             if lib.qrt_attention4(fixed, q.data_ptr(), out.data_ptr(), cache.k.data_ptr(), cache.v.data_ptr(), cache.pages["steps"].data_ptr(), cu_q.data_ptr(),
-                                  kv_lens.data_ptr(), table.data_ptr(), parts, 4 * room * d, table.shape[1], pages, group.page_size, sink, scale, softcap, code,
+                                  kv_lens.data_ptr(), table.data_ptr(), 0 if parts is None else parts.data_ptr(), 4 * room * d, table.shape[1], pages, group.page_size, sink, scale, softcap, code,
                                   groups, row_tiles, stream):
                 raise OpsError(lib.qrt_last_error().decode())
         return out

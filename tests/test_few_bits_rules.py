@@ -1,0 +1,77 @@
+"""What products and caches in few bits promise around their kernels: workspaces, launches that follow from a step's lengths alone, what
+is held. Needs no GPU but where marked."""
+
+import weakref
+
+import pytest
+import torch
+
+GPU = pytest.mark.gpu
+
+
+def host_step(q_lens, kv_lens, nq, nkv, d, page=16):
+    """Queries, a cache of 4 bits and a step's context on the host, as the attention's launches are made from them."""
+    from qwen3_runtime_amd.parts.base import CacheView, GroupView, StepContext
+    from qwen3_runtime_amd.parts.plan import CacheSpec
+
+    i32 = lambda x: torch.tensor(x, dtype=torch.int32)  # noqa: E731
+    pages = sum(-(-n // page) for n in kv_lens)
+    width = max(-(-n // page) for n in kv_lens)
+    group = GroupView(page, None, torch.zeros(len(kv_lens), width, dtype=torch.int32), i32([0] * sum(q_lens)))
+    t = {"k": torch.zeros(pages, nkv, page, d // 2, dtype=torch.uint8), "v": torch.zeros(pages, nkv, page, d // 2, dtype=torch.uint8),
+         "steps": torch.zeros(pages, nkv, page, 4, dtype=torch.bfloat16)}
+    cache = CacheView(CacheSpec("paged_kv", heads=nkv, head_dim=d, bits=4), group=group, k=t["k"], v=t["v"], pages=t)
+    cu = [0]
+    for n in q_lens:
+        cu.append(cu[-1] + n)
+    ctx = StepContext(ops=None, dtype=torch.bfloat16, device=torch.device("cpu"), num_tokens=cu[-1], num_seqs=len(q_lens),
+                      positions=i32([n - q + i for q, n in zip(q_lens, kv_lens) for i in range(q)]), cu_q=i32(cu), kv_lens=i32(kv_lens),
+                      seq_of_token=i32([s for s, q in enumerate(q_lens) for _ in range(q)]), state_slots=i32([0] * len(q_lens)),
+                      first_span=i32([0] * len(q_lens)), q_lens_host=list(q_lens), kv_lens_host=list(kv_lens), max_q_len=max(q_lens),
+                      max_kv_len=max(kv_lens), groups=[group])
+    return torch.zeros(cu[-1], nq * d, dtype=torch.bfloat16), cache, ctx
+
+
+class StubLibrary:
+    """An attention library that notes what it is called with, and whether the tensor behind the parts' room is there."""
+
+    def __init__(self, made):
+        self.made, self.calls = made, []
+
+    def qrt_attention4(self, *args):
+        parts = args[9]
+        held = [ref() for ref in self.made]
+        self.calls.append((args, not parts or any(t is not None and t.data_ptr() == parts for t in held)))
+        return 0
+
+
+@pytest.fixture
+def stub(monkeypatch):
+    from qwen3_runtime_amd.ops import hip
+
+    made = []
+    new_empty = torch.Tensor.new_empty
+
+    def noted(self, *args, **kwargs):
+        t = new_empty(self, *args, **kwargs)
+        made.append(weakref.ref(t))
+        return t
+
+    lib = StubLibrary(made)
+    monkeypatch.setattr(torch.Tensor, "new_empty", noted)
+    monkeypatch.setattr(hip, "attention4_library", lambda d: lib)
+    monkeypatch.setattr(hip, "_stream", lambda: 0)
+    monkeypatch.setattr(hip, "_need", lambda t, *a, **k: t)
+    monkeypatch.setattr(hip.HipOps, "_check_cache4", staticmethod(lambda cache, nkv, d: cache.k.shape[0]))
+    return lib
+
+
+@pytest.mark.parametrize("q_lens,kv_lens", [([1], [4000]), ([40, 1], [60, 4000]), ([24], [9000])])
+def test_the_room_for_parts_lives_until_the_launches_are_made(stub, q_lens, kv_lens):
+    """Freed before, it could be another thread's on the same stream, or gone, when the kernels write it."""
+    from qwen3_runtime_amd.ops.hip import HipOps
+
+    q, cache, ctx = host_step(q_lens, kv_lens, 8, 2, 64)
+    HipOps()._attention4(q, cache, ctx, 8, 2, 64, 0.125, 0, 0, 0.0, 0, False)
+    assert any(args[9] for args, _ in stub.calls)  # some launch of each of these steps takes its keys in pieces
+    assert all(held for _, held in stub.calls)
