@@ -89,6 +89,8 @@ class WeightLoader:
         self.dtype = dtype
         self._cache: dict[tuple, torch.Tensor] = {}
         self._int8: dict[tuple, Int8Weight] = {}
+        self._asked: list[tuple] = []           # what the part that is being loaded has asked for
+        self._askers: dict[tuple, int] = {}     # how many parts have, and may hold it
         self.num_bytes = 0
 
     def _placed_dtype(self, stored: torch.dtype) -> torch.dtype:
@@ -99,6 +101,7 @@ class WeightLoader:
         return torch.bfloat16
 
     def _remember(self, key, make):
+        self._asked.append(key)
         if key not in self._cache:
             t = make().contiguous()
             self._cache[key] = t
@@ -137,12 +140,15 @@ class WeightLoader:
         """A tensor the part computed itself (a table of constants): placed as it is."""
         return tensor.to(self.device).contiguous()
 
-
     def quantize(self, part) -> None:
-        """The matrices that ``part`` has just loaded in 8 bits in their place, one after the other (``Part.int8_products``)."""
+        """The matrices that ``part`` has just loaded in 8 bits in their place, one after the other (``Part.int8_products``). Floats that
+        no part holds any more are dropped, also those that the part has made its matrices of."""
+        asked, self._asked = list(dict.fromkeys(self._asked)), []
+        for key in asked:
+            self._askers[key] = self._askers.get(key, 0) + 1
         for name in part.int8_products:
             w = getattr(part, name)
-            key = next((k for k, t in self._cache.items() if t is w), None)
+            key = next((k for k in asked if self._cache[k] is w), None)
             made = self._int8.get(key)
             if made is None:
                 try:
@@ -150,11 +156,19 @@ class WeightLoader:
                 except ValueError as exc:
                     raise ValueError(f"{name} of {sorted(part.tensor_names.values())}: {exc}") from None
                 self.num_bytes += made.num_bytes
-            if key is not None:  # a part that asks for the same matrix shares its 8-bit form; the floats are not held beside it
+            if key is not None:  # a part that asks for the same matrix shares its 8-bit form
                 self._int8[key] = made
-                del self._cache[key]
-                self.num_bytes -= w.numel() * w.element_size()
             setattr(part, name, made)
+        if part.int8_products:
+            held = {t.untyped_storage().data_ptr() for t in vars(part).values() if isinstance(t, torch.Tensor)}
+            for key in asked:
+                t = self._cache[key]
+                if key[0] not in ("matrix", "fused") or t.untyped_storage().data_ptr() in held:
+                    continue
+                self._askers[key] -= 1
+                if not self._askers[key]:
+                    del self._cache[key]
+                    self.num_bytes -= t.numel() * t.element_size()
         part.weights_in_int8 = bool(part.int8_products)
 
 

@@ -75,3 +75,77 @@ def test_the_room_for_parts_lives_until_the_launches_are_made(stub, q_lens, kv_l
     HipOps()._attention4(q, cache, ctx, 8, 2, 64, 0.125, 0, 0, 0.0, 0, False)
     assert any(args[9] for args, _ in stub.calls)  # some launch of each of these steps takes its keys in pieces
     assert all(held for _, held in stub.calls)
+
+
+# ---- what a loader holds
+
+
+class Table:
+    """A source of random tensors for a model's declarations."""
+
+    def __init__(self, model, seed=0):
+        self.t = {}
+        for i, d in enumerate(model.tensor_decls()):
+            g = torch.Generator().manual_seed(seed + i)
+            self.t[d.file_name] = (torch.randint(0, 4, d.shape, generator=g, dtype=torch.int32) if d.storage == "int" else
+                                   torch.randn(d.shape, generator=g).to(torch.bfloat16))
+
+    def names(self):
+        return list(self.t)
+
+    def has(self, name):
+        return name in self.t
+
+    def shape(self, name):
+        return tuple(self.t[name].shape)
+
+    def dtype(self, name):
+        return self.t[name].dtype
+
+    def get(self, name, device):
+        return self.t[name].to(device)
+
+
+@pytest.mark.parametrize("name", ["dekinex_tiny_a", "dekinex_tiny_b", "tiny_b", "deginex_tiny_a", "sarudra_tiny_b"])
+def test_no_floats_stay_beside_their_8_bits(name):
+    """Also where a part makes its matrix of what it loads: queries and keys that turn in pairs of neighbours have their rows in another order."""
+    from qwen3_runtime_amd.engine.factory import build_model
+    from qwen3_runtime_amd.registry import preset_config
+    from qwen3_runtime_amd.weights import load_model
+
+    whole, model = build_model(preset_config(name))[1], build_model(preset_config(name))[1]
+    source = Table(whole)
+    floats = load_model(whole, source, "cpu", torch.bfloat16)
+    loader = load_model(model, source, "cpu", torch.bfloat16, weights="int8")
+    # what the parts with matrices in 8 bits ask for in floats is not held, and what they hold is counted in its place
+    parts = [p for p in model.parts() if p.int8_products]
+    matrices = {d.file_name: 2 * d.shape[0] * d.shape[1] for p in parts for d in p.tensor_decls() if d.init == "matrix" and len(d.shape) == 2}
+    left = [key for key in loader._cache if key[0] in ("matrix", "fused") and matrices.keys() & {key[1]} | matrices.keys() & set(key[1])]
+    assert parts and not left
+    coded = sum(getattr(p, n).num_bytes for p in parts for n in p.int8_products)
+    assert loader.num_bytes == floats.num_bytes - sum(matrices.values()) + coded
+
+
+def test_a_matrix_that_another_part_holds_as_floats_stays():
+    from qwen3_runtime_amd.ops import Int8Weight
+    from qwen3_runtime_amd.weights.loader import WeightLoader
+
+    class Holder:
+        def __init__(self, *names):
+            self.int8_products, self.tensor_names = names, {"w": "w"}
+
+        def load(self, fetch):
+            self.w = fetch.matrix("w")
+
+    class Source:
+        def get(self, name, device):
+            return torch.ones(4, 128, dtype=torch.bfloat16)
+
+    for order in ((Holder(), Holder("w"), Holder("w")), (Holder("w"), Holder("w"), Holder())):
+        loader = WeightLoader(Source(), "cpu", torch.bfloat16)
+        for part in order:
+            part.load(loader)
+            loader.quantize(part)
+        coded = [p.w for p in order if p.int8_products]
+        assert all(isinstance(w, Int8Weight) for w in coded) and coded[0] is coded[1]
+        assert loader.num_bytes == 4 * 128 * 2 + coded[0].num_bytes
