@@ -1,7 +1,8 @@
 """Pure-decode steps replayed from captured HIP graphs.
 
 A graph is captured per (batch size, bucket of the longest context, whether the
-contexts are of very unequal lengths: the attention kernel then cuts them another way). Its
+contexts are of very unequal lengths: the attention kernel then cuts them another way; where
+keys and values are held in 4 bits also whether the longest is in the bucket's last quarter). Its
 kernels read the step's arrays (token ids, positions, lengths, block tables,
 slots) from one static device buffer; a replay fills that buffer with one copy
 and launches the whole step at once, which removes the per-kernel launch cost
@@ -28,17 +29,30 @@ MIN_BUCKET = 512
 
 class DecodeGraph:
     @staticmethod
-    def key_for(batch: int, max_kv: int, all_want: bool, unequal: bool = False):
+    def key_for(batch: int, max_kv: int, all_want: bool, unequal: bool = False, by_quarter: bool = False):
+        """``by_quarter``: the third and the last quarter of a bucket apart (no context of a larger one is in the first two)."""
         if not all_want:
             return None
         bucket = MIN_BUCKET
         while bucket < max_kv:
             bucket *= 2
-        return (batch, bucket, bool(unequal))
+        return (batch, bucket, bool(unequal), by_quarter and bucket > MIN_BUCKET and max_kv > bucket * 3 // 4)
+
+    @staticmethod
+    def typical_lens(key) -> list[int]:
+        """What the contexts of a graph's steps are taken to be where the length of a launch's pieces is chosen: by its key alone, so
+        that a step is computed alike whatever came before it. The longest in the middle of its quarter, the others as it or,
+        of very unequal lengths, half of it."""
+        batch, bucket, unequal, last = key
+        longest = bucket if bucket == MIN_BUCKET else bucket * (7 if last else 5) // 8
+        return [longest] + [longest // 2 if unequal else longest] * (batch - 1)
 
     def __init__(self, runner, key):
         self.runner = runner
-        self.batch, self.bucket, self.unequal = key
+        self.key = key
+        self.batch, self.bucket, self.unequal, last = key
+        # no step beyond this length is prepared in this graph's buffer: its key would be another
+        self.longest = self.bucket * 3 // 4 if runner.graphs_by_quarter and not last and self.bucket > MIN_BUCKET else self.bucket
         cache = runner.cache
         self.width = max(1, -(-self.bucket // cache.page_size))
         self.graph: torch.cuda.CUDAGraph | None = None
@@ -152,7 +166,7 @@ class DecodeGraph:
         starts = [cache.length(r) for r in rids]
         if any(a != b + 1 for a, b in zip(starts, self._last_starts)):
             return
-        if max(starts) + 1 > min(self.bucket, self.runner.max_model_len):
+        if max(starts) + 1 > min(self.longest, self.runner.max_model_len):
             return
         try:
             for r in rids:
@@ -216,10 +230,9 @@ class DecodeGraph:
                 # the bucket's length, not the batch's, now fixes every launch shape (key splits too);
                 # where the lengths are very unequal the attention kernel is told them as they are
                 # now, to choose the length of its pieces by
-                lens = [runner.cache.length(e.request_id) + 1 for e in entries]
-                self.ctx.scratch["lens_at_capture"] = lens
+                self.ctx.scratch["typical_lens"] = self.typical_lens(self.key)
                 if self.unequal:
-                    self.ctx.scratch["attn_lens"] = lens
+                    self.ctx.scratch["attn_lens"] = [runner.cache.length(e.request_id) + 1 for e in entries]
                 self.cache_views, self.embedding_views = runner._cache_views(self.ctx.groups)
             dev = self.views_dev
             runner.last_row_slots = dev["row_slots"]

@@ -40,6 +40,8 @@ class ModelRunner:
         self.hip_graph = bool(hip_graph) and self.device.type == "cuda" and model.graph_capturable
         self._graphs: dict[tuple, "_DecodeGraph"] = {}
         self._graph_pool = None
+        # attention over a cache of 4 bits cuts its keys by the lengths more finely than buckets are
+        self.graphs_by_quarter = any(spec.bits == 4 for spec in model.plan.caches)
         # device copy of the last step's "row_slots" (state slot of each row of the logits)
         self.last_row_slots: torch.Tensor | None = None
         self._pinned: torch.Tensor | None = None
@@ -177,7 +179,7 @@ class ModelRunner:
         # contexts of very unequal lengths: the ops may cut them another way, which a capture freezes
         unequal = getattr(self.ops, "decode_in_pieces", None)
         key = DecodeGraph.key_for(len(entries), max_kv, all(len(e.want) == 1 for e in entries),
-                                  unequal is not None and unequal(lens))
+                                  unequal is not None and unequal(lens), self.graphs_by_quarter)
         if key is None:
             packed = pack_step(entries, self.cache, self.vocab_size)
             dev = self._upload(packed)

@@ -2240,10 +2240,9 @@ class HipOps:
         a.window, a.chunk, a.keep_first = window, chunk, keep_first
         if tokens is not None:
             a.merge_tokens, a.num_merge_tokens = tokens.data_ptr(), tokens.numel()
-        # a captured step is launched for its bucket's lengths, and told the lengths of its moment beside
-        # (which grow from step to step, so somewhat longer ones are counted on)
-        lens = ctx.scratch.get("lens_at_capture") if subset is None else None
-        lens = [min(n + n // 8 + 32, top) for n, top in zip(lens, kv_lens)] if lens else kv_lens
+        # a captured step is launched for its bucket's lengths, and told beside what its sequences' are about
+        lens = ctx.scratch.get("typical_lens") if subset is None else None
+        lens = [min(n, top) for n, top in zip(lens, kv_lens)] if lens else kv_lens
         most_q = max(q_lens)
         most = self.attention4_blocks(max(kv_lens), most_q, window, chunk, keep_first)
         blocks = [self.attention4_blocks(n, most_q, window, chunk, keep_first) for n in lens]

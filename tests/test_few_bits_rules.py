@@ -149,3 +149,49 @@ def test_a_matrix_that_another_part_holds_as_floats_stays():
         coded = [p.w for p in order if p.int8_products]
         assert all(isinstance(w, Int8Weight) for w in coded) and coded[0] is coded[1]
         assert loader.num_bytes == 4 * 128 * 2 + coded[0].num_bytes
+
+
+# ---- launches of captured steps
+
+
+def test_a_graphs_pieces_follow_from_its_key():
+    """Whatever lengths a graph has met first: the key is all that its launches are shaped by, and lengths of one key are no more than 1.5 apart."""
+    from qwen3_runtime_amd.engine.graph import DecodeGraph
+    from qwen3_runtime_amd.ops.hip import HipOps
+
+    for batch in (1, 2, 8, 64):
+        for unequal in (False, True):
+            for max_kv in (1, 400, 512, 513, 768, 769, 1024, 2049, 3072, 3073, 4096, 30000):
+                key = DecodeGraph.key_for(batch, max_kv, True, unequal, True)
+                typical = DecodeGraph.typical_lens(key)
+                assert len(typical) == batch and key[1] >= max_kv and max(typical) <= key[1]
+                if key[1] > 512:
+                    assert DecodeGraph.key_for(batch, max(typical), True, unequal, True) == key
+                    assert 0.75 <= max(typical) / max_kv <= 1.25
+                # as many pieces as the same lengths get uncaptured, in a launch that has room for the bucket's
+                bucket, blocks = key[1] // 32, [-(-n // 32) for n in typical]
+                piece = HipOps.choose_attention4_piece(bucket, blocks, batch, 8, True)
+                assert 1 <= piece <= bucket and -(-bucket // piece) <= 1024
+    # without a cache of 4 bits, and up to 512 keys, there is one key a bucket
+    assert DecodeGraph.key_for(4, 1000, True) == DecodeGraph.key_for(4, 600, True)
+    assert DecodeGraph.key_for(4, 512, True, by_quarter=True) == DecodeGraph.key_for(4, 1, True, by_quarter=True)
+    assert DecodeGraph.key_for(4, 800, False) is None
+
+
+@GPU
+@pytest.mark.parametrize("before,length", [(520, 900), (900, 520), (530, 740)])
+def test_a_step_is_the_same_whatever_its_engine_has_served(model_folders, before, length):
+    """Requests of other lengths of the same bucket come first, in one engine and not in the other: the same bits."""
+    import traces
+    from test_few_bits_engine import loaded
+
+    def tail(rid, n, seed):
+        toks = traces.make_requests(384, [n], seed=seed)
+        return traces.tail_one_by_one({rid: next(iter(toks.values()))}, tail=4)
+
+    def run(*steps):
+        return traces.replay(loaded(model_folders["tiny_b"], 8, 256, "bfloat16", "cuda:0", cache_bits=4, hip_graph=True), traces._number([s for x in steps for s in x]))
+
+    alone, after = run(tail("b", length, 2)), run(tail("a", before, 1), tail("b", length, 2))
+    for key, want in alone.items():
+        assert (want == after[key]).all(), key
