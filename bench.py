@@ -123,7 +123,9 @@ def main() -> int:
     ap.add_argument("--context", type=int, default=None, help="default 8192 (capacity: 32768)")
     ap.add_argument("--layers", type=int, default=None, help="run fewer layers than the configuration has")
     ap.add_argument("--dtype", default="bfloat16", choices=["bfloat16", "float32"])
-    ap.add_argument("--weights", default="model", choices=["model", "int8"], help="int8: projections and dense feed-forwards in 8 bits")
+    ap.add_argument("--weights", default="model", choices=["model", "int8"],
+                    help="int8: attention's projections and dense feed-forwards in 8 bits; experts (shared ones too), "
+                         "latent and state layers, embeddings and heads stay as they are")
     ap.add_argument("--cache-bits", type=int, default=None, choices=[4], help="4: keys and values are cached in 4 bits")
     ap.add_argument("--no-graph", action="store_true")
     ap.add_argument("--no-points", action="store_true", help="skip batch 1 / 64 and the prefill measurement")

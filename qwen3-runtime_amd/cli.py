@@ -30,7 +30,9 @@ def main(argv=None) -> int:
     ap.add_argument("--cuda-graph", action=argparse.BooleanOptionalAction, default=None,
                     help="replay decode steps from captured (HIP) graphs; default on")
     ap.add_argument("--dtype", default="bfloat16", choices=["bfloat16", "float32"])
-    ap.add_argument("--weights", default="model", choices=["model", "int8"], help="int8: projections and dense feed-forwards in 8 bits")
+    ap.add_argument("--weights", default="model", choices=["model", "int8"],
+                    help="int8: attention's projections and dense feed-forwards in 8 bits; experts (shared ones too), "
+                         "latent and state layers, embeddings and heads stay as they are")
     ap.add_argument("--cache-bits", type=int, default=None, choices=[4], help="4: keys and values are cached in 4 bits")
     ap.add_argument("--temperature", type=float, default=0.0)
     ap.add_argument("--top-k", type=int, default=0)

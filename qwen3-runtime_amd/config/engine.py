@@ -30,8 +30,9 @@ class EngineConfig:
     memory_fraction: float = 0.85
     # replay pure-decode steps from captured HIP graphs
     hip_graph: bool = True
-    # "int8": the projections and dense feed-forwards hold their matrices in 8 bits, a scale for every output channel, and
-    # multiply them by activations quantised token by token
+    # "int8": attention over keys and values and dense feed-forwards hold their matrices in 8 bits, a scale for every output
+    # channel, and multiply them by activations quantised token by token. Experts (shared ones too), latent and state layers,
+    # embeddings and heads stay as they are; a model with neither of the first two is an error
     weights: str = "model"
     # 4: keys and values are cached in 4 bits, between a lowest value and a step for every token and head
     cache_bits: int | None = None

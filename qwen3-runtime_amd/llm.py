@@ -61,7 +61,8 @@ def build_engine(
     Option names follow the reference's factory (qwen3_runtime/engine/factory.py:110-186):
     ``block_size`` is the page size, ``num_kv_blocks`` the number of pages, ``cuda_graph``
     switches the replay of decode steps from captured graphs (HIP graphs here). ``weights="int8"`` holds the
-    projections and dense feed-forwards in 8 bits, ``cache_bits=4`` keys and values in 4 (``EngineConfig``).
+    projections of attention and dense feed-forwards in 8 bits, ``cache_bits=4`` keys and values in 4 (``EngineConfig``
+    says what stays as it is).
     """
     raw = source = None
     if model_dir is None:

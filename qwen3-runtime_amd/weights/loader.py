@@ -174,9 +174,12 @@ class WeightLoader:
 
 def load_model(model, source, device, dtype, where: str = "", weights: str = "model") -> WeightLoader:
     """Check ``source`` against ``model``'s declarations, then load every part. ``weights="int8"``: the matrices of parts that have a
-    form for it (attention's projections, dense feed-forwards) are held in 8 bits; embeddings, heads and everything else as they are."""
+    form for it (attention's projections, dense feed-forwards) are held in 8 bits; experts, latent and state layers, embeddings and heads
+    as they are. A model without any such part is an error."""
     if weights not in ("model", "int8"):
         raise ValueError(f"weights are held as the model has them or in 'int8', not {weights!r}")
+    if weights == "int8" and not any(part.int8_products for part in model.parts()):
+        raise ValueError("the model has no attention over keys and values and no dense feed-forward: nothing of it is held in 8 bits")
     check_source(source, model.tensor_decls(), model.plan.ignorable, where)
     loader = WeightLoader(source, device, dtype)
     if weights == "model":

@@ -126,6 +126,23 @@ def test_no_floats_stay_beside_their_8_bits(name):
     assert loader.num_bytes == floats.num_bytes - sum(matrices.values()) + coded
 
 
+def test_a_model_without_a_part_that_has_8_bits_is_refused():
+    """Layers of memory and experts alone, one of them shared."""
+    import copy
+
+    from qwen3_runtime_amd.engine.factory import build_model
+    from qwen3_runtime_amd.registry import preset_config
+    from qwen3_runtime_amd.weights import load_model
+
+    raw = copy.deepcopy(preset_config("dekinex_tiny_a"))
+    memory, attention = raw["layers"][0], raw["layers"][1]
+    raw["layers"] = [{**memory, "mlp": attention["mlp"]}]
+    del raw["loop"]
+    load_model(model := build_model(raw)[1], Table(model), "cpu", torch.bfloat16)
+    with pytest.raises(ValueError, match="no attention over keys and values and no dense feed-forward"):
+        load_model(model := build_model(raw)[1], Table(model), "cpu", torch.bfloat16, weights="int8")
+
+
 def test_a_matrix_that_another_part_holds_as_floats_stays():
     from qwen3_runtime_amd.ops import Int8Weight
     from qwen3_runtime_amd.weights.loader import WeightLoader
