@@ -2159,7 +2159,7 @@ class HipOps:
             return q.new_empty((0, nq * d))
         group = cache.group
         table, s = group.block_table, ctx.num_seqs
-        key = ("attn4", nq, nkv, d, group.page_size, window, chunk, keep_first, q.dtype, ctx.scratch.get("attn_splits"))
+        key = ("attn4", nq, nkv, d, group.page_size, window, chunk, keep_first, q.dtype, ctx.scratch.get("attn_splits"), ctx.max_kv_len)
         plan = ctx.scratch.get(key)
         if plan is None:
             if q.dtype not in _CODE:
@@ -2182,7 +2182,7 @@ class HipOps:
             raise OpsError(f"scale {scale}, cap {softcap}")
         cu_q, kv_lens = ctx.cu_q, ctx.kv_lens
         checked = ctx.scratch.get("attn4_tensors")  # the step's own tensors are looked at once
-        if checked is None or checked[0] is not table or checked[1] is not cu_q or checked[2] is not kv_lens:
+        if checked is None or checked[0] is not table or checked[1] is not cu_q or checked[2] is not kv_lens or checked[3] != ctx.max_kv_len:
             if table.dtype != torch.int32 or table.dim() != 2 or table.shape[0] != s or not table.is_contiguous():
                 raise OpsError(f"block table {tuple(table.shape)} of {table.dtype} for {s} sequences")
             if table.shape[1] * group.page_size < ctx.max_kv_len:
@@ -2191,7 +2191,7 @@ class HipOps:
             _need(kv_lens, "kv_lens", torch.int32, (s,))
             if not (table.get_device() == kv_lens.get_device() == cu_q.get_device()):
                 raise OpsError(f"a block table on {table.device}, lengths on {kv_lens.device} and {cu_q.device}")
-            ctx.scratch["attn4_tensors"] = checked = (table, cu_q, kv_lens)
+            ctx.scratch["attn4_tensors"] = checked = (table, cu_q, kv_lens, ctx.max_kv_len)
         if not q.get_device() == cache.k.get_device() == table.get_device():
             raise OpsError(f"queries on {q.device}, a cache on {cache.k.device}, its table on {table.device}")
         out = q.new_empty((ctx.num_tokens, nq * d))
@@ -2244,7 +2244,7 @@ class HipOps:
         lens = ctx.scratch.get("typical_lens") if subset is None else None
         lens = [min(n, top) for n, top in zip(lens, kv_lens)] if lens else kv_lens
         most_q = max(q_lens)
-        most = self.attention4_blocks(max(kv_lens), most_q, window, chunk, keep_first)
+        most = self.attention4_blocks(max(kv_lens) if subset is not None else max(*kv_lens, ctx.max_kv_len), most_q, window, chunk, keep_first)
         blocks = [self.attention4_blocks(n, most_q, window, chunk, keep_first) for n in lens]
         splits = ctx.scratch.get("attn_splits")
         a.piece = max(-(-most // splits), -(-most // 1024)) if splits else self.choose_attention4_piece(most, blocks, n_tiles, nkv, keys)

@@ -77,6 +77,31 @@ def test_the_room_for_parts_lives_until_the_launches_are_made(stub, q_lens, kv_l
     assert all(held for _, held in stub.calls)
 
 
+def test_a_step_whose_lengths_have_grown_is_planned_again(stub):
+    """The same context with longer contexts in it: as many keys as there are now, and a block table that has room for them."""
+    from ctypes import sizeof
+
+    from qwen3_runtime_amd.ops.hip import HipOps, OpsError, _Attn4Plan
+
+    o = HipOps()
+    q, cache, ctx = host_step([1, 1], [1500, 100], 8, 2, 64)
+    attend = lambda: o._attention4(q, cache, ctx, 8, 2, 64, 0.125, 0, 0, 0.0, 0, False)  # noqa: E731
+
+    def reach():
+        plan = _Attn4Plan.from_buffer_copy(stub.calls[-1][0][0][:sizeof(_Attn4Plan)])
+        return 32 * plan.piece * plan.pieces
+
+    ctx.kv_lens_host, ctx.max_kv_len = [90, 100], 100
+    attend()
+    first = reach()
+    ctx.kv_lens_host, ctx.max_kv_len = [1500, 100], 1500
+    attend()
+    assert 100 <= first < 1500 <= reach()
+    ctx.kv_lens_host, ctx.max_kv_len = [1500, 100], 1505  # the longest that is said to come counts
+    with pytest.raises(OpsError, match="pages wide"):
+        attend()
+
+
 # ---- what a loader holds
 
 
