@@ -2178,7 +2178,7 @@ class HipOps:
                 plan = [self._plan_attention4(q, ctx, few, True, nq, nkv, d, window, chunk, keep_first)] if any(ctx.q_lens_host[i] for i in few) else []
                 plan.append(self._plan_attention4(q, ctx, many, False, nq, nkv, d, window, chunk, keep_first))
             ctx.scratch[key] = plan
-        if not (math.isfinite(scale) and softcap >= 0):
+        if not (math.isfinite(scale) and math.isfinite(softcap) and softcap >= 0):
             raise OpsError(f"scale {scale}, cap {softcap}")
         cu_q, kv_lens = ctx.cu_q, ctx.kv_lens
         checked = ctx.scratch.get("attn4_tensors")  # the step's own tensors are looked at once

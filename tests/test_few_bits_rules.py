@@ -102,6 +102,17 @@ def test_a_step_whose_lengths_have_grown_is_planned_again(stub):
         attend()
 
 
+@pytest.mark.parametrize("scale,softcap", [(float("nan"), 0.0), (float("inf"), 0.0), (0.1, float("inf")), (0.1, float("nan")), (0.1, -1.0)])
+def test_scales_and_caps_that_make_no_numbers_are_refused(stub, scale, softcap):
+    """Scores over an infinite cap are 0, and it times their tangent NaN."""
+    from qwen3_runtime_amd.ops.hip import HipOps, OpsError
+
+    q, cache, ctx = host_step([1], [50], 4, 2, 64)
+    with pytest.raises(OpsError):
+        HipOps()._attention4(q, cache, ctx, 4, 2, 64, scale, 0, 0, softcap, 0, False)
+    assert not stub.calls
+
+
 # ---- what a loader holds
 
 
