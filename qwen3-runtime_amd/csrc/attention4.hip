@@ -38,7 +38,7 @@ struct Attention4Plan {
   const int* tile_seq;      // null: tile i is sequence i from its first row
   const int* tile_row0;     // null: from the first row
   const int* merge_tokens;  // null: all
-  int num_merge_tokens, num_tiles, num_seqs, nq, nkv;
+  int num_merge_tokens, num_tiles, nq, nkv;
   int window, chunk, keep_first;
   int piece, pieces;  // blocks of 32 keys in a piece; how many pieces the launch has room for
 };

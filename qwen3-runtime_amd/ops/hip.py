@@ -69,7 +69,7 @@ class _AttnArgs(Structure):
 class _Attn4Plan(Structure):
     _fields_ = [
         ("tile_seq", c_void_p), ("tile_row0", c_void_p), ("merge_tokens", c_void_p), ("num_merge_tokens", c_int),
-        ("num_tiles", c_int), ("num_seqs", c_int), ("nq", c_int), ("nkv", c_int), ("window", c_int), ("chunk", c_int), ("keep_first", c_int),
+        ("num_tiles", c_int), ("nq", c_int), ("nkv", c_int), ("window", c_int), ("chunk", c_int), ("keep_first", c_int),
         ("piece", c_int), ("pieces", c_int),
     ]
 
@@ -1735,8 +1735,8 @@ class HipOps:
 
     def _int8_product(self, x, w, out_f32=False, gate=None, planes=False):
         """The product of rows by an ``Int8Weight``; ``gate`` = (activation, limit): gate rows, then up rows, and the activation of the two.
-        Up to 48 rows (64 by few outputs) go past the weight as it streams, more by tiles; up to four by few outputs are quantised by
-        the kernel that multiplies them, ``CodedRows`` are codes already. ``planes``: the result may come as planes along K."""
+        Up to 48 rows (64 by few outputs) go past the weight as it streams, more by tiles; up to four by few outputs, and up to
+        eight short ones by fewer, are quantised by the kernel that multiplies them, ``CodedRows`` are codes already. ``planes``: the result may come as planes along K."""
         if isinstance(x, ScaledRows):
             x = x.made()
         values, (n, k), width = w.values, w.shape, w.width
@@ -2236,7 +2236,7 @@ class HipOps:
         a = _Attn4Plan()
         if tiles is not None:
             a.tile_seq, a.tile_row0 = tiles.data_ptr(), tiles.data_ptr() + 4 * n_tiles
-        a.num_tiles, a.num_seqs, a.nq, a.nkv, a.num_merge_tokens = n_tiles, ctx.num_seqs, nq, nkv, ctx.num_tokens
+        a.num_tiles, a.nq, a.nkv, a.num_merge_tokens = n_tiles, nq, nkv, ctx.num_tokens
         a.window, a.chunk, a.keep_first = window, chunk, keep_first
         if tokens is not None:
             a.merge_tokens, a.num_merge_tokens = tokens.data_ptr(), tokens.numel()
