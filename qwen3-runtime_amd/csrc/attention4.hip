@@ -20,10 +20,11 @@
 // of 4,096 49.6 and 60.1 us), before that the blocks are (128 tokens 8.7 and 5.9). A launch may cut the keys into pieces of one length as well,
 // which a second kernel joins. Sums, maxima and outputs are float32.
 //
-// What bounds it: many rows, the vector instructions: some 240 a block of 32 keys and 32 rows beside 34 of the matrix cores, issued in 60 % of the
+// What bounds it: many rows, the vector instructions: some 276 a block of 32 keys and 32 rows beside 34 of the matrix cores, issued in 62 % of the
 // cycles at 2,048 tokens (0.58 PFLOP/s). Taken out on the way there: a branch an element that the compiler had made of one condition
 // (93 us -> 71), and arguments held in scalar registers, which it kept in a vector register's lanes (71 -> 64). One row a head over 32,000 tokens: 34.8 MB in
-// some 11 us, 3.2 TB/s, eight blocks of keys a wave between a start of three trips to memory and a meeting, and a merge of 3.5 us.
+// some 11 us, 3.2 TB/s, eight blocks of keys a wave between a start of three trips to memory and a meeting, and a merge of 3.5 us; its waves wait in 41 %
+// of their time with one block of keys on its way.
 #include "common.h"
 #include "cache4.h"
 

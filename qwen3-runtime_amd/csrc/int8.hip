@@ -9,7 +9,7 @@
 // own, and their whole sums meet in LDS; the order of whole sums does not matter. Eight weight rows a block (the operand's other eight
 // repeat them) leave the busiest compute unit less to fetch where there are few. Weights from memory, us and TB/s: 1 row by 6,144 x 2,560 4.6, 3.4
 // with the row's codes; 24 rows by 2,560 x 9,728 7.7, 3.2 (160 blocks for 256 compute units: more and shorter ones of 8 weight rows took
-// longer); gated, 8 rows by 2 x 9,728 x 2,560 9.8, 5.1. A launch and the first bytes' way are some 2.5 us of each.
+// longer), by 6,144 x 4,096 8.2, 3.1 (384 blocks: 32 weight rows for the busiest unit, 24 on average); gated, 8 rows by 2 x 9,728 x 2,560 9.8, 5.1. A launch and the first bytes' way are some 2.5 us of each.
 #include "common.h"
 #include "direct.h"
 #include "gemm_epilogue.h"
