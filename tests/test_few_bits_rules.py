@@ -248,3 +248,42 @@ def test_a_step_is_the_same_whatever_its_engine_has_served(model_folders, before
     alone, after = run(tail("b", length, 2)), run(tail("a", before, 1), tail("b", length, 2))
     for key, want in alone.items():
         assert (want == after[key]).all(), key
+
+
+@GPU
+def test_decoding_across_the_quarters_of_a_bucket(model_folders):
+    """Steps that leave a graph's quarter, prepared and launched ahead of their ids: the tokens of an engine without graphs."""
+    from qwen3_runtime_amd import LLM, SamplingParams
+
+    prompts = [torch.randint(0, 384, (n,), generator=torch.Generator().manual_seed(n)).tolist() for n in (757, 500)]
+    made = [LLM(str(model_folders["tiny_b"]), dtype="float32", block_size=8, cache_bits=4, max_num_seqs=4, cuda_graph=graph).generate(
+        prompts, SamplingParams(temperature=0.0), max_tokens=30) for graph in (True, False)]
+    assert made[0] == made[1] and [len(x) for x in made[0]] == [30, 30]
+
+
+# ---- rows longer than a block's registers
+
+
+@GPU
+@pytest.mark.parametrize("m,k", [(9, 16384), (9, 25600), (300, 12288), (300, 25600), (3, 8193), (300, 9001), (2, 1 << 17)])
+@pytest.mark.parametrize("dtype", [torch.bfloat16, torch.float32])
+def test_codes_of_rows_that_are_read_twice(m, k, dtype):
+    from test_int8_gpu import codes_of, ops, rnd
+
+    x = rnd(m, k, seed=k, dtype=dtype)
+    x[1, -1] = -1000
+    got, scale = ops().quantize_rows(x)
+    q, s = codes_of(x)
+    assert torch.equal(got[:, :k].float(), q) and not got[:, k:].any() and torch.equal(scale, s)
+
+
+@GPU
+@pytest.mark.parametrize("m", [1, 4, 17, 70])
+@pytest.mark.parametrize("n,k", [(5120, 25600), (40, 1 << 17)])
+def test_products_of_long_rows(m, n, k):
+    from test_int8_gpu import near, ops, product, rnd
+    from qwen3_runtime_amd.ops import Int8Weight
+
+    x, w = rnd(m, k, seed=m, dtype=torch.bfloat16), Int8Weight.quantize(rnd(n, k, seed=n))
+    near(ops().linear(x, w), product(x, w), torch.bfloat16)
+    near(ops().linear_for_residual(x, w), product(x, w), torch.float32)
