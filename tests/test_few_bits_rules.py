@@ -214,7 +214,7 @@ def test_a_graphs_pieces_follow_from_its_key():
 
     for batch in (1, 2, 8, 64):
         for unequal in (False, True):
-            for max_kv in (1, 400, 512, 513, 768, 769, 1024, 2049, 3072, 3073, 4096, 30000):
+            for max_kv in (1, 400, 512, 513, 768, 769, 1024, 1536, 1537, 2049, 4096, 30000):
                 key = DecodeGraph.key_for(batch, max_kv, True, unequal, True)
                 typical = DecodeGraph.typical_lens(key)
                 assert len(typical) == batch and key[1] >= max_kv and max(typical) <= key[1]
